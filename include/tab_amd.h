@@ -270,6 +270,74 @@ int tab_conv2d_packed_out_const(const int64_t *dev_QX, const int64_t *dev_QW, co
 enum { TAB_CONV_AUTO = 0, TAB_CONV_MATRIX = 1, TAB_CONV_POPCOUNT = 2 };
 int tab_set_conv_kernel(int kernel, int tile);
 
+/*
+ * 8-bit layers and the norms around a block.  They have no counterpart in the reference, whose networks keep their first and last layers and
+ * everything between two low-bit layers in fp32; a program needs both next to its ternary and binary layers.
+ *
+ * A packed 8-bit operand of an R x K matrix is
+ *   Q  8-bit numbers [R][128 * ceil(K/128)], zeros past K, 16-byte aligned
+ *   S  E8M0 bytes [ceil(K/128)][R] (blocks of 1 x 128) or [ceil(K/128)][ceil(R/128)] (blocks of 128 x 128)
+ * and stands for Q[r][k] * 2^(S - 127).  Real tensors are fp32, bf16 or fp16, rounded to nearest even where they are written; all sums are
+ * fp32.  Tensors are aligned to their elements and their rows are contiguous; a row stride (ld...) counts elements.
+ */
+enum { TAB_F32 = 0, TAB_BF16 = 1, TAB_F16 = 2 };
+enum { TAB_E4M3 = 0, TAB_E5M2 = 1 }; /* largest numbers 448 and 57344 */
+
+/* ceil(K/128); 0 on bad arguments. */
+int tab_blocks8(int K);
+
+/*
+ * Packs X (M x K).  A block's scale is the smallest power of two from 2^-126 on with which its largest finite magnitude fits the format, so
+ * X / scale is exact and a packed number is the nearest one to X.  NaN stays NaN; an infinity becomes NaN in E4M3 and stays in E5M2; neither
+ * changes its block's scale.
+ *   block_rows  1: blocks of 128 numbers of a row; 128: 128 x 128 (weights)
+ *   dev_Q, dev_S    the packed operand of X, or both NULL
+ *   dev_QT, dev_ST  the packed operand of X transposed (K x M; blocks of 1 x 128 then run down X's columns), or both NULL
+ */
+int tab_quantize8(const void *dev_X, int dtype, int M, int K, long ldx, int block_rows, int format, void *dev_Q, void *dev_S, void *dev_QT,
+                  void *dev_ST, void *stream);
+
+/*
+ * Y (M x N, rows contiguous) = X (M x K, packed) times the transpose of W (N x K, packed in E4M3 with blocks of w_block_rows x 128).  An fp32 Y
+ * is the sum of exact products in fp32 (operands below 2^-126 may count as zeros); towards a 16-bit Y the products of eight neighbours in K keep
+ * 13 bits below the largest of them, some 1.5e-5 of Y's size.
+ *   workspace  tab_linear8_packed_workspace_bytes(out_dtype, M, N, K) bytes, 16-byte aligned; 0 bytes: NULL will do
+ */
+size_t tab_linear8_packed_workspace_bytes(int out_dtype, int M, int N, int K);
+int tab_linear8_packed(const void *dev_QX, int x_format, const void *dev_SX, const void *dev_QW, const void *dev_SW, int w_block_rows, int M, int N,
+                       int K, void *dev_Y, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same with X quantized on the way (E4M3, 1 x 128), Y of X's type; a few rows are quantized and multiplied in one launch. */
+size_t tab_linear8_workspace_bytes(int dtype, int M, int N, int K);
+int tab_linear8(const void *dev_X, int dtype, long ldx, const void *dev_QW, const void *dev_SW, int w_block_rows, int M, int N, int K, void *dev_Y,
+                void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The norm after a block, its gate, the scaled residual, and the norm before the next block, rms(v) = (mean v^2 + eps)^-1/2 over a row:
+ *   R = alpha X + gate * (Y rms(Y) w_post);  H = R rms(R) w_pre     (H is made from R before R is rounded)
+ *   dev_X, dev_Y  M x D of type dtype; dev_Y NULL: no block before this norm, R = X is not written (dev_R, dev_gate, dev_w_post NULL, alpha 1)
+ *   dev_gate      gates x D of type gate_dtype (fp32 or dtype), each row for M/gates consecutive rows, or NULL (1)
+ *   dev_w_post, dev_w_pre  fp32 [D], or NULL (1)
+ *   dev_R         M x D
+ *   dev_H, dev_S  M x D and NULL; or the packed operand of H, E4M3 with blocks of 1 x 128; or both NULL: not wanted
+ * D is at most 16384.
+ */
+int tab_norm_residual(const void *dev_X, long ldx, const void *dev_Y, long ldy, const void *dev_gate, int gate_dtype, int gates,
+                      const float *dev_w_post, const float *dev_w_pre, float alpha, float eps, int dtype, int M, int D, void *dev_R, void *dev_H,
+                      void *dev_S, void *stream);
+
+/*
+ * Its gradients.  dev_dR, dev_dH: those of R and H (M x D, rows contiguous; either may be NULL); R and Y as they were; without a block (dev_Y
+ * NULL) R is the norm's input and dX its gradient (alpha 1).  dev_dX, dev_dY M x D, dev_dgate gates x D of gate_dtype, dev_dw_post and dev_dw_pre fp32 [D]; those
+ * of absent operands NULL, and dev_dgate, dev_dw_post, dev_dw_pre NULL where they are not wanted.  Sums over rows have a fixed order.
+ *   workspace  tab_norm_residual_backward_workspace_bytes(M, D, gates) bytes, 16-byte aligned (gates 0 without a gate)
+ */
+size_t tab_norm_residual_backward_workspace_bytes(int M, int D, int gates);
+int tab_norm_residual_backward(const void *dev_dR, const void *dev_dH, const void *dev_R, const void *dev_Y, const void *dev_gate, int gate_dtype,
+                               int gates, const float *dev_w_post, const float *dev_w_pre, float alpha, float eps, int dtype, int M, int D,
+                               void *dev_dX, void *dev_dY, void *dev_dgate, float *dev_dw_post, float *dev_dw_pre, void *workspace,
+                               size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

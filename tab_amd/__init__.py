@@ -162,6 +162,114 @@ def Conv2dPackedOut(QX, QW, btn, type, padding1, padding2, stride1, stride2, N, 
         return _call(_C.Conv2dPackedOut, {"QX": QX, "QW": QW, "btn": btn}, args, out_thresholds, int(out_bitwidth))
 
 
+E4M3, E5M2 = 0, 1                              # 8-bit formats: largest numbers 448 and 57344
+NORM_NONE, NORM_PLAIN, NORM_8BIT = 0, 1, 2     # what becomes of the norm before the next block
+
+
+def blocks8(K):
+    """Blocks of 128 in a row of K: a packed 8-bit operand of an R x K matrix is Q (R, 128 * blocks8(K)), zeros past K, and S, its
+    power-of-two scales (E8M0), (blocks8(K), R) or, with blocks of 128 x 128, (blocks8(K), blocks8(R))."""
+    return _lib.tab_blocks8(int(K))
+
+
+def Quantize8(X, M, K, block_rows=1, format=E4M3):
+    """Pack X (M x K; fp32, bf16 or fp16; contiguous or rows of a wider matrix) in 8-bit numbers with a power-of-two scale per block of
+    block_rows x 128: the smallest one, from 2^-126, with which the block's largest finite magnitude fits the format.  A packed number is
+    the nearest one to X.  NaN stays NaN, an infinity becomes NaN in E4M3 and stays one in E5M2.  Activations take blocks of one row,
+    weights of 128.  Returns [Q, S]: Q float8_e4m3fn or float8_e5m2, S float8_e8m0fnu."""
+    try:
+        return _C.Quantize8(X, M, K, block_rows, format)
+    except TypeError:
+        return _call(_C.Quantize8, {"X": X}, (M, K, block_rows, format))
+
+
+def Quantize8Transposed(X, M, K, block_rows=1, format=E4M3):
+    """Quantize8 of X transposed (K x M): [QT, ST]; what the gradient of a weight multiplies."""
+    try:
+        return _C.Quantize8Transposed(X, M, K, block_rows, format)
+    except TypeError:
+        return _call(_C.Quantize8Transposed, {"X": X}, (M, K, block_rows, format))
+
+
+def Quantize8Both(X, M, K, block_rows=1, format=E4M3):
+    """Quantize8 and Quantize8Transposed from one reading of X: [Q, S, QT, ST]."""
+    try:
+        return _C.Quantize8Both(X, M, K, block_rows, format)
+    except TypeError:
+        return _call(_C.Quantize8Both, {"X": X}, (M, K, block_rows, format))
+
+
+def Linear8(X, QW, SW, M, N, K):
+    """X (M x K, quantized on the way as Quantize8 does) times the transpose of the packed weight (N x K, E4M3, blocks of 128 x 128 or of
+    one row): Y (M, N) of X's type.  Sums in fp32.  At most 32 rows are quantized and multiplied in one launch."""
+    try:
+        return _C.Linear8(X, QW, SW, M, N, K)
+    except TypeError:
+        return _call(_C.Linear8, {"X": X, "QW": QW, "SW": SW}, (M, N, K))
+
+
+def Linear8Packed(QX, SX, QW, SW, M, N, K, out_dtype=torch.float32):
+    """Linear8 on an activation that is already packed (E4M3 or E5M2, blocks of one row): Y (M, N) of out_dtype."""
+    try:
+        return _C.Linear8Packed(QX, SX, QW, SW, M, N, K, out_dtype)
+    except TypeError:
+        if not isinstance(out_dtype, torch.dtype):
+            raise TypeError("out_dtype must be a torch.dtype")
+        return _call(_C.Linear8Packed, {"QX": QX, "SX": SX, "QW": QW, "SW": SW}, (M, N, K), out_dtype)
+
+
+def _call_norm(fn, required, optional, floats, ints):
+    """As _call, where some tensors may be None."""
+    for name, t in {**required, **optional}.items():
+        if not isinstance(t, torch.Tensor) and not (t is None and name in optional):
+            raise TypeError(f"{name} must be a torch.Tensor" + (" or None" if name in optional else ""))
+    return fn(*required.values(), *optional.values(), *(float(v) for v in floats), *(int(v) for v in ints))
+
+
+def Norm(X, w, eps, M, D, output=NORM_PLAIN):
+    """H = X rms(X) w by rows, rms(v) = (mean v^2 + eps)^-1/2; w fp32 (D,) or None.  Returns [H] of X's type, or with NORM_8BIT the packed
+    operand [QH, SH] that Linear8Packed takes."""
+    try:
+        return _C.Norm(X, w, eps, M, D, output)
+    except TypeError:
+        return _call_norm(_C.Norm, {"X": X}, {"w": w}, (eps,), (M, D, output))
+
+
+def NormResidual(X, Y, gate, w_post, w_pre, alpha, eps, M, D, output=NORM_PLAIN):
+    """The norm after a block, its gate, the scaled residual and the norm before the next block, in one pass:
+
+        R = alpha X + gate * (Y rms(Y) w_post)        H = R rms(R) w_pre
+
+    X, Y (M x D) of one type; gate (G, D), G a divisor of M, each row for M / G consecutive rows (a gate per channel, per sequence or per
+    token), fp32 or X's type, or None; w_post, w_pre fp32 (D,) or None.  Returns [R, H], [R, QH, SH] with NORM_8BIT, [R] with NORM_NONE.
+    D is at most 16384."""
+    try:
+        return _C.NormResidual(X, Y, gate, w_post, w_pre, alpha, eps, M, D, output)
+    except TypeError:
+        for name, t in {"X": X, "Y": Y}.items():
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+        return _call_norm(_C.NormResidual, {"X": X, "Y": Y}, {"gate": gate, "w_post": w_post, "w_pre": w_pre}, (alpha, eps), (M, D, output))
+
+
+def NormResidualBackward(dR, dH, R, Y, gate, w_post, w_pre, alpha, eps, M, D):
+    """Gradients of NormResidual from those of R and H (either may be None), R and Y: [dX, dY, dgate, dw_post, dw_pre], None for a gate or
+    weight that is not there.  The sums over rows have a fixed order: the same call gives the same bits."""
+    try:
+        return _C.NormResidualBackward(dR, dH, R, Y, gate, w_post, w_pre, alpha, eps, M, D)
+    except TypeError:
+        fn = lambda R, Y, dR, dH, *rest: _C.NormResidualBackward(dR, dH, R, Y, *rest)  # noqa: E731
+        return _call_norm(fn, {"R": R, "Y": Y}, {"dR": dR, "dH": dH, "gate": gate, "w_post": w_post, "w_pre": w_pre}, (alpha, eps), (M, D))
+
+
+def NormBackward(dH, X, w, eps, M, D):
+    """Gradients of Norm: [dX, dw]."""
+    try:
+        return _C.NormBackward(dH, X, w, eps, M, D)
+    except TypeError:
+        return _call_norm(_C.NormBackward, {"dH": dH, "X": X}, {"w": w}, (eps,), (M, D))
+
+
 CONV_AUTO, CONV_MATRIX, CONV_POPCOUNT = 0, 1, 2
 
 
@@ -177,4 +285,6 @@ TAB_Conv2d = Conv2d
 
 __all__ = ["Quantize", "QuantizeNCHW", "QuantizeActivation", "conv2d_launches", "QuantizeFormat", "Conv2d", "Conv2dStatic", "static_scratch_bytes", "Conv2dPacked", "Conv2dPackedOut", "Threshold", "TAB_Quantize", "TAB_Conv2d", "TabError",
            "packed_channels", "out_shape", "version", "TNN", "TBN", "BTN", "BNN", "set_conv_kernel",
-           "CONV_AUTO", "CONV_MATRIX", "CONV_POPCOUNT"]
+           "CONV_AUTO", "CONV_MATRIX", "CONV_POPCOUNT",
+           "Quantize8", "Quantize8Transposed", "Quantize8Both", "Linear8", "Linear8Packed", "blocks8", "E4M3", "E5M2",
+           "Norm", "NormResidual", "NormResidualBackward", "NormBackward", "NORM_NONE", "NORM_PLAIN", "NORM_8BIT"]

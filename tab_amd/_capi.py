@@ -39,6 +39,17 @@ SIGNATURES = {
     "tab_layer_quantize": (_int, [_vp, _int, _int, ctypes.c_float] + [_int] * 4 + [_vp, _vp, _sz, _vp]),
     "tab_layer_conv2d": (_int, [_vp, _int, ctypes.c_float, _vp, _vp] + [_int] * 12 + [_vp, _vp, _sz, _vp]),
     "tab_set_conv_kernel": (_int, [_int, _int]),
+    "tab_blocks8": (_int, [_int]),
+    "tab_quantize8": (_int, [_vp, _int, _int, _int, ctypes.c_long, _int, _int, _vp, _vp, _vp, _vp, _vp]),
+    "tab_linear8_packed_workspace_bytes": (_sz, [_int] * 4),
+    "tab_linear8_packed": (_int, [_vp, _int, _vp, _vp, _vp, _int, _int, _int, _int, _vp, _int, _vp, _sz, _vp]),
+    "tab_linear8_workspace_bytes": (_sz, [_int] * 4),
+    "tab_linear8": (_int, [_vp, _int, ctypes.c_long, _vp, _vp, _int, _int, _int, _int, _vp, _vp, _sz, _vp]),
+    "tab_norm_residual": (_int, [_vp, ctypes.c_long, _vp, ctypes.c_long, _vp, _int, _int, _vp, _vp, ctypes.c_float, ctypes.c_float,
+                                 _int, _int, _int, _vp, _vp, _vp, _vp]),
+    "tab_norm_residual_backward_workspace_bytes": (_sz, [_int] * 3),
+    "tab_norm_residual_backward": (_int, [_vp] * 5 + [_int, _int, _vp, _vp, ctypes.c_float, ctypes.c_float, _int, _int, _int] + [_vp] * 6
+                                   + [_sz, _vp]),
 }
 
 

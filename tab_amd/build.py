@@ -7,7 +7,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libtab_amd.so")
 SOURCES = ["tab_capi.hip", "tab_conv.hip", "tab_conv_mfma_tnn.hip", "tab_conv_mfma_tbn.hip", "tab_conv_mfma_btn.hip",
-           "tab_conv_mfma_bnn.hip", "tab_conv_mfma_drf.hip", "tab_conv_mfma_rtn.hip", "tab_conv_fused1x1.hip", "tab_conv_small.hip", "tab_quantize.hip", "tab_quantize_item.hip"]
+           "tab_conv_mfma_bnn.hip", "tab_conv_mfma_drf.hip", "tab_conv_mfma_rtn.hip", "tab_conv_fused1x1.hip", "tab_conv_small.hip", "tab_quantize.hip", "tab_quantize_item.hip",
+           "tab_capi8.hip", "tab_quantize8.hip", "tab_linear8.hip", "tab_norm_residual.hip"]
+EXTENSION_SOURCES = ["torch_binding.cpp", "torch_binding8.cpp"]
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -packed-fp32-ops: keep the compiler from forming packed-FP32 VALU ops from float code.
@@ -48,28 +50,37 @@ def extension_path():
     return os.path.join(HERE, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
+def _run(cmd):
+    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(os.path.basename(cmd[0]) + " failed:\n" + proc.stdout)
+    return proc.stdout
+
+
 def build_torch_extension(verbose=False):
-    """Compile csrc/torch_binding.cpp (host code only: g++, no hipify, no HIP sources) into the
+    """Compile csrc/torch_binding*.cpp (host code only: g++, no hipify, no HIP sources) into the
     CPython extension tab_amd/_C, linked against libtab_amd.so and the torch libraries."""
     import sysconfig
+    from concurrent.futures import ThreadPoolExecutor
 
     import torch
     from torch.utils import cpp_extension
 
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     includes = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], "/opt/rocm/include"]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
-    cmd += ["-I" + i for i in includes]
-    cmd += [os.path.join(CSRC, "torch_binding.cpp"), "-o", extension_path(), "-L" + torch_lib, "-L" + LIB_DIR,
-            "-ltab_amd", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
-            "-Wl,-rpath,$ORIGIN/lib", "-Wl,-rpath," + torch_lib]
-    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError("g++ failed:\n" + proc.stdout)
-    if verbose and proc.stdout.strip():
-        print(proc.stdout)
+    compile = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+               "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
+               "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    compile += ["-I" + i for i in includes]
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    objs = [os.path.join(OBJ_DIR, s.replace(".cpp", ".o")) for s in EXTENSION_SOURCES]
+    with ThreadPoolExecutor(max_workers=len(objs)) as pool:
+        outs = list(pool.map(_run, [compile + ["-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(EXTENSION_SOURCES, objs)]))
+    outs.append(_run(["g++", "-shared", "-o", extension_path()] + objs + ["-L" + torch_lib, "-L" + LIB_DIR,
+                     "-ltab_amd", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
+                     "-Wl,-rpath,$ORIGIN/lib", "-Wl,-rpath," + torch_lib]))
+    if verbose and any(o.strip() for o in outs):
+        print("\n".join(o for o in outs if o.strip()))
     return extension_path()
 
 

@@ -13,8 +13,10 @@
 static __device__ __align__(256) unsigned char scratch[TAB_STATIC_SCRATCH_BYTES];
 
 namespace {
-
 thread_local char g_last_error[512] = "";
+}
+
+namespace tab {
 
 int fail(int status, const char *fmt, ...)
 {
@@ -29,6 +31,13 @@ int device_fail(hipError_t e, const char *what)
 {
     return fail(TAB_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
 }
+
+}  // namespace tab
+
+namespace {
+
+using tab::device_fail;
+using tab::fail;
 
 constexpr long kMaxIndex = 0x7fffffffL;  // kernels index rows/pixels with 32-bit ints
 

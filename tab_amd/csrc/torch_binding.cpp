@@ -3,81 +3,15 @@
 // positional parameter lists, same return tensors; the CPU module's names (TAB_CPU.cpp:636-639)
 // are exported as aliases.  PyTorch only supplies device memory (caching allocator) and the
 // current HIP stream; all compute is in libtab_amd.so.
-#include <torch/extension.h>
+#include "torch_common.h"
 
-#include <ATen/hip/EmptyTensor.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/hip/HIPCachingAllocator.h>
-
-#include <array>
-#include <memory>
-#include <stdexcept>
-#include <tuple>
-#include <vector>
-
-#include "../../include/tab_amd.h"
 #include "tab_route.h"
 
-// CHECK_INPUT of the reference (TAB_GPU.cpp:7-9)
-#define CHECK_CUDA(x) TORCH_CHECK(x.device().is_cuda(), #x " must be a CUDA tensor")
-#define CHECK_CONTIGUOUS(x) TORCH_CHECK(x.is_contiguous(), #x " must be contiguous")
-#define CHECK_INPUT(x) \
-    CHECK_CUDA(x);     \
-    CHECK_CONTIGUOUS(x)
-// The reference converts dtypes with .toType() on a temporary (TAB_GEMM.cu:279-280,341-347),
-// which dangles whenever a conversion really happens; exact dtypes are required instead.
-#define CHECK_DTYPE(x, t) \
-    TORCH_CHECK(x.scalar_type() == torch::t, #x " must have dtype ", dtype_name(torch::t), ", got ", dtype_name(x.scalar_type()))
+using namespace tab_torch;
+
+void bind_layers8(pybind11::module_ &m);  // torch_binding8.cpp
 
 namespace {
-
-std::string dtype_name(torch::ScalarType t)
-{
-    switch (t) {
-    case torch::kFloat32: return "torch.float32";
-    case torch::kInt64: return "torch.int64";
-    case torch::kInt32: return "torch.int32";
-    default: return std::string("torch.") + c10::toString(t);
-    }
-}
-
-// A negative status of a C ABI call; Python sees tab_amd.TabError (a RuntimeError).
-struct StatusError : std::runtime_error {
-    using std::runtime_error::runtime_error;
-};
-
-void check_status(int status)
-{
-    if (status != TAB_OK) throw StatusError(std::string(tab_status_string(status)) + ": " + tab_last_error());
-}
-
-hipStream_t current_stream(const torch::Tensor &t)
-{
-    return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
-}
-
-// Uninitialised device tensor, straight from the caching allocator: torch::empty's way through the dispatcher costs
-// 0.73 us a tensor, this 0.47, beside 2.3 us for a kernel launch.
-torch::Tensor device_empty(c10::IntArrayRef sizes, torch::ScalarType dtype, const torch::Tensor &like)
-{
-    return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
-}
-
-// Device scratch of one call (0.2 us, no tensor around it).  Given back when the call returns: the allocator hands the
-// block only to later work of the same stream.
-class Workspace {
-public:
-    Workspace(size_t bytes, hipStream_t stream)
-        : ptr_(c10::hip::HIPCachingAllocator::raw_alloc_with_stream(bytes, stream)) {}
-    ~Workspace() { c10::hip::HIPCachingAllocator::raw_delete(ptr_); }
-    Workspace(const Workspace &) = delete;
-    Workspace &operator=(const Workspace &) = delete;
-    void *get() const { return ptr_; }
-
-private:
-    void *ptr_;
-};
 
 void quantize_counted(const torch::Tensor &X, const torch::Tensor &thresholds, bool nchw, int bitwidth, int N, int H, int W, int C,
                       const torch::Tensor &QX, const torch::Tensor &BTN)
@@ -699,6 +633,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("Conv2dStatic", &TAB_Conv2dStatic, "Conv2d with the packed activation in the library's built-in scratch");
     m.def("Conv2dPacked", &TAB_Conv2dPacked, "Conv2d on an already packed activation");
     m.def("Conv2dPackedOut", &TAB_Conv2dPackedOut, "Conv2dPacked with the output quantized and packed in the epilogue");
+    bind_layers8(m);
     make_fast<&TAB_Conv2d, 4, 12>(m, "Conv2d");
     make_fast<&TAB_Conv2d, 4, 12, 1>(m, "TAB_Conv2d");
     make_fast<&TAB_Quantize, 2, 5>(m, "Quantize");

@@ -1,6 +1,7 @@
 """Layer wrappers around the two operators: the caller the reference's demo notebook gestures
 at (it imports torch.nn and autograd.Function, TAB Demo CUDA.ipynb cell 1, but ships none).
-Inference only (the operators have no backward).
+Inference only (the operators have no backward).  Beside them the 8-bit layers and the norms around a block (linear8,
+norm_residual, Linear8, ResidualStack), which have one.
 
     layer = TABConv2d.from_float(weight_kn_c_kh_kw, conv_type=tab_amd.TNN, stride=1, padding=1)
     y = layer(x)            # x: (N, C, H, W) fp32 on the GPU -> (N, KN, OH, OW), logical NCHW
@@ -8,7 +9,7 @@ Inference only (the operators have no backward).
 import torch
 from torch import nn
 
-from . import _C, BNN, BTN, TBN, TNN, Quantize, Threshold
+from . import _C, BNN, BTN, E4M3, NORM_8BIT, NORM_PLAIN, TBN, TNN, Linear8Packed, Quantize, Quantize8, Threshold
 
 _ACT_BITS = {TNN: 2, TBN: 2, BTN: 1, BNN: 1}
 _WEIGHT_BITS = {TNN: 2, TBN: 1, BTN: 2, BNN: 1}
@@ -117,3 +118,86 @@ class TABPackedChain(nn.Module):
 
     def forward(self, x):
         return _C.chain_forward(list(self.layers), self.ternary_thresholds, self.data_format == "NCHW", x)
+
+
+def linear8(x, w, grad_format=E4M3):
+    """x (..., K) times the transpose of w (N, K) in 8-bit numbers with a scale per block of 128: y (..., N) of x's type.  Differentiable
+    in x and w: dx = dy w and dw = dy^T x are products of the same kind, dy packed in grad_format (E5M2 where its range needs more than
+    a scale per block of 128 gives) along its rows and its columns.  w is packed anew in every call: for weights that stay, see Linear8."""
+    if not isinstance(x, torch.Tensor) or not isinstance(w, torch.Tensor):
+        raise TypeError("x and w must be torch.Tensors")
+    return _C.linear8(x, w, int(grad_format))
+
+
+def norm_residual(x, y=None, gate=None, w_post=None, w_pre=None, alpha=1.0, eps=1e-6, output=NORM_PLAIN):
+    """tab_amd.NormResidual (with a block's output y) or tab_amd.Norm (without) on tensors (..., D), differentiable in every tensor:
+    [R, H], [R] with output=NORM_NONE, [H] without y.  output=NORM_8BIT gives H packed, for inference."""
+    return _C.norm_residual(x, y, gate, w_post, w_pre, float(alpha), float(eps), int(output))
+
+
+class Linear8(nn.Module):
+    """Fully connected layer on 8-bit numbers, for the layers of a low-bit network that keep more than two bits.  Holds the packed weight
+    (QW, SW) as buffers.  Input (..., in_features) of fp32, bf16 or fp16, or the pair (QH, SH) that a norm packed (then `rows` x out_features
+    of out_dtype); output (..., out_features)."""
+
+    def __init__(self, QW, SW, in_features, out_features, out_dtype=torch.float32):
+        super().__init__()
+        self.in_features, self.out_features, self.out_dtype = int(in_features), int(out_features), out_dtype
+        self.register_buffer("QW", QW)
+        self.register_buffer("SW", SW)
+
+    @classmethod
+    def from_float(cls, weight, out_dtype=torch.float32):
+        """Pack a weight of PyTorch's shape (out_features, in_features) on the GPU."""
+        N, K = weight.shape
+        QW, SW = Quantize8(weight.detach().cuda().contiguous(), N, K, 128)
+        return cls(QW, SW, K, N, out_dtype)
+
+    def forward(self, x):
+        if isinstance(x, (tuple, list)):
+            QX, SX = x
+            return Linear8Packed(QX, SX, self.QW, self.SW, QX.shape[0], self.out_features, self.in_features, self.out_dtype)
+        return _C.linear8_packed_weight(x, self.QW, self.SW, self.out_features, self.in_features)
+
+    def extra_repr(self):
+        return f"{self.in_features}, {self.out_features}"
+
+
+class ResidualStack(nn.Module):
+    """A residual stream through a list of blocks, each between two norms: with x_0 = x and the first norm of x_0 as the first block's input h_0,
+
+        y_i = block_i(h_i),   x_{i+1} = alpha x_i + gate_i * norm(y_i; w_post_i),   h_{i+1} = norm(x_{i+1}; w_pre_{i+1})
+
+    Every block but the last is followed by one NormResidual launch (norm, gate, residual, next norm); the output is the last norm, so that
+    a head can follow.  Blocks map (rows, D) to (rows, D): TABLinear layers, Linear8, or functions of linear8 in training.  With a Linear8 as the
+    next block and no gradient wanted, the norm packs its output for it.  `gates` of a call: one (G, D) tensor or None a block, in place
+    of the learned gate per channel."""
+
+    def __init__(self, blocks, D, alpha=1.0, eps=1e-6, gate_init=1.0, head=None):
+        super().__init__()
+        self.blocks = nn.ModuleList(blocks)
+        if not self.blocks:
+            raise ValueError("at least one block")
+        self.head = head
+        self.D, self.alpha, self.eps = int(D), float(alpha), float(eps)
+        n = len(self.blocks)
+        self.w_pre = nn.ParameterList([nn.Parameter(torch.ones(D)) for _ in range(n + 1)])
+        self.w_post = nn.ParameterList([nn.Parameter(torch.ones(D)) for _ in range(n)])
+        self.gate = nn.ParameterList([nn.Parameter(torch.full((1, D), float(gate_init))) for _ in range(n)])
+
+    def _output(self, i):
+        """How the norm before block i (or before the head) leaves its result."""
+        follower = self.blocks[i] if i < len(self.blocks) else self.head
+        return NORM_8BIT if isinstance(follower, Linear8) and not torch.is_grad_enabled() else NORM_PLAIN
+
+    def forward(self, x, gates=None):
+        if gates is not None and len(gates) != len(self.blocks):
+            raise ValueError(f"{len(gates)} gates for {len(self.blocks)} blocks")
+        shape, x = x.shape, x.reshape(-1, x.shape[-1])
+        h = norm_residual(x, w_pre=self.w_pre[0], eps=self.eps, output=self._output(0))
+        for i, block in enumerate(self.blocks):
+            y = block(h if len(h) > 1 else h[0])
+            gate = self.gate[i] if gates is None or gates[i] is None else gates[i]
+            x, *h = norm_residual(x, y.to(x.dtype), gate, self.w_post[i], self.w_pre[i + 1], self.alpha, self.eps, self._output(i + 1))
+        out = h[0] if self.head is None else self.head(h if len(h) > 1 else h[0])
+        return out.reshape(*shape[:-1], out.shape[-1])
