@@ -125,7 +125,7 @@ long linear8_threads(int out_dtype, int M, int N, int KB);  // of the launch
 hipError_t launch_linear8(int out_dtype, int x_format, const Linear8Args &a, void *workspace, hipStream_t stream);
 
 // The product that quantizes a few rows of x itself.
-bool linear8_rows_supported(int M);
+bool linear8_rows_supported(int M, int K);
 struct Linear8RowsArgs {
     const void *x;
     const uint8_t *qw, *sw;

@@ -125,7 +125,7 @@ int tab_linear8_packed(const void *dev_QX, int x_format, const void *dev_SX, con
 
 size_t tab_linear8_workspace_bytes(int dtype, int M, int N, int K)
 {
-    if (M < 1 || N < 1 || K < 1 || tab::linear8_rows_supported(M)) return 0;
+    if (M < 1 || N < 1 || K < 1 || tab::linear8_rows_supported(M, K)) return 0;
     return packed_bytes(M, K) + tab_linear8_packed_workspace_bytes(dtype, M, N, K);
 }
 
@@ -138,7 +138,7 @@ int tab_linear8(const void *dev_X, int dtype, long ldx, const void *dev_QW, cons
     TAB_CHECK(check_rows(dev_X, dtype, M, K, ldx, "X"));
     TAB_CHECK(check_packed(dev_QW, dev_SW, "QW or SW"));
     TAB_CHECK(check_rows(dev_Y, dtype, 1, N, N, "Y"));
-    if (tab::linear8_rows_supported(M)) {
+    if (tab::linear8_rows_supported(M, K)) {
         const tab::Linear8RowsArgs a = {dev_X, static_cast<const uint8_t *>(dev_QW), static_cast<const uint8_t *>(dev_SW), dev_Y, M, N, K, w_block_rows, ldx};
         const hipError_t e = tab::launch_linear8_rows(dtype, a, static_cast<hipStream_t>(stream));
         return e == hipSuccess ? TAB_OK : device_fail(e, "linear8 launch");

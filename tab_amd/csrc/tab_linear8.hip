@@ -22,7 +22,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kBufferFlags8 = 0x00020000;     // descriptor word 3: untyped 32-bit data
-constexpr uint32_t kNoRow = 0x80000000u;      // an offset past every descriptor here (they end below 2^31): reads zeros
 
 struct TileParams {
     const uint8_t *qx, *sx, *qw, *sw;
@@ -32,20 +31,9 @@ struct TileParams {
     int tiles_m, tiles_n;
 };
 
-template <int FORMAT>
-__device__ __forceinline__ f32x4 mfma16(i32x8 w, i32x8 x, f32x4 c, int w_op, int w_scale, int x_op, int x_scale)
+template <int FORMAT> __device__ __forceinline__ f32x4 mfma16(i32x8 w, i32x8 x, f32x4 c, uint32_t w_scale, uint32_t x_scale)
 {
-    // the scales' byte numbers are immediates
-#define TAB_MFMA(WO, XO) \
-    if (w_op == WO && x_op == XO) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, FORMAT, WO, w_scale, XO, x_scale)
-#define TAB_MFMA4(WO) TAB_MFMA(WO, 0); TAB_MFMA(WO, 1); TAB_MFMA(WO, 2); TAB_MFMA(WO, 3)
-    TAB_MFMA4(0);
-    TAB_MFMA4(1);
-    TAB_MFMA4(2);
-    TAB_MFMA4(3);
-#undef TAB_MFMA4
-#undef TAB_MFMA
-    return c;
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, FORMAT, 0, (int)w_scale, 0, (int)x_scale);
 }
 
 // A lane's 32 numbers of a block times their scale, exactly
@@ -80,25 +68,47 @@ __device__ __forceinline__ f32x4 mfma16_exact(const Exact32 &w, const Exact32 &x
     return c;
 }
 
-__device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t rsrc, uint8_t *dst, uint32_t lane_offset, uint32_t offset)
+// Global memory straight into LDS: 16 bytes a lane at `to` + 16 * lane, or one byte a lane, zero-extended, at `to` + 4 * lane.  A lane offset at or
+// past the end of the buffer gives zeros.  In assembly because of the waits that the compiler puts around the builtin: it has a wave that
+// reads LDS wait for all its loads on the way there, which leaves one step of K in flight at most; here wait_loads counts them.
+// (m0 may not be used by the instruction after its write, nor a scalar register by a memory instruction in the five after a vector
+// instruction's write.)
+__device__ __forceinline__ void to_lds16(i32x4 buffer, uint32_t to, uint32_t lane_offset)
 {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)dst, 16, lane_offset, offset, 0, 0);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer) : "memory");
+}
+__device__ __forceinline__ void to_lds1(i32x4 buffer, uint32_t to, uint32_t lane_offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_ubyte %1, %2, 0 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const uint8_t *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)p; }
+
+// A buffer of `bytes` (below 2^31; none if negative) from p on, the same in every lane: base, size, flags
+__device__ __forceinline__ i32x4 buffer(const uint8_t *p, int bytes)
+{
+    const uint64_t at = (uint64_t)p;
+    return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
+                 __builtin_amdgcn_readfirstlane(max(bytes, 0)), kBufferFlags8};
 }
 
-template <int N> struct ScaleBytes { uint32_t w[(N + 3) / 4]; };
+// This wave's loads but for the last `behind` have landed (s_waitcnt's vmcnt alone; bits 3:0 and 15:14)
+template <int BEHIND> __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70 | (BEHIND & 15) | (BEHIND >> 4) << 14); }
 
-// N scale bytes of a lane, one for each of its wave's 16-row groups
-template <int N> __device__ __forceinline__ ScaleBytes<N> scale_bytes(const uint8_t *p)
+template <int N> struct ScaleWords { uint32_t w[N]; };  // the scales of a lane's N groups of 16 rows
+
+template <int N> __device__ __forceinline__ ScaleWords<N> scale_words(const uint32_t *p)
 {
-    ScaleBytes<N> s;
-    if constexpr (N == 8) {
+    ScaleWords<N> s;
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+            s.w[4 * i] = v.x, s.w[4 * i + 1] = v.y, s.w[4 * i + 2] = v.z, s.w[4 * i + 3] = v.w;
+        }
+    } else {
+        static_assert(N == 2, "groups of 16 rows of a wave");
         const uint2 v = *reinterpret_cast<const uint2 *>(p);
         s.w[0] = v.x, s.w[1] = v.y;
-    } else if constexpr (N == 4) {
-        s.w[0] = *reinterpret_cast<const uint32_t *>(p);
-    } else {
-        static_assert(N == 2, "16-row groups of a wave");
-        s.w[0] = *reinterpret_cast<const uint16_t *>(p);
     }
     return s;
 }
@@ -115,19 +125,19 @@ template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v, int 
     }
 }
 
-// A workgroup of WM x WN waves makes a BM x BN tile of Y.  A step is one block of K: 128 bytes of each of the tile's rows, straight
-// from global memory into LDS, twice over (the next step's land while this one is multiplied), one barrier a step.  A row is eight
-// pieces of 16 bytes; row r has piece g at place g ^ (r & 7), so that the 8 lanes that read at once (8 rows, one piece) meet
-// different banks.  Which piece a lane multiplies is free as long as both operands agree, since a block has one scale.
-template <int BM, int BN, int WM, int WN, int FORMAT, int OUT, bool EXACT>
+// A workgroup of WM x WN waves makes a BM x BN tile of Y.  A step is one block of K: 128 bytes of each of the tile's rows and their scales,
+// straight from global memory into one of STAGES parts of LDS, STAGES - 1 steps ahead, one barrier a step.  A row is eight pieces of 16 bytes; row r
+// has piece g at place g ^ (r & 7), so that the 8 lanes that read at once (8 rows, one piece) meet different banks.  Which piece a lane
+// multiplies is free as long as both operands agree, since a block has one scale.
+template <int BM, int BN, int WM, int WN, int STAGES, int FORMAT, int OUT, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p)
 {
     using T = typename Element<OUT>::type;
-    constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, STAGE = (BM + BN) * kBlock8;
-    static_assert(BM + BN <= THREADS, "a thread stages one scale");
-    constexpr int LOADS = (BM + BN) / 8 / (WM * WN), A_LOADS = BM / 8 / (WM * WN);
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
-    __shared__ __attribute__((aligned(16))) uint8_t scales[2 * (BM + BN)];
+    constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, TM = BM / WM / 16, TN = BN / WN / 16;
+    constexpr int NUMBERS = (BM + BN) * kBlock8, STAGE = NUMBERS + 4 * THREADS;
+    constexpr int LOADS = (BM + BN) / 8 / WAVES, A_LOADS = BM / 8 / WAVES;
+    static_assert(BM + BN <= THREADS, "a lane loads one scale");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
 
     // the tile: parts of K outermost; every XCD (workgroup number modulo 8) takes one run of the tiles, and a run goes through
     // groups of 8 tiles of rows, so that what its CUs hold at one time reads few rows of either operand
@@ -138,34 +148,30 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
     const int m0 = (int)tile_m * BM, n0 = (int)tile_n * BN;
     const int kb0 = (int)part * p.kb_per_part, kb1 = min(p.KB, kb0 + p.kb_per_part);
 
-    const int t = threadIdx.x, lane = t % 64, wave = t / 64, wm = wave / WN, wn = wave % WN, l16 = lane % 16, quarter = lane / 16;
-    const uint32_t row_bytes = (uint32_t)p.KB * kBlock8;
-    const int rows_x = min(BM, p.M - m0), rows_w = min(BN, p.N - n0);
-    const __amdgpu_buffer_rsrc_t x_rsrc =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.qx) + (long)m0 * row_bytes, 0, (int)(rows_x * row_bytes), kBufferFlags8);
-    const __amdgpu_buffer_rsrc_t w_rsrc =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.qw) + (long)n0 * row_bytes, 0, (int)(rows_w * row_bytes), kBufferFlags8);
-    uint32_t offset[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; i++) {
-        const bool x = i < A_LOADS;
-        const int r = ((x ? i : i - A_LOADS) * (WM * WN) + wave) * 8 + lane / 8;
-        offset[i] = r < (x ? rows_x : rows_w) ? (uint32_t)r * row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16 : kNoRow;
-    }
-    auto load = [&](int buf, int kb) {
+    const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64), wm = wave / WN, wn = wave % WN, l16 = lane % 16, quarter = lane / 16;
+    const int row_bytes = p.KB * kBlock8, rows_x = min(BM, p.M - m0), rows_w = min(BN, p.N - n0);
+    const uint8_t *const qx = p.qx + (long)m0 * row_bytes, *const qw = p.qw + (long)n0 * row_bytes;
+    // load i of a wave is rows i * 8 * WAVES + 8 * wave .. + 7 of an operand's tile, eight lanes a row
+    const uint32_t offset = (uint32_t)(wave * 8 + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
+    // this lane's scale has place t of X's or t - BM of W's; the scales of a lane's groups of 16 rows are side by side.  (A wave's scales
+    // are all of X or all of W.)
+    const bool scale_x = wave * 64 < BM, w_rows = p.w_scale_rows == p.N;
+    const int groups = scale_x ? TM : TN, place = scale_x ? t : t - BM, scale_row = place / (16 * groups) * (16 * groups) + place % groups * 16 + place / groups % 16;
+    const uint32_t scale_offset = (uint32_t)(scale_x || w_rows ? scale_row : (n0 + scale_row) / kBlock8 - n0 / kBlock8);
+    const uint8_t *const scales = scale_x ? p.sx + m0 : p.sw + (w_rows ? n0 : n0 / kBlock8);
+    const int scale_step = scale_x ? p.M : p.w_scale_rows, scale_rows = scale_x ? rows_x : wave * 64 >= BM + BN ? 0 : w_rows ? rows_w : (n0 + rows_w - 1) / kBlock8 - n0 / kBlock8 + 1;
+    const uint32_t lds_at = lds_address(lds);
+    auto load = [&](int stage, int kb) {
+        const bool live = kb < kb1;  // past the end: zeros, so that the count of a wave's loads stays the same
+        const uint32_t to = lds_at + (uint32_t)(stage * STAGE);
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const bool x = i < A_LOADS;
-            to_lds16(x ? x_rsrc : w_rsrc, lds + buf * STAGE + (x ? 0 : BM * kBlock8) + ((x ? i : i - A_LOADS) * (WM * WN) + wave) * 1024, offset[i],
-                     (uint32_t)kb * kBlock8);
+            const int row = (x ? i : i - A_LOADS) * 8 * WAVES, bytes = live ? ((x ? rows_x : rows_w) - row) * row_bytes - kb * kBlock8 : 0;
+            to_lds16(buffer((x ? qx : qw) + (long)row * row_bytes + kb * kBlock8, bytes), to + (uint32_t)((x ? 0 : BM * kBlock8) + (row + wave * 8) * kBlock8), offset);
         }
+        to_lds1(buffer(scales + (long)kb * scale_step, live ? scale_rows : 0), to + (uint32_t)(NUMBERS + wave * 256), scale_offset);
     };
-    // this thread's scale: of row t of the tile, or of column t - BM; a lane reads those of its 16-row groups side by side
-    const bool x_scale = t < BM, stages = t < BM + BN;
-    const int r = x_scale ? t : t - BM, group16 = 16 * (x_scale ? TM : TN);
-    const int scale_at = (x_scale ? 0 : BM) + r / group16 * group16 + (r % 16) * (x_scale ? TM : TN) + r % group16 / 16;
-    const long scale_step = x_scale ? p.M : p.w_scale_rows;
-    const uint8_t *scale_from = x_scale ? p.sx + min(m0 + r, p.M - 1) : p.sw + (p.w_scale_rows == p.N ? min(n0 + r, p.N - 1) : min(n0 + r, p.N - 1) / kBlock8);
 
     f32x4 acc[TM][TN];
 #pragma unroll
@@ -173,50 +179,48 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    load(0, kb0);
-    if (stages) scales[scale_at] = scale_from[kb0 * scale_step];
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) load(i, kb0 + i);
+    int stage = 0;
     for (int kb = kb0; kb < kb1; kb++) {
-        const int buf = (kb - kb0) & 1;
-        __builtin_amdgcn_s_waitcnt(0);  // this wave's part of the step has landed
-        __syncthreads();
-        const bool more = kb + 1 < kb1;
-        uint8_t next_scale = 0;
-        if (more) {
-            load(buf ^ 1, kb + 1);
-            if (stages) next_scale = scale_from[(kb + 1) * scale_step];
-        }
-        const uint8_t *a_lds = lds + buf * STAGE + (wm * 16 * TM + l16) * kBlock8, *b_lds = lds + buf * STAGE + (BM + wn * 16 * TN + l16) * kBlock8;
+        wait_loads<(STAGES - 2) * (LOADS + 1)>();  // this wave's part of the step has landed
+        __builtin_amdgcn_s_barrier();              // and the others', and all have read what the loads below overwrite
+        load(stage == 0 ? STAGES - 1 : stage - 1, kb + STAGES - 1);
+        const uint8_t *from = lds + stage * STAGE;
+        const uint8_t *a_lds = from + (wm * 16 * TM + l16) * kBlock8, *b_lds = from + (BM + wn * 16 * TN + l16) * kBlock8;
+        const uint32_t *s_lds = reinterpret_cast<const uint32_t *>(from + NUMBERS);
         // pieces `quarter` and `quarter` + 4 of the row
         const int at0 = (quarter ^ (l16 & 7)) * 16, at1 = at0 ^ 64;
-        const ScaleBytes<TM> sx = scale_bytes<TM>(scales + buf * (BM + BN) + (wm * 16 + l16) * TM);
-        const ScaleBytes<TN> sw = scale_bytes<TN>(scales + buf * (BM + BN) + BM + (wn * 16 + l16) * TN);
-        auto fragment = [&](const uint8_t *from, int group) {
-            const i32x4 low = *reinterpret_cast<const i32x4 *>(from + group * 16 * kBlock8 + at0), high = *reinterpret_cast<const i32x4 *>(from + group * 16 * kBlock8 + at1);
+        auto fragment = [&](const uint8_t *p, int group) {
+            const i32x4 low = *reinterpret_cast<const i32x4 *>(p + group * 16 * kBlock8 + at0), high = *reinterpret_cast<const i32x4 *>(p + group * 16 * kBlock8 + at1);
             return (i32x8)__builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
         };
+        const ScaleWords<TM> sx = scale_words<TM>(s_lds + (wm * 16 + l16) * TM);
+        const ScaleWords<TN> sw = scale_words<TN>(s_lds + BM + (wn * 16 + l16) * TN);
+        i32x8 wq[TN], xq[TM];
+#pragma unroll
+        for (int j = 0; j < TN; j++) wq[j] = fragment(b_lds, j);
+#pragma unroll
+        for (int i = 0; i < TM; i++) xq[i] = fragment(a_lds, i);
         if constexpr (EXACT) {
             Exact32 wf[TN];
 #pragma unroll
-            for (int j = 0; j < TN; j++) wf[j] = exact32<0>(fragment(b_lds, j), sw.w[j / 4] >> 8 * (j % 4) & 255u);
+            for (int j = 0; j < TN; j++) wf[j] = exact32<0>(wq[j], sw.w[j]);
 #pragma unroll
             for (int i = 0; i < TM; i++) {
-                const Exact32 xf = exact32<FORMAT>(fragment(a_lds, i), sx.w[i / 4] >> 8 * (i % 4) & 255u);
+                const Exact32 xf = exact32<FORMAT>(xq[i], sx.w[i]);
 #pragma unroll
                 for (int j = 0; j < TN; j++) acc[i][j] = mfma16_exact(wf[j], xf, acc[i][j]);
             }
         } else {
-            i32x8 wf[TN];
 #pragma unroll
-            for (int j = 0; j < TN; j++) wf[j] = fragment(b_lds, j);
+            for (int i = 0; i < TM; i++)
 #pragma unroll
-            for (int i = 0; i < TM; i++) {
-                const i32x8 xf = fragment(a_lds, i);
-#pragma unroll
-                for (int j = 0; j < TN; j++) acc[i][j] = mfma16<FORMAT>(wf[j], xf, acc[i][j], j % 4, (int)sw.w[j / 4], i % 4, (int)sx.w[i / 4]);
-            }
+                for (int j = 0; j < TN; j++) acc[i][j] = mfma16<FORMAT>(wq[j], xq[i], acc[i][j], sw.w[j], sx.w[i]);
         }
-        if (more && stages) scales[(buf ^ 1) * (BM + BN) + scale_at] = next_scale;
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
+    wait_loads<0>();  // nothing is on its way to LDS when the workgroup ends
 
     // the weights are the instruction's rows: a lane holds four neighbours of one row of Y
     T *y = static_cast<T *>(p.y) + (long)part * p.M * p.N;
@@ -251,43 +255,41 @@ template <int OUT> __global__ __launch_bounds__(256) void linear8_join(const flo
     }
 }
 
-// Few rows: bound by reading QW once, so nothing is shared through LDS on the way.  A workgroup takes 16 rows of QW and all (at most
-// 16 * MT) rows of X, its waves take the blocks of K in turn, each lane loads its 2 x 16 bytes of a block itself, and the waves' sums meet
-// in LDS, added up in a fixed order.  INPUT 0 .. 2: X is fp32 / bf16 / fp16 and every wave quantizes the blocks it multiplies (a row's block
-// lies in 4 lanes); 3: packed.
+// Few rows: bound by reading QW once.  A workgroup takes some groups of 16 rows of QW and all (at most 16 * MT) rows of X.  Its waves take the blocks of
+// K in turn, each lane loads its 2 x 16 bytes of a block of QW itself, AHEAD blocks at a time, and the waves' sums meet in LDS, added up in a
+// fixed order.  X lies in LDS as packed numbers (rows 16 bytes more than whole blocks apart, so that 8 rows' pieces meet different banks) and scales:
+// INPUT 0 .. 2: fp32 / bf16 / fp16, quantized by the workgroup on the way (a block of a row is 16 lanes of eight); 3: packed.
 struct RowsParams {
     const void *x;
     const uint8_t *sx, *qw, *sw;
     void *y;
-    int M, N, K, KB, w_scale_rows;
+    int M, N, K, KB, w_scale_rows, groups_each;
     long ldx;
 };
 
-template <typename T> __device__ __forceinline__ void load16(const T *row, int k, int K, bool there, float *v)
-{
-    float a[8], b[8];
-    load8(row + k, there ? K - k : 0, a);
-    load8(row + k + 8, there ? K - k - 8 : 0, b);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = a[i], v[8 + i] = b[i];
-}
+constexpr int kRowsMost = 32;           // rows of X
+constexpr int kRowsLds = 64 << 10;      // bytes of X in LDS
+constexpr int kRowsWaves = 8;
 
-template <int INPUT, int FORMAT, int OUT, int MT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void linear8_rows(const RowsParams p)
+__host__ __device__ __forceinline__ int rows_stride(int KB) { return KB * kBlock8 + 16; }
+__host__ __device__ __forceinline__ int rows_lds(int M, int KB) { return M * (rows_stride(KB) + KB * 4); }  // numbers, then scales as words [KB][M]
+
+template <int INPUT, int FORMAT, int OUT, int MT>
+__global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams p)
 {
     using T = typename Element<OUT>::type;
+    constexpr int WAVES = kRowsWaves, AHEAD = 4;
+    extern __shared__ __attribute__((aligned(16))) uint8_t packed[];
     __shared__ __attribute__((aligned(16))) float sums[WAVES * MT * 256];
-    const int t = threadIdx.x, lane = t % 64, wave = t / 64, l16 = lane % 16, quarter = lane / 16;
-    const int n0 = blockIdx.x * 16, row_w = min(n0 + l16, p.N - 1);
-    const uint8_t *w = p.qw + (long)row_w * p.KB * kBlock8 + quarter * 16;
-    const uint8_t *sw = p.sw + (p.w_scale_rows == p.N ? row_w : row_w / kBlock8);
-    f32x4 acc[MT];
-#pragma unroll
-    for (int i = 0; i < MT; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int AHEAD = 4;  // blocks of QW that a lane has in flight
-    for (int first = wave; first < p.KB; first += AHEAD * WAVES) {
-        i32x4 w_low[AHEAD], w_high[AHEAD];
-        int w_scale[AHEAD];
+    const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64), l16 = lane % 16, quarter = lane / 16;
+    const int stride = rows_stride(p.KB);
+    uint32_t *const scales = reinterpret_cast<uint32_t *>(packed + p.M * stride);
+    const bool w_rows = p.w_scale_rows == p.N;
+    i32x4 w_low[AHEAD], w_high[AHEAD];
+    uint32_t w_scale[AHEAD];
+    auto load = [&](int n0, int first) {
+        const int row = min(n0 + l16, p.N - 1);
+        const uint8_t *const w = p.qw + (long)row * p.KB * kBlock8 + quarter * 16, *const sw = p.sw + (w_rows ? row : row / kBlock8);
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             const long kb = min(first + u * WAVES, p.KB - 1);
@@ -295,64 +297,81 @@ __global__ __launch_bounds__(64 * WAVES) void linear8_rows(const RowsParams p)
             w_high[u] = *reinterpret_cast<const i32x4 *>(w + kb * kBlock8 + 64);
             w_scale[u] = sw[kb * p.w_scale_rows];
         }
+    };
+    const int groups = (p.N + 15) / 16, group0 = (int)blockIdx.x * p.groups_each, group1 = min(groups, group0 + p.groups_each);
+    load(group0 * 16, wave);
+
+    // X into LDS: blocks in the order of memory, 16 lanes a block
+    for (int block = t / 16; block < p.M * p.KB; block += 64 * WAVES / 16) {
+        const int m = block / p.KB, kb = block - m * p.KB;
+        uint8_t *const to = packed + m * stride + kb * kBlock8 + l16 * 8;
+        if constexpr (INPUT == 3) {
+            *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p.x) + (long)block * kBlock8 + l16 * 8);
+            if (l16 == 0) scales[kb * p.M + m] = p.sx[(long)kb * p.M + m];
+        } else {
+            using X = typename Element<INPUT>::type;
+            const int k = kb * kBlock8 + l16 * 8;
+            float v[8];
+            load8(static_cast<const X *>(p.x) + m * p.ldx + k, p.K - k, v);
+            uint32_t amax = 0;
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++) {
-            const int kb = first + u * WAVES;
-            if (kb >= p.KB) break;  // (the same for the whole wave)
-            const i32x8 wf = __builtin_shufflevector(w_low[u], w_high[u], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-            for (int i = 0; i < MT; i++) {
-                const int m = i * 16 + l16;
-                const bool there = m < p.M;
-                i32x8 xf = {0, 0, 0, 0, 0, 0, 0, 0};
-                int x_scale = 1;
-                if constexpr (INPUT == 3) {
-                    if (there) {
-                        const uint8_t *x = static_cast<const uint8_t *>(p.x) + ((long)m * p.KB + kb) * kBlock8 + quarter * 16;
-                        const i32x4 a = *reinterpret_cast<const i32x4 *>(x), c = *reinterpret_cast<const i32x4 *>(x + 64);
-                        xf = __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
-                        x_scale = p.sx[(long)kb * p.M + m];
-                    }
-                } else {
-                    using X = typename Element<INPUT>::type;
-                    const X *row = static_cast<const X *>(p.x) + m * p.ldx;
-                    float v[32];
-                    load16(row, kb * kBlock8 + quarter * 16, p.K, there, v);
-                    load16(row, kb * kBlock8 + 64 + quarter * 16, p.K, there, v + 16);
-                    uint32_t amax = 0;
-#pragma unroll
-                    for (int j = 0; j < 32; j++) amax = max(amax, finite_bits(v[j]));
-                    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
-                    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-                    x_scale = (int)scale_byte<FORMAT>(amax);
-                    const float inv = inverse_scale((uint32_t)x_scale);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) xf[j] = (int)pack4<FORMAT>(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], inv);
-                }
-                if constexpr (OUT == 0) acc[i] = mfma16_exact(exact32<0>(wf, (uint32_t)w_scale[u]), exact32<FORMAT>(xf, (uint32_t)x_scale), acc[i]);
-                else acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[i], 0, FORMAT, 0, w_scale[u], 0, x_scale);
-            }
+            for (int j = 0; j < 8; j++) amax = max(amax, finite_bits(v[j]));
+            const uint32_t byte = scale_byte<FORMAT>(max_of_row16(amax));
+            const float inv = inverse_scale(byte);
+            *reinterpret_cast<uint2 *>(to) = uint2{pack4<FORMAT>(v[0], v[1], v[2], v[3], inv), pack4<FORMAT>(v[4], v[5], v[6], v[7], inv)};
+            if (l16 == 0) scales[kb * p.M + m] = byte;
         }
     }
-#pragma unroll
-    for (int i = 0; i < MT; i++) *reinterpret_cast<f32x4 *>(sums + (wave * MT + i) * 256 + l16 * 16 + quarter * 4) = acc[i];
     __syncthreads();
-    for (int i = t; i < MT * 256; i += 64 * WAVES) {
-        const int m = i / 16, n = n0 + i % 16;
-        float sum = sums[i];
+
+    for (int group = group0; group < group1; group++) {
+        const int n0 = group * 16;
+        f32x4 acc[MT];
 #pragma unroll
-        for (int k = 1; k < WAVES; k++) sum += sums[k * MT * 256 + i];
-        if (m < p.M && n < p.N) static_cast<T *>(p.y)[(long)m * p.N + n] = (T)sum;
+        for (int i = 0; i < MT; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int first = wave; first < p.KB; first += AHEAD * WAVES) {
+            if (first != wave) load(n0, first);
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                const int kb = first + u * WAVES;
+                if (kb >= p.KB) break;  // (the same for the whole wave)
+                const i32x8 wf = __builtin_shufflevector(w_low[u], w_high[u], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    const int m = min(i * 16 + l16, p.M - 1);  // (columns past M repeat the last one and are not stored)
+                    const uint8_t *const x = packed + m * stride + kb * kBlock8 + quarter * 16;
+                    const i32x4 low = *reinterpret_cast<const i32x4 *>(x), high = *reinterpret_cast<const i32x4 *>(x + 64);
+                    const i32x8 xf = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+                    const uint32_t x_scale = scales[kb * p.M + m];
+                    if constexpr (OUT == 0) acc[i] = mfma16_exact(exact32<0>(wf, w_scale[u]), exact32<FORMAT>(xf, x_scale), acc[i]);
+                    else acc[i] = mfma16<FORMAT>(wf, xf, acc[i], w_scale[u], x_scale);
+                }
+            }
+        }
+        if (group + 1 < group1) load(n0 + 16, wave);  // the next group's first blocks, on their way while the sums meet
+#pragma unroll
+        for (int i = 0; i < MT; i++) *reinterpret_cast<f32x4 *>(sums + (wave * MT + i) * 256 + l16 * 16 + quarter * 4) = acc[i];
+        __syncthreads();
+        for (int i = t; i < MT * 256; i += 64 * WAVES) {
+            const int m = i / 16, n = n0 + i % 16;
+            float sum = sums[i];
+#pragma unroll
+            for (int k = 1; k < WAVES; k++) sum += sums[k * MT * 256 + i];
+            if (m < p.M && n < p.N) static_cast<T *>(p.y)[(long)m * p.N + n] = (T)sum;
+        }
+        if (group + 1 < group1) __syncthreads();
     }
 }
 
-constexpr int kRowsMost = 32;  // rows of X that linear8_rows takes
+bool rows_fit(int M, int KB) { return M <= kRowsMost && (long)rows_lds(M, 1) * KB <= kRowsLds; }
 
-template <int INPUT, int FORMAT, int OUT> hipError_t launch_rows(const RowsParams &p, hipStream_t stream)
+template <int INPUT, int FORMAT, int OUT> hipError_t launch_rows(RowsParams p, hipStream_t stream)
 {
-    const unsigned groups = (unsigned)((p.N + 15) / 16);
-    if (p.M <= 16) linear8_rows<INPUT, FORMAT, OUT, 1, 8><<<groups, 512, 0, stream>>>(p);
-    else linear8_rows<INPUT, FORMAT, OUT, 2, 8><<<groups, 512, 0, stream>>>(p);
+    const int groups = (p.N + 15) / 16;
+    p.groups_each = (groups + 511) / 512;  // two workgroups a CU, each with X in its LDS once
+    const unsigned workgroups = (unsigned)((groups + p.groups_each - 1) / p.groups_each), lds = (unsigned)rows_lds(p.M, p.KB);
+    if (p.M <= 16) linear8_rows<INPUT, FORMAT, OUT, 1><<<workgroups, 64 * kRowsWaves, lds, stream>>>(p);
+    else linear8_rows<INPUT, FORMAT, OUT, 2><<<workgroups, 64 * kRowsWaves, lds, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -368,7 +387,7 @@ Plan8 plan8(int out, int M, int N, int KB)
     const int tile = out != 0 && tiles(256) >= 256 ? 256 : tiles(128) >= 128 ? 128 : 64;
     int parts = 1;
     const long have = tiles(tile);
-    while (have * parts * 2 <= 512 && KB / (parts * 2) >= 4) parts *= 2;
+    while (have * parts * 2 <= (tile == 256 ? 256 : 512) && KB / (parts * 2) >= 4) parts *= 2;
     const int per = (KB + parts - 1) / parts;
     return {tile, (KB + per - 1) / per, per};
 }
@@ -377,19 +396,19 @@ template <int FORMAT, int OUT, bool EXACT> hipError_t launch_tiles(int tile, uns
 {
     if constexpr (!EXACT)
         if (tile == 256) {
-            linear8_tiles<256, 256, 2, 4, FORMAT, OUT, EXACT><<<groups, 512, 0, stream>>>(p);
+            linear8_tiles<256, 256, 2, 4, 2, FORMAT, OUT, EXACT><<<groups, 512, 0, stream>>>(p);
             return hipGetLastError();
         }
-    if (tile == 128) linear8_tiles<128, 128, 2, 2, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
-    else linear8_tiles<64, 64, 2, 2, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
+    if (tile == 128) linear8_tiles<128, 128, 2, 2, 2, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
+    else linear8_tiles<64, 64, 2, 2, 4, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 
 template <int FORMAT> hipError_t launch_format(int out, const Linear8Args &a, void *workspace, hipStream_t stream)
 {
     const int scale_rows = w_scale_rows(a.N, a.w_block_rows);
-    if (a.M <= kRowsMost) {
-        const RowsParams p = {a.qx, a.sx, a.qw, a.sw, a.y, a.M, a.N, a.KB * kBlock8, a.KB, scale_rows, 0};
+    if (rows_fit(a.M, a.KB)) {
+        const RowsParams p = {a.qx, a.sx, a.qw, a.sw, a.y, a.M, a.N, a.KB * kBlock8, a.KB, scale_rows, 0, 0};
         return out == 0 ? launch_rows<3, FORMAT, 0>(p, stream) : out == 1 ? launch_rows<3, FORMAT, 1>(p, stream) : launch_rows<3, FORMAT, 2>(p, stream);
     }
     const Plan8 plan = plan8(out, a.M, a.N, a.KB);
@@ -414,14 +433,14 @@ template <int FORMAT> hipError_t launch_format(int out, const Linear8Args &a, vo
 
 size_t linear8_workspace(int out_dtype, int M, int N, int KB)
 {
-    if (M <= kRowsMost) return 0;
+    if (rows_fit(M, KB)) return 0;
     const Plan8 plan = plan8(out_dtype, M, N, KB);
     return plan.parts > 1 ? (size_t)plan.parts * (size_t)M * (size_t)N * sizeof(float) : 0;
 }
 
 long linear8_threads(int out_dtype, int M, int N, int KB)
 {
-    if (M <= kRowsMost) return ((long)N + 15) / 16 * 512;
+    if (rows_fit(M, KB)) return 0;  // (at most 512 workgroups)
     const Plan8 plan = plan8(out_dtype, M, N, KB);
     const long edge = plan.tile;
     return ((M + edge - 1) / edge) * ((N + edge - 1) / edge) * plan.parts * (edge == 256 ? 512 : 256);
@@ -432,11 +451,11 @@ hipError_t launch_linear8(int out_dtype, int x_format, const Linear8Args &a, voi
     return x_format == 0 ? launch_format<0>(out_dtype, a, workspace, stream) : launch_format<1>(out_dtype, a, workspace, stream);
 }
 
-bool linear8_rows_supported(int M) { return M <= kRowsMost; }
+bool linear8_rows_supported(int M, int K) { return rows_fit(M, blocks8(K)); }
 
 hipError_t launch_linear8_rows(int dtype, const Linear8RowsArgs &a, hipStream_t stream)
 {
-    const RowsParams p = {a.x, nullptr, a.qw, a.sw, a.y, a.M, a.N, a.K, blocks8(a.K), w_scale_rows(a.N, a.w_block_rows), a.ldx};
+    const RowsParams p = {a.x, nullptr, a.qw, a.sw, a.y, a.M, a.N, a.K, blocks8(a.K), w_scale_rows(a.N, a.w_block_rows), 0, a.ldx};
     return dtype == 0 ? launch_rows<0, 0, 0>(p, stream) : dtype == 1 ? launch_rows<1, 0, 1>(p, stream) : launch_rows<2, 0, 2>(p, stream);
 }
 
