@@ -126,9 +126,13 @@ template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v, int 
 }
 
 // A workgroup of WM x WN waves makes a BM x BN tile of Y.  A step is one block of K: 128 bytes of each of the tile's rows and their scales,
-// straight from global memory into one of STAGES parts of LDS, STAGES - 1 steps ahead, one barrier a step.  A row is eight pieces of 16 bytes; row r
-// has piece g at place g ^ (r & 7), so that the 8 lanes that read at once (8 rows, one piece) meet different banks.  Which piece a lane
-// multiplies is free as long as both operands agree, since a block has one scale.
+// straight from global memory into one of STAGES parts of LDS.  A row is eight pieces of 16 bytes; row r has piece g at place g ^ (r & 7), so
+// that lanes that read at once meet different banks.  Which piece a lane multiplies is free as long as both operands agree, since a block
+// has one scale.
+//
+// The loads are what bounds the largest tile: 72 instructions of 1 KB a step take a CU some 2900 cycles, its products 2048.  So the loads never run
+// dry: a step begins when its part of LDS has landed (one barrier), the waves read all their fragments, and as soon as they have them
+// (another barrier) the loads of the step STAGES ahead follow those still on their way, between the products.
 template <int BM, int BN, int WM, int WN, int STAGES, int FORMAT, int OUT, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p)
 {
@@ -161,16 +165,17 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
     const uint8_t *const scales = scale_x ? p.sx + m0 : p.sw + (w_rows ? n0 : n0 / kBlock8);
     const int scale_step = scale_x ? p.M : p.w_scale_rows, scale_rows = scale_x ? rows_x : wave * 64 >= BM + BN ? 0 : w_rows ? rows_w : (n0 + rows_w - 1) / kBlock8 - n0 / kBlock8 + 1;
     const uint32_t lds_at = lds_address(lds);
-    auto load = [&](int stage, int kb) {
-        const bool live = kb < kb1;  // past the end: zeros, so that the count of a wave's loads stays the same
+    // load i of a step, the scales last; past the end of K zeros, so that the count of a wave's loads stays the same
+    auto load = [&](int stage, int kb, int i) {
+        const bool live = kb < kb1;
         const uint32_t to = lds_at + (uint32_t)(stage * STAGE);
-#pragma unroll
-        for (int i = 0; i < LOADS; i++) {
+        if (i < LOADS) {
             const bool x = i < A_LOADS;
             const int row = (x ? i : i - A_LOADS) * 8 * WAVES, bytes = live ? ((x ? rows_x : rows_w) - row) * row_bytes - kb * kBlock8 : 0;
             to_lds16(buffer((x ? qx : qw) + (long)row * row_bytes + kb * kBlock8, bytes), to + (uint32_t)((x ? 0 : BM * kBlock8) + (row + wave * 8) * kBlock8), offset);
+        } else {
+            to_lds1(buffer(scales + (long)kb * scale_step, live ? scale_rows : 0), to + (uint32_t)(NUMBERS + wave * 256), scale_offset);
         }
-        to_lds1(buffer(scales + (long)kb * scale_step, live ? scale_rows : 0), to + (uint32_t)(NUMBERS + wave * 256), scale_offset);
     };
 
     f32x4 acc[TM][TN];
@@ -179,59 +184,95 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    const int at0 = (quarter ^ (l16 & 7)) * 16, at1 = at0 ^ 64;  // pieces `quarter` and `quarter` + 4 of a row
+    const int a_at = (wm * 16 * TM + l16) * kBlock8, b_at = (BM + wn * 16 * TN + l16) * kBlock8;
+    auto fragment = [&](const uint8_t *from, int group) {
+        const i32x4 low = *reinterpret_cast<const i32x4 *>(from + group * 16 * kBlock8 + at0), high = *reinterpret_cast<const i32x4 *>(from + group * 16 * kBlock8 + at1);
+        return (i32x8)__builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    constexpr int BEFORE = TM > 4 ? 3 : TM / 2;  // rows of 16 multiplied while the step's other fragments are read
+    constexpr int EACH = (LOADS + TM - BEFORE) / (TM - BEFORE);  // loads behind each of the other rows
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) load(i, kb0 + i);
+    for (int k = 0; k < STAGES; k++)
+#pragma unroll
+        for (int i = 0; i <= LOADS; i++) load(k, kb0 + k, i);
     int stage = 0;
     for (int kb = kb0; kb < kb1; kb++) {
-        wait_loads<(STAGES - 2) * (LOADS + 1)>();  // this wave's part of the step has landed
-        __builtin_amdgcn_s_barrier();              // and the others', and all have read what the loads below overwrite
-        load(stage == 0 ? STAGES - 1 : stage - 1, kb + STAGES - 1);
-        const uint8_t *from = lds + stage * STAGE;
-        const uint8_t *a_lds = from + (wm * 16 * TM + l16) * kBlock8, *b_lds = from + (BM + wn * 16 * TN + l16) * kBlock8;
-        const uint32_t *s_lds = reinterpret_cast<const uint32_t *>(from + NUMBERS);
-        // pieces `quarter` and `quarter` + 4 of the row
-        const int at0 = (quarter ^ (l16 & 7)) * 16, at1 = at0 ^ 64;
-        auto fragment = [&](const uint8_t *p, int group) {
-            const i32x4 low = *reinterpret_cast<const i32x4 *>(p + group * 16 * kBlock8 + at0), high = *reinterpret_cast<const i32x4 *>(p + group * 16 * kBlock8 + at1);
-            return (i32x8)__builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
-        };
-        const ScaleWords<TM> sx = scale_words<TM>(s_lds + (wm * 16 + l16) * TM);
+        wait_loads<(STAGES - 1) * (LOADS + 1)>();  // this wave's part of the step has landed,
+        __builtin_amdgcn_s_barrier();              // and the others'
+        asm volatile("" ::: "memory");
+        const uint8_t *const from = lds + stage * STAGE;
+        const uint32_t *const s_lds = reinterpret_cast<const uint32_t *>(from + NUMBERS);
         const ScaleWords<TN> sw = scale_words<TN>(s_lds + BM + (wn * 16 + l16) * TN);
+        const ScaleWords<TM> sx = scale_words<TM>(s_lds + (wm * 16 + l16) * TM);
         i32x8 wq[TN], xq[TM];
+        Exact32 wf[EXACT ? TN : 1];
 #pragma unroll
-        for (int j = 0; j < TN; j++) wq[j] = fragment(b_lds, j);
+        for (int j = 0; j < TN; j++) wq[j] = fragment(from + b_at, j);
 #pragma unroll
-        for (int i = 0; i < TM; i++) xq[i] = fragment(a_lds, i);
-        if constexpr (EXACT) {
-            Exact32 wf[TN];
+        for (int i = 0; i < TM; i++) xq[i] = fragment(from + a_at, i);
+        __builtin_amdgcn_sched_barrier(0);
+        auto row = [&](int i) {
+            if constexpr (EXACT) {
+                if (i == 0) {
 #pragma unroll
-            for (int j = 0; j < TN; j++) wf[j] = exact32<0>(wq[j], sw.w[j]);
-#pragma unroll
-            for (int i = 0; i < TM; i++) {
+                    for (int j = 0; j < TN; j++) wf[j] = exact32<0>(wq[j], sw.w[j]);
+                }
                 const Exact32 xf = exact32<FORMAT>(xq[i], sx.w[i]);
 #pragma unroll
                 for (int j = 0; j < TN; j++) acc[i][j] = mfma16_exact(wf[j], xf, acc[i][j]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < TM; i++)
+            } else {
 #pragma unroll
                 for (int j = 0; j < TN; j++) acc[i][j] = mfma16<FORMAT>(wq[j], xq[i], acc[i][j], sw.w[j], sx.w[i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int i = 0; i < BEFORE; i++) row(i);
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave has read all of the step,
+        __builtin_amdgcn_s_barrier();        // and the others
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = BEFORE; i < TM; i++) {
+#pragma unroll
+            for (int k = (i - BEFORE) * EACH; k < (i - BEFORE + 1) * EACH && k <= LOADS; k++) load(stage, kb + STAGES, k);
+            row(i);
         }
         stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
-    wait_loads<0>();  // nothing is on its way to LDS when the workgroup ends
+    wait_loads<0>();  // nothing is on its way to LDS any more,
+    __builtin_amdgcn_s_barrier();  // and every wave has read its last step: LDS is free
+    asm volatile("" ::: "memory");
 
-    // the weights are the instruction's rows: a lane holds four neighbours of one row of Y
-    T *y = static_cast<T *>(p.y) + (long)part * p.M * p.N;
+    // The weights are the instruction's rows: a lane holds four neighbours of one row of Y.  Rows of 16 at a time go through a part of LDS of the
+    // wave's own, so that they are stored in pieces of 16 bytes and whole cache lines (four neighbours a lane, straight from the registers:
+    // 25 us for a tile of 256 x 256, a fifth of 8192^3).
+    constexpr int V = 16 / (int)sizeof(T), PIECES = TN * 16 / V, PITCH = TN * 16 * (int)sizeof(T) + 16;
+    static_assert(WAVES * 16 * PITCH <= STAGES * STAGE, "the waves' parts fit");
+    uint8_t *const mine = lds + wave * (16 * PITCH);
+    T *const y = static_cast<T *>(p.y) + (long)part * p.M * p.N;
+    struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[V]; };
+    struct alignas(4 * sizeof(T)) Four { T v[4]; };
 #pragma unroll
     for (int i = 0; i < TM; i++) {
-        const int m = m0 + (wm * TM + i) * 16 + l16;
-        if (m >= p.M) continue;
 #pragma unroll
-        for (int j = 0; j < TN; j++) {
-            const int n = n0 + (wn * TN + j) * 16 + quarter * 4;
-            if (n < p.N) store4(y + (long)m * p.N + n, acc[i][j], p.N - n);
+        for (int j = 0; j < TN; j++)
+            *reinterpret_cast<Four *>(mine + l16 * PITCH + (j * 16 + quarter * 4) * (int)sizeof(T)) =
+                Four{{(T)acc[i][j][0], (T)acc[i][j][1], (T)acc[i][j][2], (T)acc[i][j][3]}};
+#pragma unroll
+        for (int c = 0; c < 16 * PIECES / 64; c++) {
+            const int piece = c * 64 + lane, row = piece / PIECES, column = piece % PIECES * V;
+            const Piece v = *reinterpret_cast<const Piece *>(mine + row * PITCH + column * (int)sizeof(T));
+            const int m = m0 + (wm * TM + i) * 16 + row, n = n0 + wn * TN * 16 + column;
+            if (m >= p.M) continue;
+            T *const to = y + (long)m * p.N + n;
+            if (n + V <= p.N) {
+                *reinterpret_cast<Piece *>(to) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (n + e < p.N) to[e] = v.v[e];
+            }
         }
     }
 }
