@@ -129,10 +129,6 @@ template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v, int 
 // straight from global memory into one of STAGES parts of LDS.  A row is eight pieces of 16 bytes; row r has piece g at place g ^ (r & 7), so
 // that lanes that read at once meet different banks.  Which piece a lane multiplies is free as long as both operands agree, since a block
 // has one scale.
-//
-// The loads are what bounds the largest tile: 72 instructions of 1 KB a step take a CU some 2900 cycles, its products 2048.  So the loads never run
-// dry: a step begins when its part of LDS has landed (one barrier), the waves read all their fragments, and as soon as they have them
-// (another barrier) the loads of the step STAGES ahead follow those still on their way, between the products.
 template <int BM, int BN, int WM, int WN, int STAGES, int FORMAT, int OUT, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p)
 {
@@ -155,8 +151,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
     const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64), wm = wave / WN, wn = wave % WN, l16 = lane % 16, quarter = lane / 16;
     const int row_bytes = p.KB * kBlock8, rows_x = min(BM, p.M - m0), rows_w = min(BN, p.N - n0);
     const uint8_t *const qx = p.qx + (long)m0 * row_bytes, *const qw = p.qw + (long)n0 * row_bytes;
-    // load i of a wave is rows i * 8 * WAVES + 8 * wave .. + 7 of an operand's tile, eight lanes a row
-    const uint32_t offset = (uint32_t)(wave * 8 + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
+    // load i of a wave is eight rows of an operand's tile, eight lanes a row: of W all waves take turns, of X those that multiply the rows
+    const int first_x = wm * (BM / WM) + wn * 8, first_w = wave * 8;
+    const uint32_t offset_x = (uint32_t)(first_x + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
+    const uint32_t offset_w = (uint32_t)(first_w + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
     // this lane's scale has place t of X's or t - BM of W's; the scales of a lane's groups of 16 rows are side by side.  (A wave's scales
     // are all of X or all of W.)
     const bool scale_x = wave * 64 < BM, w_rows = p.w_scale_rows == p.N;
@@ -171,8 +169,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
         const uint32_t to = lds_at + (uint32_t)(stage * STAGE);
         if (i < LOADS) {
             const bool x = i < A_LOADS;
-            const int row = (x ? i : i - A_LOADS) * 8 * WAVES, bytes = live ? ((x ? rows_x : rows_w) - row) * row_bytes - kb * kBlock8 : 0;
-            to_lds16(buffer((x ? qx : qw) + (long)row * row_bytes + kb * kBlock8, bytes), to + (uint32_t)((x ? 0 : BM * kBlock8) + (row + wave * 8) * kBlock8), offset);
+            const int row = x ? i * 8 * WN : (i - A_LOADS) * 8 * WAVES, bytes = live ? ((x ? rows_x : rows_w) - row) * row_bytes - kb * kBlock8 : 0;
+            to_lds16(buffer((x ? qx : qw) + (long)row * row_bytes + kb * kBlock8, bytes),
+                     to + (uint32_t)((x ? first_x : BM + first_w) + row) * kBlock8, x ? offset_x : offset_w);
         } else {
             to_lds1(buffer(scales + (long)kb * scale_step, live ? scale_rows : 0), to + (uint32_t)(NUMBERS + wave * 256), scale_offset);
         }
@@ -190,55 +189,108 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
         const i32x4 low = *reinterpret_cast<const i32x4 *>(from + group * 16 * kBlock8 + at0), high = *reinterpret_cast<const i32x4 *>(from + group * 16 * kBlock8 + at1);
         return (i32x8)__builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    constexpr int BEFORE = TM > 4 ? 3 : TM / 2;  // rows of 16 multiplied while the step's other fragments are read
-    constexpr int EACH = (LOADS + TM - BEFORE) / (TM - BEFORE);  // loads behind each of the other rows
-#pragma unroll
-    for (int k = 0; k < STAGES; k++)
-#pragma unroll
-        for (int i = 0; i <= LOADS; i++) load(k, kb0 + k, i);
-    int stage = 0;
-    for (int kb = kb0; kb < kb1; kb++) {
-        wait_loads<(STAGES - 1) * (LOADS + 1)>();  // this wave's part of the step has landed,
-        __builtin_amdgcn_s_barrier();              // and the others'
-        asm volatile("" ::: "memory");
+    i32x8 wq[TN], xq[TM];
+    ScaleWords<TN> sw;
+    ScaleWords<TM> sx;
+    auto read = [&](int stage) {
         const uint8_t *const from = lds + stage * STAGE;
         const uint32_t *const s_lds = reinterpret_cast<const uint32_t *>(from + NUMBERS);
-        const ScaleWords<TN> sw = scale_words<TN>(s_lds + BM + (wn * 16 + l16) * TN);
-        const ScaleWords<TM> sx = scale_words<TM>(s_lds + (wm * 16 + l16) * TM);
-        i32x8 wq[TN], xq[TM];
-        Exact32 wf[EXACT ? TN : 1];
+        sw = scale_words<TN>(s_lds + BM + (wn * 16 + l16) * TN);
+        sx = scale_words<TM>(s_lds + (wm * 16 + l16) * TM);
 #pragma unroll
         for (int j = 0; j < TN; j++) wq[j] = fragment(from + b_at, j);
 #pragma unroll
         for (int i = 0; i < TM; i++) xq[i] = fragment(from + a_at, i);
-        __builtin_amdgcn_sched_barrier(0);
-        auto row = [&](int i) {
-            if constexpr (EXACT) {
-                if (i == 0) {
+    };
+    // rows [first, last) of 16, behind each of the first `count` products one load of step kb into a stage
+    auto multiply = [&](int first, int last, int count, int stage, int kb) {
+        Exact32 wf[EXACT ? TN : 1];
+        if constexpr (EXACT) {
 #pragma unroll
-                    for (int j = 0; j < TN; j++) wf[j] = exact32<0>(wq[j], sw.w[j]);
+            for (int j = 0; j < TN; j++) wf[j] = exact32<0>(wq[j], sw.w[j]);
+        }
+#pragma unroll
+        for (int i = first; i < last; i++) {
+            Exact32 xf;
+            if constexpr (EXACT) xf = exact32<FORMAT>(xq[i], sx.w[i]);
+#pragma unroll
+            for (int j = 0; j < TN; j++) {
+                if constexpr (EXACT) acc[i][j] = mfma16_exact(wf[j], xf, acc[i][j]);
+                else acc[i][j] = mfma16<FORMAT>(wq[j], xq[i], acc[i][j], sw.w[j], sx.w[i]);
+                if ((i - first) * TN + j < count) {
+                    load(stage, kb, (i - first) * TN + j);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                const Exact32 xf = exact32<FORMAT>(xq[i], sx.w[i]);
-#pragma unroll
-                for (int j = 0; j < TN; j++) acc[i][j] = mfma16_exact(wf[j], xf, acc[i][j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < TN; j++) acc[i][j] = mfma16<FORMAT>(wq[j], xq[i], acc[i][j], sw.w[j], sx.w[i]);
             }
             __builtin_amdgcn_sched_barrier(0);
-        };
-#pragma unroll
-        for (int i = 0; i < BEFORE; i++) row(i);
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave has read all of the step,
-        __builtin_amdgcn_s_barrier();        // and the others
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int i = BEFORE; i < TM; i++) {
-#pragma unroll
-            for (int k = (i - BEFORE) * EACH; k < (i - BEFORE + 1) * EACH && k <= LOADS; k++) load(stage, kb + STAGES, k);
-            row(i);
         }
-        stage = stage == STAGES - 1 ? 0 : stage + 1;
+#pragma unroll
+        for (int l = (last - first) * TN; l < count; l++) load(stage, kb, l);
+    };
+    auto barrier = [] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto all_read = [] { __builtin_amdgcn_s_waitcnt(0xc07f); };  // this wave's reads of LDS are done
+#pragma unroll
+    for (int k = 0; k < STAGES; k++)
+#pragma unroll
+        for (int i = 0; i <= LOADS; i++) load(k, kb0 + k, i);
+    wait_loads<(STAGES - 1) * (LOADS + 1)>();
+    barrier();
+    if constexpr (WAVES == 8) {
+        // Two waves a SIMD take turns: while one multiplies the other reads, a barrier at every change.  Slot 2s: the first four waves read step s, the
+        // others multiply step s - 1; slot 2s + 1 the other way round.  Of a step's part of LDS the rows of X that only the first four waves
+        // read are free from slot 2s + 1 on, the rest from slot 2s + 2; there the loads of step s + 2 go out.  Slot 2s + 4 reads them, and every
+        // wave has waited for its own by the barrier before.
+        static_assert(STAGES == 2, "two steps in LDS");
+        if (wm == 0) {
+            for (int kb = kb0; kb < kb1; kb++) {
+                const int stage = (kb - kb0) & 1;
+                if (kb > kb0) {
+#pragma unroll
+                    for (int i = A_LOADS; i <= LOADS; i++) load(stage ^ 1, kb + 1, i);
+                }
+                read(stage);
+                all_read();
+                barrier();
+                __builtin_amdgcn_s_setprio(1);
+                multiply(0, TM, A_LOADS, stage, kb + 2);
+                __builtin_amdgcn_s_setprio(0);
+                wait_loads<A_LOADS>();
+                barrier();
+            }
+            barrier();
+        } else {
+            barrier();
+            for (int kb = kb0; kb < kb1; kb++) {
+                const int stage = (kb - kb0) & 1;
+                read(stage);
+                all_read();
+                wait_loads<0>();
+                barrier();
+                __builtin_amdgcn_s_setprio(1);
+                multiply(0, TM, LOADS + 1, stage, kb + 2);
+                __builtin_amdgcn_s_setprio(0);
+                barrier();
+            }
+        }
+    } else {
+        // one wave a SIMD and workgroup, so the workgroups of a CU overlap each other
+        constexpr int BEFORE = TM / 2;
+        int stage = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            read(stage);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(0, BEFORE, 0, 0, 0);
+            all_read();
+            barrier();  // all have read the step: its part of LDS is free
+            multiply(BEFORE, TM, LOADS + 1, stage, kb + STAGES);
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            wait_loads<(STAGES - 1) * (LOADS + 1)>();  // this wave's part of the next step has landed,
+            barrier();                                 // and the others'
+        }
     }
     wait_loads<0>();  // nothing is on its way to LDS any more,
     __builtin_amdgcn_s_barrier();  // and every wave has read its last step: LDS is free
