@@ -233,18 +233,19 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
         asm volatile("" ::: "memory");
     };
     auto all_read = [] { __builtin_amdgcn_s_waitcnt(0xc07f); };  // this wave's reads of LDS are done
+    constexpr int FIRST = WAVES == 8 ? STAGES : STAGES - 1;  // steps on their way at first
 #pragma unroll
-    for (int k = 0; k < STAGES; k++)
+    for (int k = 0; k < FIRST; k++)
 #pragma unroll
         for (int i = 0; i <= LOADS; i++) load(k, kb0 + k, i);
-    wait_loads<(STAGES - 1) * (LOADS + 1)>();
-    barrier();
     if constexpr (WAVES == 8) {
         // Two waves a SIMD take turns: while one multiplies the other reads, a barrier at every change.  Slot 2s: the first four waves read step s, the
         // others multiply step s - 1; slot 2s + 1 the other way round.  Of a step's part of LDS the rows of X that only the first four waves
         // read are free from slot 2s + 1 on, the rest from slot 2s + 2; there the loads of step s + 2 go out.  Slot 2s + 4 reads them, and every
         // wave has waited for its own by the barrier before.
         static_assert(STAGES == 2, "two steps in LDS");
+        wait_loads<LOADS + 1>();
+        barrier();
         if (wm == 0) {
             for (int kb = kb0; kb < kb1; kb++) {
                 const int stage = (kb - kb0) & 1;
@@ -277,19 +278,14 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
             }
         }
     } else {
-        // one wave a SIMD and workgroup, so the workgroups of a CU overlap each other
-        constexpr int BEFORE = TM / 2;
         int stage = 0;
         for (int kb = kb0; kb < kb1; kb++) {
+            wait_loads<(STAGES - 2) * (LOADS + 1)>();  // this wave's part of the step has landed,
+            all_read();                                // it has read all of the step before,
+            barrier();                                 // and so have the others: that one's part of LDS is free
             read(stage);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(0, BEFORE, 0, 0, 0);
-            all_read();
-            barrier();  // all have read the step: its part of LDS is free
-            multiply(BEFORE, TM, LOADS + 1, stage, kb + STAGES);
+            multiply(0, TM, LOADS + 1, stage == 0 ? STAGES - 1 : stage - 1, kb + STAGES - 1);
             stage = stage == STAGES - 1 ? 0 : stage + 1;
-            wait_loads<(STAGES - 1) * (LOADS + 1)>();  // this wave's part of the next step has landed,
-            barrier();                                 // and the others'
         }
     }
     wait_loads<0>();  // nothing is on its way to LDS any more,
@@ -474,15 +470,37 @@ struct Plan8 {
     int tile, parts, kb_per_part;  // tile: the square tile's edge
 };
 
+// The tile and the parts that K is cut into: the least of what a launch takes by the busiest CU's work.  A tile's step alone on its CU takes
+// `alone` us (latency), a step of one among as many as the CU holds `among`, its way out `out`; parts are written in fp32, read and added
+// up by a launch of their own.  Constants fitted to every (tile, parts) of 60 products of 33 .. 16384 rows, 64 .. 8192 columns and K on an MI355X;
+// what the rule picks takes 0.7 % (16-bit output) and 0.2 % (fp32) longer than the best of them in the mean, at most 13 % (8192 x 8192 x 1024).
+struct TileTimes { double alone, among, out; int held; };
+
 Plan8 plan8(int out, int M, int N, int KB)
 {
-    auto tiles = [&](long edge) { return ((M + edge - 1) / edge) * ((N + edge - 1) / edge); };
-    const int tile = out != 0 && tiles(256) >= 256 ? 256 : tiles(128) >= 128 ? 128 : 64;
-    int parts = 1;
-    const long have = tiles(tile);
-    while (have * parts * 2 <= (tile == 256 ? 256 : 512) && KB / (parts * 2) >= 4) parts *= 2;
-    const int per = (KB + parts - 1) / parts;
-    return {tile, (KB + per - 1) / per, per};
+    constexpr int kEdges[] = {64, 128, 256};
+    constexpr TileTimes kFast[] = {{0.31, 0.194, 0.72, 3}, {0.74, 0.473, 1.56, 2}, {1.43, 1.454, 5.2, 1}}, kExact[] = {{0.42, 0.32, 0.47, 3}, {1.04, 0.844, 1.27, 2}};
+    const TileTimes *const times = out == 0 ? kExact : kFast;
+    const double join = out == 0 ? 2.8 : 1.8, join_part = out == 0 ? 0.956e-6 : 0.865e-6, join_out = 0.1e-6;
+    Plan8 best = {64, 1, KB};
+    double least = 1e30;
+    for (int i = 0; i < (out == 0 ? 2 : 3); i++) {
+        const long edge = kEdges[i], tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
+        for (int parts = 1; parts <= 16 && parts <= KB; parts *= 2) {
+            if (parts > 1 && tiles * parts > 2048) break;
+            const int steps = (KB + parts - 1) / parts;
+            if ((KB + steps - 1) / steps != parts) continue;
+            const long each = (tiles * parts + 255) / 256, rounds = (each + times[i].held - 1) / times[i].held;
+            const double alone = times[i].alone * (double)rounds, among = times[i].among * (double)each;
+            double t = steps * (alone > among ? alone : among) + times[i].out * (double)each * (parts > 1 || out == 0 ? 2 : 1);
+            if (parts > 1) t += join + (parts * join_part + join_out) * (double)M * (double)N;
+            if (t < least) {
+                least = t;
+                best = {(int)edge, parts, steps};
+            }
+        }
+    }
+    return best;
 }
 
 template <int FORMAT, int OUT, bool EXACT> hipError_t launch_tiles(int tile, unsigned groups, const TileParams &p, hipStream_t stream)
@@ -493,7 +511,7 @@ template <int FORMAT, int OUT, bool EXACT> hipError_t launch_tiles(int tile, uns
             return hipGetLastError();
         }
     if (tile == 128) linear8_tiles<128, 128, 2, 2, 2, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
-    else linear8_tiles<64, 64, 2, 2, 4, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
+    else linear8_tiles<64, 64, 2, 2, 3, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 
