@@ -201,7 +201,8 @@ def Quantize8Both(X, M, K, block_rows=1, format=E4M3):
 
 def Linear8(X, QW, SW, M, N, K):
     """X (M x K, quantized on the way as Quantize8 does) times the transpose of the packed weight (N x K, E4M3, blocks of 128 x 128 or of
-    one row): Y (M, N) of X's type.  Sums in fp32.  At most 32 rows are quantized and multiplied in one launch."""
+    one row): Y (M, N) of X's type.  Sums in fp32.  Up to 32 rows, their packed numbers at most 72 KB, are
+    quantized and multiplied in one launch."""
     try:
         return _C.Linear8(X, QW, SW, M, N, K)
     except TypeError:

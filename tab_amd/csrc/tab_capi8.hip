@@ -193,7 +193,7 @@ int tab_norm_residual(const void *dev_X, long ldx, const void *dev_Y, long ldy, 
 size_t tab_norm_residual_backward_workspace_bytes(int M, int D, int gates)
 {
     if (M < 1 || D < 1 || D > tab::kNormWidthMost || gates < 0 || (gates > 0 && M % gates)) return 0;
-    return tab::norm_grad_workspace(M, D, gates ? M / gates : M);
+    return tab::norm_grad_workspace(gates != 0, M, D, gates ? M / gates : M);
 }
 
 int tab_norm_residual_backward(const void *dev_dR, const void *dev_dH, const void *dev_R, const void *dev_Y, const void *dev_gate, int gate_dtype,

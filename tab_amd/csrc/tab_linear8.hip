@@ -354,10 +354,11 @@ struct RowsParams {
     void *y;
     int M, N, K, KB, w_scale_rows, groups_each;
     long ldx;
+    Div32 div_kb;
 };
 
 constexpr int kRowsMost = 32;           // rows of X
-constexpr int kRowsLds = 64 << 10;      // bytes of X in LDS
+constexpr int kRowsLds = 72 << 10;      // bytes of X in LDS: 16 rows of 4096 and two workgroups a CU
 constexpr int kRowsWaves = 8;
 
 __host__ __device__ __forceinline__ int rows_stride(int KB) { return KB * kBlock8 + 16; }
@@ -390,24 +391,32 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
     const int groups = (p.N + 15) / 16, group0 = (int)blockIdx.x * p.groups_each, group1 = min(groups, group0 + p.groups_each);
     load(group0 * 16, wave);
 
-    // X into LDS: blocks in the order of memory, 16 lanes a block
-    for (int block = t / 16; block < p.M * p.KB; block += 64 * WAVES / 16) {
-        const int m = block / p.KB, kb = block - m * p.KB;
-        uint8_t *const to = packed + m * stride + kb * kBlock8 + l16 * 8;
-        if constexpr (INPUT == 3) {
-            *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p.x) + (long)block * kBlock8 + l16 * 8);
-            if (l16 == 0) scales[kb * p.M + m] = p.sx[(long)kb * p.M + m];
-        } else {
-            using X = typename Element<INPUT>::type;
-            const int k = kb * kBlock8 + l16 * 8;
-            float v[8];
-            load8(static_cast<const X *>(p.x) + m * p.ldx + k, p.K - k, v);
-            uint32_t amax = 0;
+    // X into LDS: blocks in the order of memory, 16 lanes a block, AT_ONCE of them on their way
+    constexpr int AT_ONCE = 8, STEP = 64 * WAVES / 16;
+    const int blocks = p.M * p.KB;
+    for (int first = t / 16; first < blocks; first += AT_ONCE * STEP) {
+        using X = typename Element<INPUT == 3 ? 0 : INPUT>::type;
+        Words<X> v[AT_ONCE];
 #pragma unroll
-            for (int j = 0; j < 8; j++) amax = max(amax, finite_bits(v[j]));
-            const uint32_t byte = scale_byte<FORMAT>(max_of_row16(amax));
-            const float inv = inverse_scale(byte);
-            *reinterpret_cast<uint2 *>(to) = uint2{pack4<FORMAT>(v[0], v[1], v[2], v[3], inv), pack4<FORMAT>(v[4], v[5], v[6], v[7], inv)};
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int block = first + u * STEP, m = (int)div32(block, p.div_kb), kb = block - m * p.KB;
+            if (block >= blocks) break;
+            if constexpr (INPUT == 3) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p.x) + (long)block * kBlock8 + l16 * 8);
+                v[u].w[0] = w.x, v[u].w[1] = w.y, v[u].w[2] = p.sx[(long)kb * p.M + m];
+            } else {
+                v[u] = load_words(static_cast<const X *>(p.x) + m * p.ldx, kb * kBlock8 + l16 * 8, p.K);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int block = first + u * STEP, m = (int)div32(block, p.div_kb), kb = block - m * p.KB;
+            if (block >= blocks) break;
+            uint32_t byte;
+            uint2 w;
+            if constexpr (INPUT == 3) w = {v[u].w[0], v[u].w[1]}, byte = v[u].w[2];
+            else w = pack_run<X, FORMAT>(v[u], byte);
+            *reinterpret_cast<uint2 *>(packed + m * stride + kb * kBlock8 + l16 * 8) = w;
             if (l16 == 0) scales[kb * p.M + m] = byte;
         }
     }
@@ -452,7 +461,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
     }
 }
 
-bool rows_fit(int M, int KB) { return M <= kRowsMost && (long)rows_lds(M, 1) * KB <= kRowsLds; }
+bool rows_fit(int M, int KB) { return M <= kRowsMost && KB <= kRowsLds / kBlock8 && rows_lds(M, KB) <= kRowsLds; }
 
 template <int INPUT, int FORMAT, int OUT> hipError_t launch_rows(RowsParams p, hipStream_t stream)
 {
@@ -519,7 +528,7 @@ template <int FORMAT> hipError_t launch_format(int out, const Linear8Args &a, vo
 {
     const int scale_rows = w_scale_rows(a.N, a.w_block_rows);
     if (rows_fit(a.M, a.KB)) {
-        const RowsParams p = {a.qx, a.sx, a.qw, a.sw, a.y, a.M, a.N, a.KB * kBlock8, a.KB, scale_rows, 0, 0};
+        const RowsParams p = {a.qx, a.sx, a.qw, a.sw, a.y, a.M, a.N, a.KB * kBlock8, a.KB, scale_rows, 0, 0, make_div32((uint32_t)a.KB)};
         return out == 0 ? launch_rows<3, FORMAT, 0>(p, stream) : out == 1 ? launch_rows<3, FORMAT, 1>(p, stream) : launch_rows<3, FORMAT, 2>(p, stream);
     }
     const Plan8 plan = plan8(out, a.M, a.N, a.KB);
@@ -566,7 +575,7 @@ bool linear8_rows_supported(int M, int K) { return rows_fit(M, blocks8(K)); }
 
 hipError_t launch_linear8_rows(int dtype, const Linear8RowsArgs &a, hipStream_t stream)
 {
-    const RowsParams p = {a.x, nullptr, a.qw, a.sw, a.y, a.M, a.N, a.K, blocks8(a.K), w_scale_rows(a.N, a.w_block_rows), 0, a.ldx};
+    const RowsParams p = {a.x, nullptr, a.qw, a.sw, a.y, a.M, a.N, a.K, blocks8(a.K), w_scale_rows(a.N, a.w_block_rows), 0, a.ldx, make_div32((uint32_t)blocks8(a.K))};
     return dtype == 0 ? launch_rows<0, 0, 0>(p, stream) : dtype == 1 ? launch_rows<1, 0, 1>(p, stream) : launch_rows<2, 0, 2>(p, stream);
 }
 

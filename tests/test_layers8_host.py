@@ -21,10 +21,12 @@ def test_sizes_of_packed_operands():
     lib = _capi.load()
     assert [lib.tab_blocks8(k) for k in (-1, 0, 1, 127, 128, 129, 2050)] == [0, 0, 1, 1, 1, 2, 17]
     assert tab_amd.blocks8(2050) == 17
-    # few rows are quantized and multiplied in one launch, longer ones packed in the workspace (numbers, then scales)
+    # up to 32 rows whose packed numbers and scales fit 72 KB are quantized and multiplied in one launch, others packed in the workspace
+    # (numbers, then scales)
     for out in (0, 1, 2):
-        assert lib.tab_linear8_workspace_bytes(out, 32, 1000, 4096) == 0
-        assert lib.tab_linear8_packed_workspace_bytes(out, 32, 1000, 4096) == 0
+        assert lib.tab_linear8_workspace_bytes(out, 17, 1000, 4096) == 0 < lib.tab_linear8_workspace_bytes(out, 18, 1000, 4096)
+        assert lib.tab_linear8_workspace_bytes(out, 32, 1000, 1000) == 0 < lib.tab_linear8_workspace_bytes(out, 33, 1000, 1000)
+        assert lib.tab_linear8_packed_workspace_bytes(out, 17, 1000, 4096) == 0
         assert lib.tab_linear8_workspace_bytes(out, 1000, 4096, 300) >= 1000 * (384 + 3)
         assert lib.tab_linear8_workspace_bytes(out, 0, 1, 1) == lib.tab_linear8_packed_workspace_bytes(out, 1, -1, 1) == 0
     assert lib.tab_norm_residual_backward_workspace_bytes(10, 64, 3) == 0       # 10 rows have no 3 gates
