@@ -447,8 +447,8 @@ struct GradPlan {
 
 GradPlan grad_plan(bool gate, int M, int D, int rows_per_gate)
 {
-    // as many groups as the chip holds at once, but four rows in each before there are more than CUs: every group writes 2 D sums
-    const long held = groups_at_once(shape_of(D)), few = M / 4 > 256 ? M / 4 : 256, most = held < few ? held : few, rows = (M + most - 1) / most;
+    // as many groups as the chip holds at once, but two rows in each before there are more than CUs: every group writes 2 D sums
+    const long held = groups_at_once(shape_of(D)), few = M / 2 > 256 ? M / 2 : 256, most = held < few ? held : few, rows = (M + most - 1) / most;
     const bool whole = gate && rows_per_gate <= rows;
     // (at least one row a group and, for pieces, as even as they come)
     const long pieces = whole ? 1 : (rows_per_gate + rows - 1) / rows;
