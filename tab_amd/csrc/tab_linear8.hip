@@ -4,7 +4,7 @@
 // 16-bit outputs: v_mfma_scale_f32_16x16x128_f8f6f4.  One instruction is a 16 x 16 tile over one block of K, and it takes the E8M0 bytes of its
 // 16 rows and 16 columns as operands, so the scales cost no vector instruction and the sums stay in one set of fp32 accumulators.  Inside
 // the instruction, products of eight neighbours in K are aligned to the largest of them and keep 13 bits below it (measured): 1.5e-5 of the
-// output's size for normal operands, far below the 2^-9 or 2^-12 of the output's own rounding, but not what an fp32 output is for.
+// output's size for normal operands, far below the 2^-8 or 2^-11 of the output's own rounding, but not what an fp32 output is for.
 // fp32 outputs (EXACT): the numbers times their scales are bf16 numbers exactly (4 of 8 significant bits, the exponent range of fp32), made by one
 // conversion of two numbers, and v_mfma_f32_16x16x32_bf16 multiplies them at half the rate with full fp32 sums.  A number below 2^-126 may
 // count as zero there.
@@ -564,6 +564,13 @@ long linear8_threads(int out_dtype, int M, int N, int KB)
     const Plan8 plan = plan8(out_dtype, M, N, KB);
     const long edge = plan.tile;
     return ((M + edge - 1) / edge) * ((N + edge - 1) / edge) * plan.parts * (edge == 256 ? 512 : 256);
+}
+
+int linear8_way(int out_dtype, int M, int N, int KB)
+{
+    if (rows_fit(M, KB)) return 0;
+    const Plan8 plan = plan8(out_dtype, M, N, KB);
+    return plan.tile * 100 + plan.parts;
 }
 
 hipError_t launch_linear8(int out_dtype, int x_format, const Linear8Args &a, void *workspace, hipStream_t stream)

@@ -11,10 +11,23 @@ from tab_amd import nn as tab_nn
 
 P = 4096  # an aligned address that is never dereferenced: every call below fails its checks
 
+# (0 fp32 or 1 16-bit output, M, N, K, edge of the tile * 100 + parts of K): every tile, K whole and in parts, one step of K and many
+WAYS = [(0, 34, 35, 60, 6401), (0, 33, 34, 940, 6408), (0, 2970, 643, 60, 12801), (0, 2100, 4003, 500, 12801), (0, 514, 661, 8873, 12808),
+        (1, 34, 35, 60, 6401), (1, 33, 39, 1412, 6404), (1, 2970, 643, 60, 12801), (1, 2100, 2050, 1100, 12801), (1, 654, 1476, 8658, 12804),
+        (1, 1425, 8304, 61, 25601), (1, 2300, 4099, 4100, 25601), (1, 1031, 2893, 11022, 25604)]
+
 
 def _refuses(status, message, code=-1):
     assert status == code, status
     assert message in _capi.load().tab_last_error().decode()
+
+
+@pytest.mark.parametrize("out,M,N,K,way", WAYS)
+def test_products_take_the_tiles_that_they_are_tested_for(out, M, N, K, way):
+    assert ctypes.CDLL(_capi.LIB_PATH).tab_internal_linear8_way(out, M, N, K) == way
+    if out == 1:
+        assert ctypes.CDLL(_capi.LIB_PATH).tab_internal_linear8_way(2, M, N, K) == way
+    assert ctypes.CDLL(_capi.LIB_PATH).tab_internal_linear8_way(out, 32, N, 1000) == 0
 
 
 def test_sizes_of_packed_operands():
