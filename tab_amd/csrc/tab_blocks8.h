@@ -261,7 +261,7 @@ struct Linear8Args {
 constexpr int kBlocks8Most = 65535;   // blocks of K: 256 packed rows stay below 2^31 bytes
 size_t linear8_workspace(int out_dtype, int M, int N, int KB);
 long linear8_threads(int out_dtype, int M, int N, int KB);  // of the launch
-int linear8_way(int out_dtype, int M, int N, int KB);  // 0: few rows; else the tile's edge * 100 + the parts of K
+int linear8_way(int out_dtype, int M, int N, int KB);  // 0: few rows; else (the tile's rows + columns) / 2 * 100 + the parts of K
 hipError_t launch_linear8(int out_dtype, int x_format, const Linear8Args &a, void *workspace, hipStream_t stream);
 
 // The product that quantizes a few rows of x itself.

@@ -224,8 +224,8 @@ int tab_norm_residual_backward(const void *dev_dR, const void *dev_dH, const voi
     return e == hipSuccess ? TAB_OK : device_fail(e, "norm gradient launch");
 }
 
-/* Test hook, absent from include/tab_amd.h: how an M x N product over K would be computed: 0 as few rows, else the tile's edge * 100 + the
- * parts of K. */
+/* Test hook, absent from include/tab_amd.h: how an M x N product over K would be computed: 0 as few rows, else (the tile's rows + columns) / 2 * 100
+ * + the parts of K. */
 int tab_internal_linear8_way(int out_dtype, int M, int N, int K) { return tab::linear8_way(out_dtype, M, N, tab::blocks8(K)); }
 
 }  // extern "C"

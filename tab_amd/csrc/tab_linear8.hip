@@ -130,7 +130,7 @@ template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v, int 
 // that lanes that read at once meet different banks.  Which piece a lane multiplies is free as long as both operands agree, since a block
 // has one scale.
 template <int BM, int BN, int WM, int WN, int STAGES, int FORMAT, int OUT, bool EXACT>
-__global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p)
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const TileParams p)
 {
     using T = typename Element<OUT>::type;
     constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -153,27 +153,32 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
     const uint8_t *const qx = p.qx + (long)m0 * row_bytes, *const qw = p.qw + (long)n0 * row_bytes;
     // load i of a wave is eight rows of an operand's tile, eight lanes a row: of W all waves take turns, of X those that multiply the rows
     const int first_x = wm * (BM / WM) + wn * 8, first_w = wave * 8;
-    const uint32_t offset_x = (uint32_t)(first_x + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
-    const uint32_t offset_w = (uint32_t)(first_w + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
+    const uint32_t x_at = (uint32_t)(first_x + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
+    const uint32_t w_at = (uint32_t)(first_w + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
     // this lane's scale has place t of X's or t - BM of W's; the scales of a lane's groups of 16 rows are side by side.  (A wave's scales
     // are all of X or all of W.)
-    const bool scale_x = wave * 64 < BM, w_rows = p.w_scale_rows == p.N;
+    const bool scale_x = wave * 64 < BM, row_scales = p.w_scale_rows == p.N;
     const int groups = scale_x ? TM : TN, place = scale_x ? t : t - BM, scale_row = place / (16 * groups) * (16 * groups) + place % groups * 16 + place / groups % 16;
-    const uint32_t scale_offset = (uint32_t)(scale_x || w_rows ? scale_row : (n0 + scale_row) / kBlock8 - n0 / kBlock8);
-    const uint8_t *const scales = scale_x ? p.sx + m0 : p.sw + (w_rows ? n0 : n0 / kBlock8);
-    const int scale_step = scale_x ? p.M : p.w_scale_rows, scale_rows = scale_x ? rows_x : wave * 64 >= BM + BN ? 0 : w_rows ? rows_w : (n0 + rows_w - 1) / kBlock8 - n0 / kBlock8 + 1;
+    const uint32_t scale_offset = (uint32_t)(scale_x || row_scales ? scale_row : (n0 + scale_row) / kBlock8 - n0 / kBlock8);
+    const int scale_step = scale_x ? p.M : p.w_scale_rows;
+    const uint8_t *scales = (scale_x ? p.sx + m0 : p.sw + (row_scales ? n0 : n0 / kBlock8)) + (long)kb0 * scale_step;
+    const int scale_rows = scale_x ? rows_x : wave * 64 >= BM + BN ? 0 : row_scales ? rows_w : (n0 + rows_w - 1) / kBlock8 - n0 / kBlock8 + 1;
     const uint32_t lds_at = lds_address(lds);
-    // load i of a step, the scales last; past the end of K zeros, so that the count of a wave's loads stays the same
+    // the rows of an operand's tile are one buffer: rows past its end, and with a size of zero all of it, load as zeros
+    const i32x4 x_rows = buffer(qx, rows_x * row_bytes), w_rows = buffer(qw, rows_w * row_bytes);
+    auto sized = [](i32x4 b, bool live) { return i32x4{b[0], b[1], live ? b[2] : 0, b[3]}; };
+    // load i of step kb into the part of LDS at `stage`, the scales last (those of one step after another).  Past the end of K zeros, so
+    // that the count of a wave's loads stays the same.
     auto load = [&](int stage, int kb, int i) {
         const bool live = kb < kb1;
-        const uint32_t to = lds_at + (uint32_t)(stage * STAGE);
-        if (i < LOADS) {
-            const bool x = i < A_LOADS;
-            const int row = x ? i * 8 * WN : (i - A_LOADS) * 8 * WAVES, bytes = live ? ((x ? rows_x : rows_w) - row) * row_bytes - kb * kBlock8 : 0;
-            to_lds16(buffer((x ? qx : qw) + (long)row * row_bytes + kb * kBlock8, bytes),
-                     to + (uint32_t)((x ? first_x : BM + first_w) + row) * kBlock8, x ? offset_x : offset_w);
+        const uint32_t to = lds_at + (uint32_t)stage;
+        if (i < A_LOADS) {
+            to_lds16(sized(x_rows, live), to + (uint32_t)(first_x + i * 8 * WN) * kBlock8, x_at + (uint32_t)(i * 8 * WN * row_bytes + kb * kBlock8));
+        } else if (i < LOADS) {
+            to_lds16(sized(w_rows, live), to + (uint32_t)(BM + first_w + (i - A_LOADS) * 8 * WAVES) * kBlock8, w_at + (uint32_t)((i - A_LOADS) * 8 * WAVES * row_bytes + kb * kBlock8));
         } else {
-            to_lds1(buffer(scales + (long)kb * scale_step, live ? scale_rows : 0), to + (uint32_t)(NUMBERS + wave * 256), scale_offset);
+            to_lds1(buffer(scales, live ? scale_rows : 0), to + (uint32_t)(NUMBERS + wave * 256), scale_offset);
+            scales += scale_step;
         }
     };
 
@@ -189,43 +194,52 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
         const i32x4 low = *reinterpret_cast<const i32x4 *>(from + group * 16 * kBlock8 + at0), high = *reinterpret_cast<const i32x4 *>(from + group * 16 * kBlock8 + at1);
         return (i32x8)__builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    i32x8 wq[TN], xq[TM];
-    ScaleWords<TN> sw;
-    ScaleWords<TM> sx;
-    auto read = [&](int stage) {
-        const uint8_t *const from = lds + stage * STAGE;
-        const uint32_t *const s_lds = reinterpret_cast<const uint32_t *>(from + NUMBERS);
-        sw = scale_words<TN>(s_lds + BM + (wn * 16 + l16) * TN);
-        sx = scale_words<TM>(s_lds + (wm * 16 + l16) * TM);
-#pragma unroll
-        for (int j = 0; j < TN; j++) wq[j] = fragment(from + b_at, j);
-#pragma unroll
-        for (int i = 0; i < TM; i++) xq[i] = fragment(from + a_at, i);
+    struct Operands {  // a wave's part of a step
+        i32x8 wq[TN], xq[TM];
+        ScaleWords<TN> sw;
+        ScaleWords<TM> sx;
     };
-    // rows [first, last) of 16, behind each of the first `count` products one load of step kb into a stage
-    auto multiply = [&](int first, int last, int count, int stage, int kb) {
+    constexpr int READS = 1 + TN + TM;
+    auto read = [&](Operands &o, int stage, int i) {  // read i of a step
+        const uint8_t *const from = lds + stage;
+        if (i == 0) {
+            const uint32_t *const s_lds = reinterpret_cast<const uint32_t *>(from + NUMBERS);
+            o.sw = scale_words<TN>(s_lds + BM + (wn * 16 + l16) * TN);
+            o.sx = scale_words<TM>(s_lds + (wm * 16 + l16) * TM);
+        } else if (i <= TN) {
+            o.wq[i - 1] = fragment(from + b_at, i - 1);
+        } else {
+            o.xq[i - 1 - TN] = fragment(from + a_at, i - 1 - TN);
+        }
+    };
+    auto read_all = [&](Operands &o, int stage) {
+#pragma unroll
+        for (int i = 0; i < READS; i++) read(o, stage, i);
+    };
+    // behind each of the first `count` products what `behind` does
+    auto multiply = [&](const Operands &o, int count, auto behind) {
         Exact32 wf[EXACT ? TN : 1];
         if constexpr (EXACT) {
 #pragma unroll
-            for (int j = 0; j < TN; j++) wf[j] = exact32<0>(wq[j], sw.w[j]);
+            for (int j = 0; j < TN; j++) wf[j] = exact32<0>(o.wq[j], o.sw.w[j]);
         }
 #pragma unroll
-        for (int i = first; i < last; i++) {
+        for (int i = 0; i < TM; i++) {
             Exact32 xf;
-            if constexpr (EXACT) xf = exact32<FORMAT>(xq[i], sx.w[i]);
+            if constexpr (EXACT) xf = exact32<FORMAT>(o.xq[i], o.sx.w[i]);
 #pragma unroll
             for (int j = 0; j < TN; j++) {
                 if constexpr (EXACT) acc[i][j] = mfma16_exact(wf[j], xf, acc[i][j]);
-                else acc[i][j] = mfma16<FORMAT>(wq[j], xq[i], acc[i][j], sw.w[j], sx.w[i]);
-                if ((i - first) * TN + j < count) {
-                    load(stage, kb, (i - first) * TN + j);
+                else acc[i][j] = mfma16<FORMAT>(o.wq[j], o.xq[i], acc[i][j], o.sw.w[j], o.sx.w[i]);
+                if (i * TN + j < count) {
+                    behind(i * TN + j);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int l = (last - first) * TN; l < count; l++) load(stage, kb, l);
+        for (int l = TM * TN; l < count; l++) behind(l);
     };
     auto barrier = [] {
         asm volatile("" ::: "memory");
@@ -233,31 +247,31 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
         asm volatile("" ::: "memory");
     };
     auto all_read = [] { __builtin_amdgcn_s_waitcnt(0xc07f); };  // this wave's reads of LDS are done
-    constexpr int FIRST = WAVES == 8 ? STAGES : STAGES - 1;  // steps on their way at first
+    #pragma unroll
+    for (int k = 0; k < STAGES; k++)
 #pragma unroll
-    for (int k = 0; k < FIRST; k++)
-#pragma unroll
-        for (int i = 0; i <= LOADS; i++) load(k, kb0 + k, i);
+        for (int i = 0; i <= LOADS; i++) load(k * STAGE, kb0 + k, i);
     if constexpr (WAVES == 8) {
         // Two waves a SIMD take turns: while one multiplies the other reads, a barrier at every change.  Slot 2s: the first four waves read step s, the
         // others multiply step s - 1; slot 2s + 1 the other way round.  Of a step's part of LDS the rows of X that only the first four waves
         // read are free from slot 2s + 1 on, the rest from slot 2s + 2; there the loads of step s + 2 go out.  Slot 2s + 4 reads them, and every
         // wave has waited for its own by the barrier before.
         static_assert(STAGES == 2, "two steps in LDS");
+        Operands o;
         wait_loads<LOADS + 1>();
         barrier();
         if (wm == 0) {
             for (int kb = kb0; kb < kb1; kb++) {
-                const int stage = (kb - kb0) & 1;
+                const int stage = (kb - kb0) & 1 ? STAGE : 0;
                 if (kb > kb0) {
 #pragma unroll
-                    for (int i = A_LOADS; i <= LOADS; i++) load(stage ^ 1, kb + 1, i);
+                    for (int i = A_LOADS; i <= LOADS; i++) load(STAGE - stage, kb + 1, i);
                 }
-                read(stage);
+                read_all(o, stage);
                 all_read();
                 barrier();
                 __builtin_amdgcn_s_setprio(1);
-                multiply(0, TM, A_LOADS, stage, kb + 2);
+                multiply(o, A_LOADS, [&](int i) { load(stage, kb + 2, i); });
                 __builtin_amdgcn_s_setprio(0);
                 wait_loads<A_LOADS>();
                 barrier();
@@ -266,26 +280,70 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tiles(const TileParams p
         } else {
             barrier();
             for (int kb = kb0; kb < kb1; kb++) {
-                const int stage = (kb - kb0) & 1;
-                read(stage);
+                const int stage = (kb - kb0) & 1 ? STAGE : 0;
+                read_all(o, stage);
                 all_read();
                 wait_loads<0>();
                 barrier();
                 __builtin_amdgcn_s_setprio(1);
-                multiply(0, TM, LOADS + 1, stage, kb + 2);
+                multiply(o, LOADS + 1, [&](int i) { load(stage, kb + 2, i); });
                 __builtin_amdgcn_s_setprio(0);
                 barrier();
             }
         }
+    } else if constexpr (EXACT && BM * BN > 64 * 128) {
+        // no registers for two steps' operands
+        static_assert(STAGES == 2, "steps in LDS");
+        Operands o;
+        for (int kb = kb0, stage = 0; kb < kb1; kb++, stage = STAGE - stage) {
+            wait_loads<LOADS + 1>();  // this wave's part of the step has landed,
+            barrier();                // and so has the others'
+            read_all(o, stage);
+            all_read();
+            barrier();                // the step's part of LDS is free
+            multiply(o, LOADS + 1, [&](int i) { load(stage, kb + 2, i); });
+        }
     } else {
-        int stage = 0;
-        for (int kb = kb0; kb < kb1; kb++) {
-            wait_loads<(STAGES - 2) * (LOADS + 1)>();  // this wave's part of the step has landed,
-            all_read();                                // it has read all of the step before,
-            barrier();                                 // and so have the others: that one's part of LDS is free
-            read(stage);
-            multiply(0, TM, LOADS + 1, stage == 0 ? STAGES - 1 : stage - 1, kb + STAGES - 1);
-            stage = stage == STAGES - 1 ? 0 : stage + 1;
+        // a step's operands are read from LDS while the step before is multiplied
+        Operands even, odd;
+        auto step = [&](const Operands &now, Operands &next, int kb, int stage) {
+            wait_loads<(STAGES - 2) * (LOADS + 1)>();  // this wave's part of the next step has landed,
+            all_read();                                // it has read all of this one,
+            barrier();                                 // and so have the others: this one's part of LDS is free
+            multiply(now, READS > LOADS + 1 ? READS : LOADS + 1, [&](int i) {
+                if (i < READS) read(next, stage == (STAGES - 1) * STAGE ? 0 : stage + STAGE, i);
+                if (i <= LOADS) load(stage, kb + STAGES, i);
+            });
+        };
+        wait_loads<(STAGES - 1) * (LOADS + 1)>();
+        barrier();
+        read_all(even, 0);
+        if constexpr (STAGES == 3) {  // places in LDS are constants of the code
+            for (int kb = kb0;; kb += 6) {
+                step(even, odd, kb, 0);
+                if (kb + 1 >= kb1) break;
+                step(odd, even, kb + 1, STAGE);
+                if (kb + 2 >= kb1) break;
+                step(even, odd, kb + 2, 2 * STAGE);
+                if (kb + 3 >= kb1) break;
+                step(odd, even, kb + 3, 0);
+                if (kb + 4 >= kb1) break;
+                step(even, odd, kb + 4, STAGE);
+                if (kb + 5 >= kb1) break;
+                step(odd, even, kb + 5, 2 * STAGE);
+                if (kb + 6 >= kb1) break;
+            }
+        } else {  // (with constants the largest of these tiles needs more registers than there are)
+            static_assert(STAGES == 2, "steps in LDS");
+            int stage = 0;
+            for (int kb = kb0; kb < kb1; kb += 2) {
+                step(even, odd, kb, stage);
+                stage = stage == STAGE ? 0 : STAGE;
+                if (kb + 1 < kb1) {
+                    step(odd, even, kb + 1, stage);
+                    stage = stage == STAGE ? 0 : STAGE;
+                }
+            }
         }
     }
     wait_loads<0>();  // nothing is on its way to LDS any more,
@@ -476,51 +534,57 @@ template <int INPUT, int FORMAT, int OUT> hipError_t launch_rows(RowsParams p, h
 int w_scale_rows(int N, int w_block_rows) { return w_block_rows == 1 ? N : (N + kBlock8 - 1) / kBlock8; }
 
 struct Plan8 {
-    int tile, parts, kb_per_part;  // tile: the square tile's edge
+    int rows, columns;  // of the tile
+    int parts, kb_per_part;
+    long tiles;
 };
 
-// The tile and the parts that K is cut into: the least of what a launch takes by the busiest CU's work.  A tile's step alone on its CU takes
-// `alone` us (latency), a step of one among as many as the CU holds `among`, its way out `out`; parts are written in fp32, read and added
+// The tile and the parts that K is cut into: the least of what a launch takes by the busiest CU's work.  A step of one of the tiles that a CU holds at
+// once takes `alone` us (latency) or, of all its tiles, `among` (throughput), a tile's way out `out`; parts are written in fp32, read and added
 // up by a launch of their own.  Constants fitted to every (tile, parts) of 60 products of 33 .. 16384 rows, 64 .. 8192 columns and K on an MI355X;
-// what the rule picks takes 0.7 % (16-bit output) and 0.2 % (fp32) longer than the best of them in the mean, at most 13 % (8192 x 8192 x 1024).
-struct TileTimes { double alone, among, out; int held; };
+// what the rule picks takes 0.7 % (16-bit output) and 0.3 % (fp32) longer than the best of them in the mean, at most 17 % (40 x 64 x 8192).
+struct TileTimes { int rows, columns, held; double alone, among, out; };
 
 Plan8 plan8(int out, int M, int N, int KB)
 {
-    constexpr int kEdges[] = {64, 128, 256};
-    constexpr TileTimes kFast[] = {{0.31, 0.194, 0.72, 3}, {0.74, 0.473, 1.56, 2}, {1.43, 1.454, 5.2, 1}}, kExact[] = {{0.42, 0.32, 0.47, 3}, {1.04, 0.844, 1.27, 2}};
-    const TileTimes *const times = out == 0 ? kExact : kFast;
-    const double join = out == 0 ? 2.8 : 1.8, join_part = out == 0 ? 0.956e-6 : 0.865e-6, join_out = 0.1e-6;
-    Plan8 best = {64, 1, KB};
+    constexpr TileTimes kFast[] = {{64, 64, 3, 0.063, 0.172, 0.82}, {64, 128, 2, 0.003, 0.238, 1.39}, {128, 128, 2, 0.557, 0.481, 1.81}, {256, 256, 1, 1.448, 0.067, 6.1}};
+    constexpr TileTimes kExact[] = {{64, 64, 3, 0.371, 0.242, 0.7}, {64, 128, 2, 0.553, 0.336, 1.32}, {128, 128, 2, 1.22, 0.716, 1.65}};
+    const double join = out == 0 ? 2.5 : 1.8, join_part = out == 0 ? 0.936e-6 : 0.638e-6, join_out = out == 0 ? 0.008e-6 : 0.238e-6;
+    Plan8 best = {};
     double least = 1e30;
-    for (int i = 0; i < (out == 0 ? 2 : 3); i++) {
-        const long edge = kEdges[i], tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
+    for (int i = 0; i < (out == 0 ? 3 : 4); i++) {
+        const TileTimes &tile = out == 0 ? kExact[i] : kFast[i];
+        const long tiles = ((M + (long)tile.rows - 1) / tile.rows) * ((N + (long)tile.columns - 1) / tile.columns);
         for (int parts = 1; parts <= 16 && parts <= KB; parts *= 2) {
             if (parts > 1 && tiles * parts > 2048) break;
             const int steps = (KB + parts - 1) / parts;
             if ((KB + steps - 1) / steps != parts) continue;
-            const long each = (tiles * parts + 255) / 256, rounds = (each + times[i].held - 1) / times[i].held;
-            const double alone = times[i].alone * (double)rounds, among = times[i].among * (double)each;
-            double t = steps * (alone > among ? alone : among) + times[i].out * (double)each * (parts > 1 || out == 0 ? 2 : 1);
+            const long each = (tiles * parts + 255) / 256, rounds = (each + tile.held - 1) / tile.held;
+            const double alone = tile.alone * (double)rounds, among = tile.among * (double)each;
+            double t = steps * (alone > among ? alone : among) + tile.out * (double)each * (parts > 1 || out == 0 ? 2 : 1);
             if (parts > 1) t += join + (parts * join_part + join_out) * (double)M * (double)N;
             if (t < least) {
                 least = t;
-                best = {(int)edge, parts, steps};
+                best = {tile.rows, tile.columns, parts, steps, tiles};
             }
         }
     }
     return best;
 }
 
-template <int FORMAT, int OUT, bool EXACT> hipError_t launch_tiles(int tile, unsigned groups, const TileParams &p, hipStream_t stream)
+int threads_of(const Plan8 &plan) { return plan.rows == 256 ? 512 : 256; }
+
+template <int FORMAT, int OUT, bool EXACT> hipError_t launch_tiles(const Plan8 &plan, const TileParams &p, hipStream_t stream)
 {
+    const unsigned groups = (unsigned)(plan.tiles * plan.parts);
     if constexpr (!EXACT)
-        if (tile == 256) {
-            linear8_tiles<256, 256, 2, 4, 2, FORMAT, OUT, EXACT><<<groups, 512, 0, stream>>>(p);
+        if (plan.rows == 256) {
+            linear8_tiles<256, 256, 2, 4, 2, FORMAT, OUT, EXACT><<<groups, threads_of(plan), 0, stream>>>(p);
             return hipGetLastError();
         }
-    if (tile == 128) linear8_tiles<128, 128, 2, 2, 2, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
-    else linear8_tiles<64, 64, 2, 2, 3, FORMAT, OUT, EXACT><<<groups, 256, 0, stream>>>(p);
+    if (plan.rows == 128) linear8_tiles<128, 128, 2, 2, 2, FORMAT, OUT, EXACT><<<groups, threads_of(plan), 0, stream>>>(p);
+    else if (plan.columns == 128) linear8_tiles<64, 128, 2, 2, 3, FORMAT, OUT, EXACT><<<groups, threads_of(plan), 0, stream>>>(p);
+    else linear8_tiles<64, 64, 2, 2, 3, FORMAT, OUT, EXACT><<<groups, threads_of(plan), 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -532,13 +596,12 @@ template <int FORMAT> hipError_t launch_format(int out, const Linear8Args &a, vo
         return out == 0 ? launch_rows<3, FORMAT, 0>(p, stream) : out == 1 ? launch_rows<3, FORMAT, 1>(p, stream) : launch_rows<3, FORMAT, 2>(p, stream);
     }
     const Plan8 plan = plan8(out, a.M, a.N, a.KB);
-    const int tiles_m = (a.M + plan.tile - 1) / plan.tile, tiles_n = (a.N + plan.tile - 1) / plan.tile;
+    const int tiles_m = (a.M + plan.rows - 1) / plan.rows, tiles_n = (a.N + plan.columns - 1) / plan.columns;
     TileParams p = {a.qx, a.sx, a.qw, a.sw, plan.parts > 1 ? workspace : a.y, a.M, a.N, a.KB, scale_rows, plan.kb_per_part, tiles_m, tiles_n};
-    const unsigned groups = (unsigned)tiles_m * (unsigned)tiles_n * (unsigned)plan.parts;
     if (plan.parts == 1)
-        return out == 0 ? launch_tiles<FORMAT, 0, true>(plan.tile, groups, p, stream)
-                        : out == 1 ? launch_tiles<FORMAT, 1, false>(plan.tile, groups, p, stream) : launch_tiles<FORMAT, 2, false>(plan.tile, groups, p, stream);
-    const hipError_t e = out == 0 ? launch_tiles<FORMAT, 0, true>(plan.tile, groups, p, stream) : launch_tiles<FORMAT, 0, false>(plan.tile, groups, p, stream);
+        return out == 0 ? launch_tiles<FORMAT, 0, true>(plan, p, stream)
+                        : out == 1 ? launch_tiles<FORMAT, 1, false>(plan, p, stream) : launch_tiles<FORMAT, 2, false>(plan, p, stream);
+    const hipError_t e = out == 0 ? launch_tiles<FORMAT, 0, true>(plan, p, stream) : launch_tiles<FORMAT, 0, false>(plan, p, stream);
     if (e != hipSuccess) return e;
     const long count = (long)a.M * a.N;
     const unsigned joins = (unsigned)((count + 1023) / 1024);
@@ -562,15 +625,14 @@ long linear8_threads(int out_dtype, int M, int N, int KB)
 {
     if (rows_fit(M, KB)) return 0;  // (at most 512 workgroups)
     const Plan8 plan = plan8(out_dtype, M, N, KB);
-    const long edge = plan.tile;
-    return ((M + edge - 1) / edge) * ((N + edge - 1) / edge) * plan.parts * (edge == 256 ? 512 : 256);
+    return plan.tiles * plan.parts * threads_of(plan);
 }
 
 int linear8_way(int out_dtype, int M, int N, int KB)
 {
     if (rows_fit(M, KB)) return 0;
     const Plan8 plan = plan8(out_dtype, M, N, KB);
-    return plan.tile * 100 + plan.parts;
+    return (plan.rows + plan.columns) / 2 * 100 + plan.parts;
 }
 
 hipError_t launch_linear8(int out_dtype, int x_format, const Linear8Args &a, void *workspace, hipStream_t stream)

@@ -11,10 +11,12 @@ from tab_amd import nn as tab_nn
 
 P = 4096  # an aligned address that is never dereferenced: every call below fails its checks
 
-# (0 fp32 or 1 16-bit output, M, N, K, edge of the tile * 100 + parts of K): every tile, K whole and in parts, one step of K and many
-WAYS = [(0, 34, 35, 60, 6401), (0, 33, 34, 940, 6408), (0, 2970, 643, 60, 12801), (0, 2100, 4003, 500, 12801), (0, 514, 661, 8873, 12808),
-        (1, 34, 35, 60, 6401), (1, 33, 39, 1412, 6404), (1, 2970, 643, 60, 12801), (1, 2100, 2050, 1100, 12801), (1, 654, 1476, 8658, 12804),
-        (1, 1425, 8304, 61, 25601), (1, 2300, 4099, 4100, 25601), (1, 1031, 2893, 11022, 25604)]
+# (0 fp32 or 1 16-bit output, M, N, K, half of the tile's rows + columns * 100 + parts of K): every tile, K whole and in parts, one step of K and
+# many
+WAYS = [(0, 34, 35, 60, 6401), (0, 33, 34, 940, 6408), (0, 65, 8299, 63, 9601), (0, 578, 1252, 6526, 9604), (0, 2970, 643, 60, 12801),
+        (0, 2100, 4003, 500, 12801), (1, 34, 35, 60, 6401), (1, 37, 33, 2708, 6408), (1, 65, 8299, 63, 9601), (1, 2100, 2050, 1100, 9601),
+        (1, 260, 771, 6986, 9604), (1, 2970, 643, 60, 12801), (1, 2322, 833, 903, 12801), (1, 1425, 8304, 61, 25601),
+        (1, 3343, 3616, 252, 25601), (1, 1283, 9011, 2007, 25601), (1, 2214, 2718, 10855, 25602)]
 
 
 def _refuses(status, message, code=-1):
