@@ -135,7 +135,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const TileParam
     using T = typename Element<OUT>::type;
     constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, TM = BM / WM / 16, TN = BN / WN / 16;
     constexpr int NUMBERS = (BM + BN) * kBlock8, STAGE = NUMBERS + 4 * THREADS;
-    constexpr int LOADS = (BM + BN) / 8 / WAVES, A_LOADS = BM / 8 / WAVES;
+    constexpr int W_WAVES = WAVES == 8 ? WN : WAVES;  // of eight waves the first four load W and the scales
+    constexpr int A_LOADS = BM / 8 / WAVES, W_LOADS = BN / 8 / W_WAVES, LOADS = A_LOADS + W_LOADS;
     static_assert(BM + BN <= THREADS, "a lane loads one scale");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
 
@@ -151,18 +152,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const TileParam
     const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64), wm = wave / WN, wn = wave % WN, l16 = lane % 16, quarter = lane / 16;
     const int row_bytes = p.KB * kBlock8, rows_x = min(BM, p.M - m0), rows_w = min(BN, p.N - n0);
     const uint8_t *const qx = p.qx + (long)m0 * row_bytes, *const qw = p.qw + (long)n0 * row_bytes;
-    // load i of a wave is eight rows of an operand's tile, eight lanes a row: of W all waves take turns, of X those that multiply the rows
+    // load i of a wave is eight rows of an operand's tile, eight lanes a row: of W the waves take turns, of X those that multiply the rows
     const int first_x = wm * (BM / WM) + wn * 8, first_w = wave * 8;
     const uint32_t x_at = (uint32_t)(first_x + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
     const uint32_t w_at = (uint32_t)(first_w + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
-    // this lane's scale has place t of X's or t - BM of W's; the scales of a lane's groups of 16 rows are side by side.  (A wave's scales
-    // are all of X or all of W.)
-    const bool scale_x = wave * 64 < BM, row_scales = p.w_scale_rows == p.N;
-    const int groups = scale_x ? TM : TN, place = scale_x ? t : t - BM, scale_row = place / (16 * groups) * (16 * groups) + place % groups * 16 + place / groups % 16;
-    const uint32_t scale_offset = (uint32_t)(scale_x || row_scales ? scale_row : (n0 + scale_row) / kBlock8 - n0 / kBlock8);
-    const int scale_step = scale_x ? p.M : p.w_scale_rows;
-    const uint8_t *scales = (scale_x ? p.sx + m0 : p.sw + (row_scales ? n0 : n0 / kBlock8)) + (long)kb0 * scale_step;
-    const int scale_rows = scale_x ? rows_x : wave * 64 >= BM + BN ? 0 : row_scales ? rows_w : (n0 + rows_w - 1) / kBlock8 - n0 / kBlock8 + 1;
+    // A lane loads one scale: place t of X's, then of W's (of eight waves the first four load one of each).  The scales of a lane's groups of 16 rows are
+    // side by side.  (A wave's scales are all of X or all of W.)
+    const bool row_scales = p.w_scale_rows == p.N;
+    struct Scales { const uint8_t *at; int step, rows; uint32_t offset; };
+    auto scales_of = [&](bool x, int place, bool any) {
+        const int groups = x ? TM : TN, row = place / (16 * groups) * (16 * groups) + place % groups * 16 + place / groups % 16, step = x ? p.M : p.w_scale_rows;
+        return Scales{(x ? p.sx + m0 : p.sw + (row_scales ? n0 : n0 / kBlock8)) + (long)kb0 * step, step,
+                      !any ? 0 : x ? rows_x : row_scales ? rows_w : (n0 + rows_w - 1) / kBlock8 - n0 / kBlock8 + 1,
+                      (uint32_t)(x || row_scales ? row : (n0 + row) / kBlock8 - n0 / kBlock8)};
+    };
+    const bool scale_x = WAVES == 8 || wave * 64 < BM;
+    Scales scales = scales_of(scale_x, scale_x ? t : t - BM, wave * 64 < BM + BN), more_scales = scales_of(false, t, true);
     const uint32_t lds_at = lds_address(lds);
     // the rows of an operand's tile are one buffer: rows past its end, and with a size of zero all of it, load as zeros
     const i32x4 x_rows = buffer(qx, rows_x * row_bytes), w_rows = buffer(qw, rows_w * row_bytes);
@@ -175,10 +180,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const TileParam
         if (i < A_LOADS) {
             to_lds16(sized(x_rows, live), to + (uint32_t)(first_x + i * 8 * WN) * kBlock8, x_at + (uint32_t)(i * 8 * WN * row_bytes + kb * kBlock8));
         } else if (i < LOADS) {
-            to_lds16(sized(w_rows, live), to + (uint32_t)(BM + first_w + (i - A_LOADS) * 8 * WAVES) * kBlock8, w_at + (uint32_t)((i - A_LOADS) * 8 * WAVES * row_bytes + kb * kBlock8));
+            to_lds16(sized(w_rows, live), to + (uint32_t)(BM + first_w + (i - A_LOADS) * 8 * W_WAVES) * kBlock8, w_at + (uint32_t)((i - A_LOADS) * 8 * W_WAVES * row_bytes + kb * kBlock8));
         } else {
-            to_lds1(buffer(scales, live ? scale_rows : 0), to + (uint32_t)(NUMBERS + wave * 256), scale_offset);
-            scales += scale_step;
+            Scales &of = i == LOADS ? scales : more_scales;
+            to_lds1(buffer(of.at, live ? of.rows : 0), to + (uint32_t)(NUMBERS + (i - LOADS) * 4 * BM + wave * 256), of.offset);
+            of.at += of.step;
         }
     };
 
@@ -247,53 +253,67 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const TileParam
         asm volatile("" ::: "memory");
     };
     auto all_read = [] { __builtin_amdgcn_s_waitcnt(0xc07f); };  // this wave's reads of LDS are done
-    #pragma unroll
-    for (int k = 0; k < STAGES; k++)
+        auto load_first = [&] {
 #pragma unroll
-        for (int i = 0; i <= LOADS; i++) load(k * STAGE, kb0 + k, i);
+        for (int k = 0; k < STAGES; k++)
+#pragma unroll
+            for (int i = 0; i <= LOADS; i++) load(k * STAGE, kb0 + k, i);
+    };
     if constexpr (WAVES == 8) {
         // Two waves a SIMD take turns: while one multiplies the other reads, a barrier at every change.  Slot 2s: the first four waves read step s, the
         // others multiply step s - 1; slot 2s + 1 the other way round.  Of a step's part of LDS the rows of X that only the first four waves
-        // read are free from slot 2s + 1 on, the rest from slot 2s + 2; there the loads of step s + 2 go out.  Slot 2s + 4 reads them, and every
-        // wave has waited for its own by the barrier before.
+        // read are free from slot 2s + 1 on, where those load theirs of step s + 2; the rest from slot 2s + 2 on, the slot in which the first four
+        // waves load W and the scales of step s + 2 (which slot 2s + 4 reads), and 2s + 3, in which the others load their rows of X (for slot 2s + 5).
+        // Few loads go out between the products: a wave that waits to get one out does not multiply.
         static_assert(STAGES == 2, "two steps in LDS");
         Operands o;
-        wait_loads<LOADS + 1>();
-        barrier();
         if (wm == 0) {
+#pragma unroll
+            for (int i = 0; i < LOADS + 2; i++) load(0, kb0, i);
+#pragma unroll
+            for (int i = 0; i < A_LOADS; i++) load(STAGE, kb0 + 1, i);
+            wait_loads<A_LOADS>();
+            barrier();
             for (int kb = kb0; kb < kb1; kb++) {
                 const int stage = (kb - kb0) & 1 ? STAGE : 0;
-                if (kb > kb0) {
-#pragma unroll
-                    for (int i = A_LOADS; i <= LOADS; i++) load(STAGE - stage, kb + 1, i);
-                }
                 read_all(o, stage);
+#pragma unroll
+                for (int i = A_LOADS; i < LOADS + 2; i++) load(STAGE - stage, kb + 1, i);
                 all_read();
                 barrier();
                 __builtin_amdgcn_s_setprio(1);
-                multiply(o, A_LOADS, [&](int i) { load(stage, kb + 2, i); });
+                multiply(o, TM * TN, [&](int i) {
+                    if (i % (TM * TN / A_LOADS) == 0) load(stage, kb + 2, i / (TM * TN / A_LOADS));
+                });
                 __builtin_amdgcn_s_setprio(0);
                 wait_loads<A_LOADS>();
                 barrier();
             }
             barrier();
         } else {
+#pragma unroll
+            for (int i = 0; i < A_LOADS; i++) load(0, kb0, i);
+            wait_loads<0>();
+            barrier();
             barrier();
             for (int kb = kb0; kb < kb1; kb++) {
                 const int stage = (kb - kb0) & 1 ? STAGE : 0;
                 read_all(o, stage);
+#pragma unroll
+                for (int i = 0; i < A_LOADS; i++) load(STAGE - stage, kb + 1, i);
                 all_read();
-                wait_loads<0>();
                 barrier();
                 __builtin_amdgcn_s_setprio(1);
-                multiply(o, LOADS + 1, [&](int i) { load(stage, kb + 2, i); });
+                multiply(o, 0, [](int) {});
                 __builtin_amdgcn_s_setprio(0);
+                wait_loads<0>();
                 barrier();
             }
         }
     } else if constexpr (EXACT && BM * BN > 64 * 128) {
         // no registers for two steps' operands
         static_assert(STAGES == 2, "steps in LDS");
+        load_first();
         Operands o;
         for (int kb = kb0, stage = 0; kb < kb1; kb++, stage = STAGE - stage) {
             wait_loads<LOADS + 1>();  // this wave's part of the step has landed,
@@ -315,6 +335,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const TileParam
                 if (i <= LOADS) load(stage, kb + STAGES, i);
             });
         };
+        load_first();
         wait_loads<(STAGES - 1) * (LOADS + 1)>();
         barrier();
         read_all(even, 0);
