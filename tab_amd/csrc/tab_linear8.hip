@@ -125,7 +125,15 @@ template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v, int 
     }
 }
 
-// A workgroup of WM x WN waves makes a BM x BN tile of Y.  A step is one block of K: 128 bytes of each of the tile's rows and their scales,
+// A workgroup of WM x WN waves makes a BM x BN tile of Y, for more rows than linear8_rows takes; bound by the matrix instructions and, the smaller the tile,
+// by the way of its operands into LDS (54 bytes a clock and CU measured; reads of LDS reach 200).  What cost most was a wave that waits to get a load
+// out, or whose scalar instructions make the load's address, and does not multiply meanwhile.  So a step's operands are read from LDS while the
+// step before is multiplied, loads, reads and products alternate, and a load takes two scalar instructions and one addition.
+//   256 x 256  8192^3 432-456 us, 2.4-2.5 PFLOP/s (a library's fp8 product with one scale a tensor 361); all loads between the products 426-478
+//   128 x 128  4096 x 2048 x 4096 37-41 us, 1.7-1.9 PFLOP/s
+//   64 x 128   512 x 4096 x 4096 13.8 us, 1.25 PFLOP/s (64 x 64 16.4; both 19 with read and multiplied in turn)
+//   64 x 64    128 x 4096 x 4096 9.0 us (14.0 in turn); fp32 1000 x 776 x 520 6.6 us
+// A step is one block of K: 128 bytes of each of the tile's rows and their scales,
 // straight from global memory into one of STAGES parts of LDS.  A row is eight pieces of 16 bytes; row r has piece g at place g ^ (r & 7), so
 // that lanes that read at once meet different banks.  Which piece a lane multiplies is free as long as both operands agree, since a block
 // has one scale.
@@ -404,7 +412,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const TileParam
     }
 }
 
-// The parts of a K that was split over workgroups, added up in their order and rounded once.
+// The parts of a K that was split over workgroups, added up in their order and rounded once (so the same call gives the same bits, which sums by
+// atomics would not).  Memory bound, and a launch: about 2.5 us for 4 parts of 64 x 4096.
 template <int OUT> __global__ __launch_bounds__(256) void linear8_join(const float *parts, void *y, long count, int n)
 {
     using T = typename Element<OUT>::type;
@@ -427,6 +436,9 @@ template <int OUT> __global__ __launch_bounds__(256) void linear8_join(const flo
 // K in turn, each lane loads its 2 x 16 bytes of a block of QW itself, AHEAD blocks at a time, and the waves' sums meet in LDS, added up in a
 // fixed order.  X lies in LDS as packed numbers (rows 16 bytes more than whole blocks apart, so that 8 rows' pieces meet different banks) and scales:
 // INPUT 0 .. 2: fp32 / bf16 / fp16, quantized by the workgroup on the way (a block of a row is 16 lanes of eight); 3: packed.
+// One row of 4096 by 4096 x 4096: 5.2-6.0 us with its launch, 16.9 MB at 2.8-3.2 TB/s (through the tiles and a launch of the quantizer 14).  24 rows of
+// 2050 (fp16) by 1003: 9.3-10.4 us, bound by every workgroup's conversion of all of X, which costs less than a launch for it alone; 16 waves
+// instead of 8 took 5.9-6.4 and 10.9-11.2 us.
 struct RowsParams {
     const void *x;
     const uint8_t *sx, *qw, *sw;

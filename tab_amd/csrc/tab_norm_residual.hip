@@ -72,6 +72,7 @@ template <int LANES> struct RowsOfGroup {
 };
 
 // OUT: 0 no H, 1 H in the streams' type, 2 H packed (E4M3, 1 x 128 blocks)
+// bf16 16384 x 4096 with 16 gates: 109-117 us, 537 MB at 4.6-4.9 TB/s (a copy 5.1); one token of 4096 with packed H 2.9 us, its launch.
 template <int DTYPE, int GATE, bool BLOCK, int OUT, int LANES, int RUNS>
 __global__ __launch_bounds__(RowsOfGroup<LANES>::THREADS) void norm_residual(const NormParams p)
 {
@@ -183,6 +184,8 @@ __global__ __launch_bounds__(RowsOfGroup<LANES>::THREADS) void norm_residual(con
 //   s = sum over a gate's rows of t Y q:  dgate = s w_post,  dw_post = sum over gates of gate s
 // p and q are made anew from R and Y, which are here anyway, so the forward pass keeps nothing.  Sums over rows: a group of lanes adds up
 // its own rows in registers and leaves them in the workspace, a second launch adds the groups up in a fixed order.
+// bf16 16384 x 4096 with 16 gates: 162-167 us, 805 MB at 4.8-5.0 TB/s, and 11-13 for the join; fp32 777 x 1531 with a gate for each row: 16 and 3-4
+// (two rows to a group; with four 19 and 3-4).  The next row is loaded before this one's sums are taken, as a row alone is all latency.
 
 struct NormGradParams {
     const void *dr, *dh, *r, *y, *gate;

@@ -3,7 +3,7 @@
 //
 //   amax = largest finite |x| of the block;  scale = smallest 2^e >= 2^-126 with amax <= MAX * 2^e;  q = nearest8(x / scale)
 //
-// Memory bound: reads X once, writes a byte per number and layout.
+// Memory bound: reads X once, writes a byte per number and layout.  A large copy reaches 5.1 TB/s on an MI355X (8.4 within the last cache).
 #include "tab_blocks8.h"
 #include "tab_common.h"
 
@@ -21,7 +21,9 @@ struct QuantizeParams {
     Div32 div_kb;
 };
 
-// Rows of X alone, 1 x 128 blocks: a workgroup takes 32 rows of one block, a row is 16 lanes of eight elements.
+// Rows of X alone, 1 x 128 blocks: a workgroup takes 32 rows of one block, a row is 16 lanes of eight elements: the largest of a block stays in
+// a row of 16 lanes (four exchanges, no LDS), a lane's load is 16 bytes and its store eight.  Small workgroups without a loop, since nothing is kept
+// from one block to the next.  bf16 8192 x 8192: 36-38 us, 202 MB at 5.3-5.6 TB/s.
 template <int DTYPE, int FORMAT>
 __global__ __launch_bounds__(kThreads) void quantize8_rows(const QuantizeParams p)
 {
@@ -125,6 +127,10 @@ __device__ __forceinline__ void special_tile(const QuantizeParams &p, uint32_t *
 }
 
 // A tile of 128 x 128: a lane holds 8 rows of 8 columns.  X^T goes through LDS, so that its rows are written as whole cache lines.
+// Both layouts leave one reading of X.  What bounded it besides memory was the conversion (an element took its own instructions in each layout):
+// two elements an instruction throughout, four waves a SIMD, infinities and NaN in a path of their own that a tile without them skips.
+// bf16 8192 x 4096, both layouts: 23 us, 135 MB at 5.8 TB/s (element by element 32); fp32 1531 x 1333 in 128 x 128 blocks 5.4 us (launch and
+// one round trip to memory).
 template <int DTYPE, int FORMAT, bool SQUARE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void quantize8_tile(const QuantizeParams p)
 {
