@@ -299,7 +299,7 @@ int tab_quantize8(const void *dev_X, int dtype, int M, int K, long ldx, int bloc
 
 /*
  * Y (M x N, rows contiguous) = X (M x K, packed) times the transpose of W (N x K, packed in E4M3 with blocks of w_block_rows x 128).  An fp32 Y
- * is the sum of exact products in fp32 (operands below 2^-126 may count as zeros); towards a 16-bit Y the products of eight neighbours in K keep
+ * is the sum of exact products in fp32 (operands below 2^-126 may count as zeros, one that rounds to 2^128 as an infinity); towards a 16-bit Y the products of eight neighbours in K keep
  * 13 bits below the largest of them, some 1.5e-5 of Y's size.
  *   workspace  tab_linear8_packed_workspace_bytes(out_dtype, M, N, K) bytes, 16-byte aligned; 0 bytes: NULL will do
  */

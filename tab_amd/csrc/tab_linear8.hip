@@ -575,14 +575,14 @@ struct Plan8 {
 // The tile and the parts that K is cut into: the least of what a launch takes by the busiest CU's work.  A step of one of the tiles that a CU holds at
 // once takes `alone` us (latency) or, of all its tiles, `among` (throughput), a tile's way out `out`; parts are written in fp32, read and added
 // up by a launch of their own.  Constants fitted to every (tile, parts) of 60 products of 33 .. 16384 rows, 64 .. 8192 columns and K on an MI355X;
-// what the rule picks takes 0.7 % (16-bit output) and 0.3 % (fp32) longer than the best of them in the mean, at most 17 % (40 x 64 x 8192).
+// what the rule picks takes 0.6 % (16-bit output) and 0.3 % (fp32) longer than the best of them in the mean, at most 14 % (40 x 64 x 8192).
 struct TileTimes { int rows, columns, held; double alone, among, out; };
 
 Plan8 plan8(int out, int M, int N, int KB)
 {
-    constexpr TileTimes kFast[] = {{64, 64, 3, 0.063, 0.172, 0.82}, {64, 128, 2, 0.003, 0.238, 1.39}, {128, 128, 2, 0.557, 0.481, 1.81}, {256, 256, 1, 1.448, 0.067, 6.1}};
+    constexpr TileTimes kFast[] = {{64, 64, 3, 0.05, 0.174, 0.8}, {64, 128, 2, 0.171, 0.242, 1.37}, {128, 128, 2, 0.571, 0.473, 1.69}, {256, 256, 1, 1.235, 1.125, 6.25}};
     constexpr TileTimes kExact[] = {{64, 64, 3, 0.371, 0.242, 0.7}, {64, 128, 2, 0.553, 0.336, 1.32}, {128, 128, 2, 1.22, 0.716, 1.65}};
-    const double join = out == 0 ? 2.5 : 1.8, join_part = out == 0 ? 0.936e-6 : 0.638e-6, join_out = out == 0 ? 0.008e-6 : 0.238e-6;
+    const double join = out == 0 ? 2.5 : 1.9, join_part = out == 0 ? 0.936e-6 : 0.747e-6, join_out = out == 0 ? 0.008e-6 : 0;
     Plan8 best = {};
     double least = 1e30;
     for (int i = 0; i < (out == 0 ? 3 : 4); i++) {
