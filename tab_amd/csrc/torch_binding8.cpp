@@ -287,6 +287,9 @@ Tensor matrix(const Tensor &x)
     return rows || m.size(1) == 1 ? (m.size(1) == 1 ? m.contiguous() : m) : m.contiguous();
 }
 
+// An output in its final shape that is no view: one of an autograd function that is a view may not be changed in place (a bias added, an activation).
+Tensor shaped(const Tensor &t, c10::IntArrayRef sizes) { return t.sizes() == sizes ? t : at::_unsafe_view(t, sizes); }
+
 // y = Q(x) Q(w)^T with gradients dx = Q(dy) Q(w), dw = Q(dy^T) Q(x^T)^T: three products of packed operands.  What the backward pass multiplies is
 // packed in the forward pass, from the same reading of x and w.
 struct Linear8Function : torch::autograd::Function<Linear8Function> {
@@ -303,7 +306,7 @@ struct Linear8Function : torch::autograd::Function<Linear8Function> {
         ctx->saved_data["shape"] = x.sizes().vec();
         auto shape = x.sizes().vec();
         shape.back() = N;
-        return y.view(shape);
+        return shaped(y, shape);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads)
     {
@@ -372,7 +375,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         const OptionalTensor y2 = y ? OptionalTensor(matrix(*y)) : y;
         const int M = as_size(x2.size(0), "rows of x"), D = as_size(x2.size(1), "columns of x");
         auto out = norm_forward(x2, y2, gate, w_post, w_pre, alpha, eps, M, D, (int)output);
-        for (Tensor &t : out) t = t.view(x.sizes());
+        for (Tensor &t : out) t = shaped(t, x.sizes());
         ctx->save_for_backward({y ? out[0] : x2.contiguous(), y ? y2->contiguous() : Tensor(), defined(gate), defined(w_post), defined(w_pre)});
         ctx->saved_data["alpha"] = alpha;
         ctx->saved_data["eps"] = eps;
@@ -393,8 +396,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         auto whole = [](const Tensor &t) { return t.defined() ? OptionalTensor(t.contiguous()) : c10::nullopt; };
         const auto out = norm_backward(whole(dr), whole(dh), saved[0], optional(saved[1]), optional(saved[2]), optional(saved[3]), optional(saved[4]),
                                        ctx->saved_data["alpha"].toDouble(), ctx->saved_data["eps"].toDouble(), M, D);
-        auto shaped = [&](const OptionalTensor &t) { return t ? t->view(like.sizes()) : Tensor(); };
-        return {shaped(out[0]), shaped(out[1]), defined(out[2]), defined(out[3]), defined(out[4]), none, none, none};
+        auto like_it = [&](const OptionalTensor &t) { return t ? t->view(like.sizes()) : Tensor(); };
+        return {like_it(out[0]), like_it(out[1]), defined(out[2]), defined(out[3]), defined(out[4]), none, none, none};
     }
 };
 

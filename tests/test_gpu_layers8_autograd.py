@@ -1,0 +1,59 @@
+"""The differentiable 8-bit layers and norms as parts of a user's program: outputs changed in place, weights of other shapes and types, blocks
+without a gradient, layers moved and converted."""
+import copy
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import layers8_reference as ref
+import tab_amd
+from tab_amd import nn as tab_nn
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(shape, seed, scale=1.0):
+    return torch.randn(shape, generator=torch.Generator("cpu").manual_seed(seed)) * scale
+
+
+def _leaves(*tensors):
+    return [t.detach().cuda().requires_grad_() for t in tensors]
+
+
+@pytest.mark.parametrize("shape", [(6, 200), (2, 3, 200)])
+def test_linear8_output_changed_in_place(shape):
+    """As after torch's own linear: a bias added and an activation applied in place, and the gradients of the same out of place."""
+    x, w, b = _rand(shape, 1), _rand((30, 200), 2, 0.1), _rand((30,), 3)
+    dy = _rand((*shape[:-1], 30), 4).cuda()
+    a = _leaves(x, w, b)
+    y = tab_nn.linear8(a[0], a[1])
+    y += a[2]
+    torch.relu_(y)
+    c = _leaves(x, w, b)
+    want = torch.relu(tab_nn.linear8(c[0], c[1]) + c[2])
+    assert torch.equal(y, want)
+    for got, expected in zip(torch.autograd.grad(y, a, dy), torch.autograd.grad(want, c, dy)):
+        assert torch.equal(got, expected)
+
+
+@pytest.mark.parametrize("shape", [(6, 200), (2, 3, 200)])
+def test_norm_outputs_changed_in_place(shape):
+    """H is nobody's but the caller's.  R is what the backward pass reads: once changed, it says so."""
+    x, y, gate, w = _rand(shape, 5), _rand(shape, 6, 9.0), _rand((2, 200), 7), _rand((200,), 8)
+    dh = _rand(shape, 9).cuda()
+    for block in (True, False):
+        def norm(leaves):
+            return tab_nn.norm_residual(leaves[0], leaves[1], leaves[2], leaves[3], leaves[3], 0.9) if block else tab_nn.norm_residual(leaves[0], w_pre=leaves[3])
+        a, c = _leaves(x, y, gate, w), _leaves(x, y, gate, w)
+        h, want = norm(a)[-1], norm(c)[-1] * 3.0
+        h *= 3.0
+        assert torch.equal(h, want)
+        wanted = (0, 1, 2, 3) if block else (0, 3)
+        for got, expected in zip(torch.autograd.grad(h, [a[i] for i in wanted], dh), torch.autograd.grad(want, [c[i] for i in wanted], dh)):
+            assert torch.equal(got, expected)
+    a = _leaves(x, y, gate, w)
+    r, h = tab_nn.norm_residual(*a, a[3], 0.9)
+    r += 1.0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, a, dh)
