@@ -276,8 +276,20 @@ int as_size(int64_t v, const char *name)
     return (int)v;
 }
 
+// There are no formulas for tangents (torch.autograd.forward_ad, one level): an input that has one is an error, as the kernels would drop it.
+void no_tangent(std::initializer_list<const Tensor *> tensors)
+{
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor *t : tensors)
+        TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), "the 8-bit layers and the norms have no derivatives in forward mode (an input has a tangent)");
+}
+
 // The kernels' gradients are no graph: asking for their derivatives is an error, not a zero.
-void no_second_derivative() { TORCH_CHECK(!at::GradMode::is_enabled(), "the 8-bit layers and the norms have no second derivatives (create_graph)"); }
+void no_second_derivative(const torch::autograd::variable_list &grads)
+{
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the 8-bit layers and the norms have no second derivatives (create_graph)");
+    for (const Tensor &g : grads) no_tangent({&g});
+}
 
 // Rows of the last dimension as a matrix with contiguous rows, and the same for the gradients.
 Tensor matrix(const Tensor &x)
@@ -310,7 +322,7 @@ struct Linear8Function : torch::autograd::Function<Linear8Function> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads)
     {
-        no_second_derivative();
+        no_second_derivative(grads);
         const auto saved = ctx->get_saved_variables();
         const auto sizes = ctx->saved_data["sizes"].toIntVector();
         const int M = (int)sizes[0], N = (int)sizes[1], K = (int)sizes[2], format = (int)sizes[3];
@@ -342,6 +354,7 @@ Tensor linear8(const Tensor &x, const Tensor &w, int grad_format)
     format_type(grad_format);
     TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1), "x (..., K) and w (N, K) must agree in K, got ", x.sizes(), " and ", w.sizes());
     TORCH_CHECK(x.numel() > 0 && w.numel() > 0, "x and w must not be empty, got ", x.sizes(), " and ", w.sizes());
+    no_tangent({&x, &w});
     check_device(w, x, "w");
     if (wants_gradient({&x, &w})) return Linear8Function::apply(x, w, (int64_t)grad_format);
     const Tensor x2 = matrix(x), w2 = matrix(w);
@@ -356,6 +369,7 @@ Tensor linear8(const Tensor &x, const Tensor &w, int grad_format)
 Tensor linear8_packed_weight(const Tensor &x, const Tensor &QW, const Tensor &SW, int N, int K)
 {
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) == K && x.numel() > 0, "input must be (..., ", K, ") and not empty, got ", x.sizes());
+    no_tangent({&x});
     TORCH_CHECK(!wants_gradient({&x}), "a packed weight is for inference: take nn.linear8 for training");
     const Tensor x2 = matrix(x);
     auto shape = x.sizes().vec();
@@ -385,7 +399,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads)
     {
-        no_second_derivative();
+        no_second_derivative(grads);
         const auto saved = ctx->get_saved_variables();
         const bool block = saved[1].defined();
         const int64_t output = ctx->saved_data["output"].toInt();
@@ -409,6 +423,7 @@ std::vector<Tensor> norm_residual(const Tensor &x, const OptionalTensor &y, cons
     TORCH_CHECK(!y || y->sizes() == x.sizes(), "y must have x's shape, got ", y ? y->sizes() : x.sizes(), " and ", x.sizes());
     TORCH_CHECK(y || output != NORM_NONE, "without a block there is nothing to do but the norm");
     const auto at = [](const OptionalTensor &t) { return t ? &*t : nullptr; };
+    no_tangent({&x, at(y), at(gate), at(w_post), at(w_pre)});
     if (output != NORM_8BIT && wants_gradient({&x, at(y), at(gate), at(w_post), at(w_pre)}))
         return NormFunction::apply(x, y, gate, w_post, w_pre, alpha, eps, (int64_t)output);
     TORCH_CHECK(!wants_gradient({&x, at(y), at(gate), at(w_post), at(w_pre)}), "the packed output has no gradient: take the plain one and linear8 for training");

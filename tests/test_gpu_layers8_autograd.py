@@ -57,3 +57,15 @@ def test_norm_outputs_changed_in_place(shape):
     r += 1.0
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(h, a, dh)
+
+
+def test_tangent_of_a_gradient_is_refused():
+    x, w = _leaves(_rand((6, 200), 10), _rand((30, 200), 11))
+    y = tab_nn.linear8(x, w)
+    h, = tab_nn.norm_residual(x)
+    with forward_ad.dual_level():
+        for out in (y, h):
+            dy = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="forward mode"):
+                torch.autograd.grad(out, x, dy, retain_graph=True)
+    torch.autograd.grad(y, x, torch.ones_like(y))

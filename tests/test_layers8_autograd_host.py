@@ -1,0 +1,30 @@
+"""What the differentiable 8-bit layers and norms refuse before anything touches a GPU: tangents of forward mode, for which they have no formula."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import tab_amd
+from tab_amd import nn as tab_nn
+
+
+def test_tangents_are_refused_and_not_dropped():
+    def dual(*shape):
+        return forward_ad.make_dual(torch.ones(shape), torch.ones(shape))
+
+    x, w = torch.zeros(4, 128), torch.zeros(8, 128)
+    q, s = torch.zeros(8, 128).to(torch.float8_e4m3fn), torch.zeros(1, 1, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    with forward_ad.dual_level():
+        for a, b in ((dual(4, 128), w), (x, dual(8, 128)), (dual(4, 128).requires_grad_(), w)):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                tab_nn.linear8(a, b)
+        with pytest.raises(RuntimeError, match="forward mode"):
+            tab_nn.Linear8(q, s, 128, 8)(dual(4, 128))
+        v = torch.zeros(128)
+        for args in ((dual(4, 128), x), (x, dual(4, 128)), (x, x, dual(1, 128)), (x, x, None, dual(128)), (x, x, None, v, dual(128)), (dual(4, 128),)):
+            for output in (tab_amd.NORM_PLAIN, tab_amd.NORM_8BIT):
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    tab_nn.norm_residual(*args, output=output)
+        with pytest.raises(RuntimeError, match="CUDA tensor"):  # a level alone changes nothing
+            tab_nn.linear8(x, w)
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="CUDA tensor"):
+            tab_nn.linear8(dual(4, 128), w)
