@@ -163,6 +163,19 @@ class Linear8(nn.Module):
         return f"{self.in_features}, {self.out_features}"
 
 
+class _NoGradient(torch.autograd.Function):
+    """y, made from h by a layer without a backward pass: a gradient on its way to h ends in an error."""
+
+    @staticmethod
+    def forward(ctx, y, h):
+        return y
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("TABConv2d, TABLinear and TABPackedChain have no gradient: give a block that has one, detach what comes before it, "
+                           "or run under torch.no_grad()")
+
+
 class ResidualStack(nn.Module):
     """A residual stream through a list of blocks, each between two norms: with x_0 = x and the first norm of x_0 as the first block's input h_0,
 
@@ -171,7 +184,7 @@ class ResidualStack(nn.Module):
     Every block but the last is followed by one NormResidual launch (norm, gate, residual, next norm); the output is the last norm, so that
     a head can follow.  Blocks map (rows, D) to (rows, D): TABLinear layers, Linear8, or functions of linear8 in training.  With a Linear8 as the
     next block and no gradient wanted, the norm packs its output for it.  `gates` of a call: one (G, D) tensor or None a block, in place
-    of the learned gate per channel."""
+    of the learned gate per channel.  TABLinear layers have no backward pass: a gradient that would have to go through one is an error."""
 
     def __init__(self, blocks, D, alpha=1.0, eps=1e-6, gate_init=1.0, head=None):
         super().__init__()
@@ -197,6 +210,9 @@ class ResidualStack(nn.Module):
         h = norm_residual(x, w_pre=self.w_pre[0], eps=self.eps, output=self._output(0))
         for i, block in enumerate(self.blocks):
             y = block(h if len(h) > 1 else h[0])
+            if h[0].requires_grad and not y.requires_grad and torch.is_grad_enabled() and any(
+                    isinstance(m, (TABConv2d, TABLinear, TABPackedChain)) for m in block.modules()):
+                y = _NoGradient.apply(y, h[0])
             gate = self.gate[i] if gates is None or gates[i] is None else gates[i]
             x, *h = norm_residual(x, y.to(x.dtype), gate, self.w_post[i], self.w_pre[i + 1], self.alpha, self.eps, self._output(i + 1))
         out = h[0] if self.head is None else self.head(h if len(h) > 1 else h[0])

@@ -69,3 +69,36 @@ def test_tangent_of_a_gradient_is_refused():
             with pytest.raises(RuntimeError, match="forward mode"):
                 torch.autograd.grad(out, x, dy, retain_graph=True)
     torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("nested", [False, True])
+def test_stack_does_not_cut_a_gradient_in_silence(nested):
+    """A ternary layer has no backward pass: the stack's outputs are as without gradients, and a gradient that would have to pass it is an error."""
+    D, x = 64, _rand((10, 64), 20).cuda()
+    layer = tab_nn.TABLinear.from_float(_rand((D, D), 21), tab_amd.TNN)
+    stack = tab_nn.ResidualStack([torch.nn.Sequential(layer) if nested else layer], D).cuda()
+    with torch.no_grad():
+        want = stack(x)
+    out = stack(x)
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        out.sum().backward()
+    stack.w_pre[0].requires_grad_(False)  # nothing before the block wants one
+    out = stack(x)
+    assert torch.equal(out, want)
+    out.sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in (stack.gate[0], stack.w_post[0], stack.w_pre[1]))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        stack(x.clone().requires_grad_()).sum().backward()
+
+
+def test_stack_leaves_a_gradient_that_a_block_stops_on_purpose():
+    D, x = 64, _rand((10, 64), 22).cuda()
+
+    class Stop(torch.nn.Module):
+        def forward(self, h):
+            return h.detach() * 2
+
+    stack = tab_nn.ResidualStack([Stop()], D).cuda()
+    stack(x).sum().backward()
+    assert torch.isfinite(stack.gate[0].grad).all()
