@@ -244,8 +244,8 @@ std::vector<OptionalTensor> norm_backward(const OptionalTensor &dR, const Option
     out[0] = device_empty({M, D}, R.scalar_type(), R);
     if (Y) out[1] = device_empty({M, D}, R.scalar_type(), R);
     if (gate) out[2] = device_empty(gate->sizes(), gate->scalar_type(), R);
-    if (w_post) out[3] = device_empty({D}, torch::kFloat32, R);
-    if (w_pre) out[4] = device_empty({D}, torch::kFloat32, R);
+    if (w_post) out[3] = device_empty(w_post->sizes(), torch::kFloat32, R);
+    if (w_pre) out[4] = device_empty(w_pre->sizes(), torch::kFloat32, R);
     auto at = [](const OptionalTensor &t) -> void * { return t ? t->data_ptr() : nullptr; };
     const size_t bytes = tab_norm_residual_backward_workspace_bytes(M, D, g.rows);
     with_workspace(bytes, R, [&](void *ws, hipStream_t stream) {

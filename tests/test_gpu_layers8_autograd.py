@@ -71,6 +71,21 @@ def test_tangent_of_a_gradient_is_refused():
     torch.autograd.grad(y, x, torch.ones_like(y))
 
 
+def test_weights_of_one_row():
+    M, D = 5, 300
+    x, y, gate, w_post, w_pre = _rand((M, D), 12), _rand((M, D), 13), _rand((1, D), 14), _rand((D,), 15), _rand((D,), 16)
+    dr, dh = _rand((M, D), 17).cuda(), _rand((M, D), 18).cuda()
+    a, c = _leaves(x, y, gate, w_post, w_pre), _leaves(x, y, gate, w_post[None], w_pre[None, None])
+    want = torch.autograd.grad(tab_nn.norm_residual(*a), a, (dr, dh))
+    got = torch.autograd.grad(tab_nn.norm_residual(*c), c, (dr, dh))
+    for g, e, leaf in zip(got, want, c):
+        assert g.shape == leaf.shape and torch.equal(g.view(e.shape), e)
+    w = _rand((1, D), 19).cuda().requires_grad_()
+    h, = tab_nn.norm_residual(x.cuda(), w_pre=w)
+    h.backward(dh)
+    assert w.grad.shape == (1, D)
+
+
 @pytest.mark.parametrize("nested", [False, True])
 def test_stack_does_not_cut_a_gradient_in_silence(nested):
     """A ternary layer has no backward pass: the stack's outputs are as without gradients, and a gradient that would have to pass it is an error."""
