@@ -179,8 +179,9 @@ __global__ __launch_bounds__(RowsOfGroup<LANES>::THREADS) void norm_residual(con
 }
 
 // ---- gradients -------------------------------------------------------------------------------------------------------
-//   a = dH w_pre, p = rms(R):  t = dR + p a - R p^3 mean(R a),  dX = alpha t,  dw_pre = sum over rows of dH R p
-//   q = rms(Y), b = t gate w_post:  dY = q b - Y q^3 mean(Y b)
+//   a = dH w_pre, p = rms(R):  t = dR + p (a - R p^2 mean(R a)),  dX = alpha t,  dw_pre = sum over rows of dH R p
+//   q = rms(Y), b = t gate w_post:  dY = q (b - Y q^2 mean(Y b))
+// (p^3 and q^3 are outside fp32 for rows beyond 1e13 or, with a small eps, below 1e-13; p p mean(R a), from the right, is as large as a / R)
 //   s = sum over a gate's rows of t Y q:  dgate = s w_post,  dw_post = sum over gates of gate s
 // p and q are made anew from R and Y, which are here anyway, so the forward pass keeps nothing.  Sums over rows: a group of lanes adds up
 // its own rows in registers and leaves them in the workspace, a second launch adds the groups up in a fixed order.
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(RowsOfGroup<LANES>::THREADS) __attribute__((amdgpu_
                 if (BLOCK) sum[2] += element(y[c], i) * element(y[c], i);
             }
         sum_of_row<LANES>(sum, part[BLOCK ? 0 : m & 1]);
-        const float p1 = rsqrtf(sum[0] * over_d + p.eps), p3 = p1 * p1 * p1 * (sum[1] * over_d), q = rsqrtf(sum[2] * over_d + p.eps);
+        const float p1 = rsqrtf(sum[0] * over_d + p.eps), mean_a = p1 * (p1 * (sum[1] * over_d)), q = rsqrtf(sum[2] * over_d + p.eps);
         float t[RUNS][8], again[1] = {0.f};
 #pragma unroll
         for (int c = 0; c < RUNS; c++) {
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(RowsOfGroup<LANES>::THREADS) __attribute__((amdgpu_
                 const float rv = element(r[c], i), d = element(dh[c], i);
                 t[c][i] = element(dr[c], i);
                 if (p.dh) {
-                    t[c][i] += p1 * (d * w_pre[c][i]) - rv * p3;
+                    t[c][i] += p1 * (d * w_pre[c][i] - rv * mean_a);
                     dw_pre[c][i] += d * rv * p1;
                 }
                 dx[i] = p.alpha * t[c][i];
@@ -322,12 +323,12 @@ __global__ __launch_bounds__(RowsOfGroup<LANES>::THREADS) __attribute__((amdgpu_
         }
         if constexpr (BLOCK) {
             sum_of_row<LANES>(again, part[1]);
-            const float q3 = q * q * q * (again[0] * over_d);
+            const float mean_b = q * (q * (again[0] * over_d));
 #pragma unroll
             for (int c = 0; c < RUNS; c++) {
                 float dy[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) dy[i] = q * t[c][i] - element(y[c], i) * q3;
+                for (int i = 0; i < 8; i++) dy[i] = q * (t[c][i] - element(y[c], i) * mean_b);
                 store8(static_cast<T *>(p.dy) + m * p.D + at[c], left[c], dy);
             }
         }

@@ -117,3 +117,35 @@ def test_stack_leaves_a_gradient_that_a_block_stops_on_purpose():
     stack = tab_nn.ResidualStack([Stop()], D).cuda()
     stack(x).sum().backward()
     assert torch.isfinite(stack.gate[0].grad).all()
+
+
+def _norm_gradients(dr, dh, r, y, w_post, w_pre, eps):
+    """dX, dY by the formulas in 64 bits, no gate, alpha 1, and the magnitudes they are made from."""
+    r, y, a = r.double(), y.double(), dh.double() * w_pre.double()
+    p, q = (1 / torch.sqrt((v * v).mean(dim=1, keepdim=True) + eps) for v in (r, y))
+    t = p * (a - r * p * (r * p * a).mean(dim=1, keepdim=True))
+    mag = p * (a.abs() + (r * p).abs() * (r * p * a).abs().mean(dim=1, keepdim=True))
+    if dr is not None:
+        t, mag = t + dr.double(), mag + dr.double().abs()
+    b, mag_b = t * w_post.double(), mag * w_post.double()
+    dy = q * (b - y * q * (y * q * b).mean(dim=1, keepdim=True))
+    return t, mag, dy, 2 * q * (mag_b + (y * q).abs() * ((y * q).abs() * mag_b).mean(dim=1, keepdim=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size,eps", [(1e13, 1e-6), (1e17, 1e-6), (1e-14, 0.0), (1e-16, 0.0)])
+@pytest.mark.parametrize("D", [200, 3000])
+def test_gradients_of_large_and_small_streams(D, size, eps, dtype):
+    """rms^3 of these rows is beyond fp32, their gradients are not.  Bound: that of the ordinary sizes, 2^-18 of the magnitudes and a rounding."""
+    M = 5
+    r, y = _rand((M, D), 36, size).to(dtype), _rand((M, D), 37, size).to(dtype)
+    dr, dh = _rand((M, D), 38, 0.1 / size).to(dtype), _rand((M, D), 39, 0.1).to(dtype)
+    w_post, w_pre = _rand((D,), 40).abs() + 0.5, _rand((D,), 41).abs() + 0.5
+    for with_dr in (True, False):
+        d = dr if with_dr else None
+        dx, dy, _, _, _ = tab_amd.NormResidualBackward(None if d is None else d.cuda(), dh.cuda(), r.cuda(), y.cuda(), None, w_post.cuda(), w_pre.cuda(), 1.0, eps, M, D)
+        want_x, mag_x, want_y, mag_y = _norm_gradients(d, dh, r, y, w_post, w_pre, eps)
+        for got, want, mag in ((dx, want_x, mag_x), (dy, want_y, mag_y)):
+            got = got.cpu().double()
+            off, bound = (got - want).abs(), 2.0 ** -18 * mag + ref.UNIT[dtype] * (1 + 2.0 ** -8) * want.abs() + ref.TINY[dtype]
+            assert (off <= bound).all(), float((off / bound).max())
