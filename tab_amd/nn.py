@@ -153,6 +153,17 @@ class Linear8(nn.Module):
         QW, SW = Quantize8(weight.detach().cuda().contiguous(), N, K, 128)
         return cls(QW, SW, K, N, out_dtype)
 
+    def _apply(self, fn, recurse=True):
+        """What moves or converts the module moves the packed weight, whose types are its format: fn sees their bytes, and a conversion to another type leaves
+        them as they are."""
+        def bytes_alone(t):
+            if t.dtype not in (torch.float8_e4m3fn, torch.float8_e8m0fnu):
+                return fn(t)
+            moved = fn(t.view(torch.uint8))
+            return moved.view(t.dtype) if moved.dtype == torch.uint8 else t.to(moved.device)
+
+        return super()._apply(bytes_alone, recurse)
+
     def forward(self, x):
         if isinstance(x, (tuple, list)):
             QX, SX = x

@@ -119,6 +119,19 @@ def test_stack_leaves_a_gradient_that_a_block_stops_on_purpose():
     assert torch.isfinite(stack.gate[0].grad).all()
 
 
+@pytest.mark.parametrize("convert", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.float(), lambda m: m.cpu().cuda(),
+                                     lambda m: m.to("cuda", torch.bfloat16), lambda m: m.type(torch.float16), copy.deepcopy],
+                         ids=["half", "bfloat16", "double", "float", "cpu_and_back", "to", "type", "copy"])
+def test_packed_weight_survives_conversions(convert):
+    layer = tab_nn.Linear8.from_float(_rand((30, 300), 34, 1e-6))  # scales that 16 bits do not hold
+    x = _rand((5, 300), 35).cuda()
+    want, qw, sw = layer(x), layer.QW.view(torch.uint8).clone(), layer.SW.view(torch.uint8).clone()
+    layer = convert(layer)
+    assert layer.QW.dtype == torch.float8_e4m3fn and layer.SW.dtype == torch.float8_e8m0fnu
+    assert torch.equal(layer.QW.view(torch.uint8), qw) and torch.equal(layer.SW.view(torch.uint8), sw)
+    assert torch.equal(layer(x), want)
+
+
 def _norm_gradients(dr, dh, r, y, w_post, w_pre, eps):
     """dX, dY by the formulas in 64 bits, no gate, alpha 1, and the magnitudes they are made from."""
     r, y, a = r.double(), y.double(), dh.double() * w_pre.double()
