@@ -415,15 +415,22 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     }
 };
 
+// Weights of a module that was converted to 16 bits, as the kernels take them; the conversion is differentiable.
+OptionalTensor as_fp32(const OptionalTensor &w)
+{
+    return w && (w->scalar_type() == torch::kBFloat16 || w->scalar_type() == torch::kFloat16) ? OptionalTensor(w->to(torch::kFloat32)) : w;
+}
+
 // nn.norm_residual: x (..., D) and y of its shape
-std::vector<Tensor> norm_residual(const Tensor &x, const OptionalTensor &y, const OptionalTensor &gate, const OptionalTensor &w_post, const OptionalTensor &w_pre,
+std::vector<Tensor> norm_residual(const Tensor &x, const OptionalTensor &y, const OptionalTensor &gate, const OptionalTensor &w_post_any, const OptionalTensor &w_pre_any,
                                   double alpha, double eps, int output)
 {
     TORCH_CHECK(x.dim() >= 1 && x.numel() > 0, "x must not be empty, got ", x.sizes());
     TORCH_CHECK(!y || y->sizes() == x.sizes(), "y must have x's shape, got ", y ? y->sizes() : x.sizes(), " and ", x.sizes());
     TORCH_CHECK(y || output != NORM_NONE, "without a block there is nothing to do but the norm");
     const auto at = [](const OptionalTensor &t) { return t ? &*t : nullptr; };
-    no_tangent({&x, at(y), at(gate), at(w_post), at(w_pre)});
+    no_tangent({&x, at(y), at(gate), at(w_post_any), at(w_pre_any)});
+    const OptionalTensor w_post = as_fp32(w_post_any), w_pre = as_fp32(w_pre_any);
     if (output != NORM_8BIT && wants_gradient({&x, at(y), at(gate), at(w_post), at(w_pre)}))
         return NormFunction::apply(x, y, gate, w_post, w_pre, alpha, eps, (int64_t)output);
     TORCH_CHECK(!wants_gradient({&x, at(y), at(gate), at(w_post), at(w_pre)}), "the packed output has no gradient: take the plain one and linear8 for training");

@@ -131,7 +131,8 @@ def linear8(x, w, grad_format=E4M3):
 
 def norm_residual(x, y=None, gate=None, w_post=None, w_pre=None, alpha=1.0, eps=1e-6, output=NORM_PLAIN):
     """tab_amd.NormResidual (with a block's output y) or tab_amd.Norm (without) on tensors (..., D), differentiable in every tensor:
-    [R, H], [R] with output=NORM_NONE, [H] without y.  output=NORM_8BIT gives H packed, for inference."""
+    [R, H], [R] with output=NORM_NONE, [H] without y.  output=NORM_8BIT gives H packed, for inference.  Weights of 16 bits, as a converted
+    module has, are taken as fp32."""
     return _C.norm_residual(x, y, gate, w_post, w_pre, float(alpha), float(eps), int(output))
 
 
@@ -192,10 +193,11 @@ class ResidualStack(nn.Module):
 
         y_i = block_i(h_i),   x_{i+1} = alpha x_i + gate_i * norm(y_i; w_post_i),   h_{i+1} = norm(x_{i+1}; w_pre_{i+1})
 
-    Every block but the last is followed by one NormResidual launch (norm, gate, residual, next norm); the output is the last norm, so that
-    a head can follow.  Blocks map (rows, D) to (rows, D): TABLinear layers, Linear8, or functions of linear8 in training.  With a Linear8 as the
-    next block and no gradient wanted, the norm packs its output for it.  `gates` of a call: one (G, D) tensor or None a block, in place
-    of the learned gate per channel.  TABLinear layers have no backward pass: a gradient that would have to go through one is an error."""
+    Every block is followed by one NormResidual launch (norm, gate, residual, next norm); the output is the last norm, so that a head can
+    follow.  Blocks map (rows, D) to (rows, D): TABLinear layers, Linear8, or functions of linear8 in training; TABLinear's input is fp32 also
+    in a stream of 16 bits.  With a Linear8 as the next block and no gradient wanted, the norm packs its output for it.  `gates` of a call: one
+    (G, D) tensor or None a block, in place of the learned gate per channel.  TABLinear layers have no backward pass: a gradient that would
+    have to go through one is an error."""
 
     def __init__(self, blocks, D, alpha=1.0, eps=1e-6, gate_init=1.0, head=None):
         super().__init__()
@@ -214,17 +216,21 @@ class ResidualStack(nn.Module):
         follower = self.blocks[i] if i < len(self.blocks) else self.head
         return NORM_8BIT if isinstance(follower, Linear8) and not torch.is_grad_enabled() else NORM_PLAIN
 
+    @staticmethod
+    def _input(layer, h):
+        return h if len(h) > 1 else h[0].float() if isinstance(layer, TABLinear) else h[0]
+
     def forward(self, x, gates=None):
         if gates is not None and len(gates) != len(self.blocks):
             raise ValueError(f"{len(gates)} gates for {len(self.blocks)} blocks")
         shape, x = x.shape, x.reshape(-1, x.shape[-1])
         h = norm_residual(x, w_pre=self.w_pre[0], eps=self.eps, output=self._output(0))
         for i, block in enumerate(self.blocks):
-            y = block(h if len(h) > 1 else h[0])
+            y = block(self._input(block, h))
             if h[0].requires_grad and not y.requires_grad and torch.is_grad_enabled() and any(
                     isinstance(m, (TABConv2d, TABLinear, TABPackedChain)) for m in block.modules()):
                 y = _NoGradient.apply(y, h[0])
             gate = self.gate[i] if gates is None or gates[i] is None else gates[i]
             x, *h = norm_residual(x, y.to(x.dtype), gate, self.w_post[i], self.w_pre[i + 1], self.alpha, self.eps, self._output(i + 1))
-        out = h[0] if self.head is None else self.head(h if len(h) > 1 else h[0])
+        out = h[0] if self.head is None else self.head(self._input(self.head, h))
         return out.reshape(*shape[:-1], out.shape[-1])

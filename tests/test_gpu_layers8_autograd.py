@@ -119,6 +119,40 @@ def test_stack_leaves_a_gradient_that_a_block_stops_on_purpose():
     assert torch.isfinite(stack.gate[0].grad).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_norm_weights_of_16_bits(dtype):
+    """They are the fp32 weights of the same values; their gradients are rounded to their type."""
+    M, D = 7, 300
+    x, y, gate = (t.to(dtype) for t in (_rand((M, D), 23), _rand((M, D), 24), _rand((1, D), 25)))
+    w_post, w_pre = (_rand((D,), s).to(dtype) for s in (26, 27))
+    dr, dh = _rand((M, D), 28).to(dtype).cuda(), _rand((M, D), 29).to(dtype).cuda()
+    a, c = _leaves(x, y, gate, w_post, w_pre), _leaves(x, y, gate, w_post.float(), w_pre.float())
+    got, want = tab_nn.norm_residual(*a), tab_nn.norm_residual(*c)
+    for g, e in zip(got, want):
+        assert torch.equal(g, e)
+    for g, e, leaf in zip(torch.autograd.grad(got, a, (dr, dh)), torch.autograd.grad(want, c, (dr, dh)), a):
+        assert g.dtype == leaf.dtype and torch.equal(g, e.to(dtype))
+    with torch.no_grad():
+        for output in (tab_amd.NORM_PLAIN, tab_amd.NORM_8BIT):
+            for g, e in zip(tab_nn.norm_residual(*a, output=output), tab_nn.norm_residual(*c, output=output)):
+                assert torch.equal(g.view(torch.uint8), e.view(torch.uint8))
+
+
+@pytest.mark.parametrize("ternary_head", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_stack_converted_to_16_bits(dtype, ternary_head):
+    D, w = 128, _rand((10, 128), 32, 128 ** -0.5)
+    head = tab_nn.TABLinear.from_float(w, tab_amd.TNN) if ternary_head else tab_nn.Linear8.from_float(w)
+    blocks = [tab_nn.Linear8.from_float(_rand((D, D), 30, D ** -0.5)), tab_nn.TABLinear.from_float(_rand((D, D), 31), tab_amd.TBN)]
+    stack = tab_nn.ResidualStack(blocks, D, alpha=0.5, head=head).cuda()
+    x = _rand((9, D), 33).to(dtype).cuda()
+    half = copy.deepcopy(stack).to(dtype)
+    with torch.no_grad():  # its parameters are ones, the same in every type
+        out = half(x)
+        assert torch.equal(out, stack(x))
+    assert torch.isfinite(out).all() and float(out.abs().max()) > 0
+
+
 @pytest.mark.parametrize("convert", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.float(), lambda m: m.cpu().cuda(),
                                      lambda m: m.to("cuda", torch.bfloat16), lambda m: m.type(torch.float16), copy.deepcopy],
                          ids=["half", "bfloat16", "double", "float", "cpu_and_back", "to", "type", "copy"])
