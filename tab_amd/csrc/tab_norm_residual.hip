@@ -185,8 +185,8 @@ __global__ __launch_bounds__(RowsOfGroup<LANES>::THREADS) void norm_residual(con
 //   s = sum over a gate's rows of t Y q:  dgate = s w_post,  dw_post = sum over gates of gate s
 // p and q are made anew from R and Y, which are here anyway, so the forward pass keeps nothing.  Sums over rows: a group of lanes adds up
 // its own rows in registers and leaves them in the workspace, a second launch adds the groups up in a fixed order.
-// bf16 16384 x 4096 with 16 gates: 162-167 us, 805 MB at 4.8-5.0 TB/s, and 11-13 for the join; fp32 777 x 1531 with a gate for each row: 16 and 3-4
-// (two rows to a group; with four 19 and 3-4).  The next row is loaded before this one's sums are taken, as a row alone is all latency.
+// bf16 16384 x 4096 with 16 gates: 162-167 us, 805 MB at 4.8-5.0 TB/s, and 11-13 for the join; fp32 777 x 1531 with a gate for each row: 17.6-17.9 in
+// all (two rows to a group; with three 19.1-19.6).  The next row is loaded before this one's sums are taken, as a row alone is all latency.
 
 struct NormGradParams {
     const void *dr, *dh, *r, *y, *gate;
@@ -451,8 +451,8 @@ struct GradPlan {
 
 GradPlan grad_plan(bool gate, int M, int D, int rows_per_gate)
 {
-    // as many groups as the chip holds at once, but two rows in each before there are more than CUs: every group writes 2 D sums
-    const long held = groups_at_once(shape_of(D)), few = M / 2 > 256 ? M / 2 : 256, most = held < few ? held : few, rows = (M + most - 1) / most;
+    // as many groups as the chip holds at once, but two rows in each (one where M is odd) before there are more than CUs: every group writes 2 D sums
+    const long held = groups_at_once(shape_of(D)), few = M > 512 ? ((long)M + 1) / 2 : 256, most = held < few ? held : few, rows = (M + most - 1) / most;
     const bool whole = gate && rows_per_gate <= rows;
     // (at least one row a group and, for pieces, as even as they come)
     const long pieces = whole ? 1 : (rows_per_gate + rows - 1) / rows;
