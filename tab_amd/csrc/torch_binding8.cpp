@@ -428,6 +428,12 @@ std::vector<Tensor> norm_residual(const Tensor &x, const OptionalTensor &y, cons
     TORCH_CHECK(x.dim() >= 1 && x.numel() > 0, "x must not be empty, got ", x.sizes());
     TORCH_CHECK(!y || y->sizes() == x.sizes(), "y must have x's shape, got ", y ? y->sizes() : x.sizes(), " and ", x.sizes());
     TORCH_CHECK(y || output != NORM_NONE, "without a block there is nothing to do but the norm");
+    if (gate && gate->dim() == x.dim() && x.dim() > 2) {
+        // (torch would broadcast a gate of (1, S, D) over the first dimension; a row of the kernels' gate holds for consecutive rows of x)
+        int64_t d = 0;
+        while (d < x.dim() - 1 && gate->size(d) == x.size(d)) d++;
+        for (; d < x.dim() - 1; d++) TORCH_CHECK(gate->size(d) == 1, "a row of the gate holds for consecutive rows of x: sizes other than 1 must be x's first ones, got ", gate->sizes(), " and ", x.sizes());
+    }
     const auto at = [](const OptionalTensor &t) { return t ? &*t : nullptr; };
     no_tangent({&x, at(y), at(gate), at(w_post_any), at(w_pre_any)});
     const OptionalTensor w_post = as_fp32(w_post_any), w_pre = as_fp32(w_pre_any);

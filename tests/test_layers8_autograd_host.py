@@ -28,3 +28,14 @@ def test_tangents_are_refused_and_not_dropped():
             tab_nn.linear8(x, w)
         with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="CUDA tensor"):
             tab_nn.linear8(dual(4, 128), w)
+
+
+def test_gates_that_would_have_to_be_repeated_are_refused():
+    """A row of the gate holds for consecutive rows: a gate for each position, repeated over the sequences, would be taken for something else."""
+    x = torch.zeros(2, 3, 4, 8)
+    for sizes in ((1, 3, 4, 8), (1, 3, 1, 8), (2, 1, 4, 8), (1, 1, 4, 8), (3, 1, 1, 8)):
+        with pytest.raises(RuntimeError, match="consecutive rows"):
+            tab_nn.norm_residual(x, x, torch.zeros(sizes))
+    for sizes in ((1, 1, 1, 8), (2, 1, 1, 8), (2, 3, 1, 8), (2, 3, 4, 8), (6, 8), (1, 8), (8,)):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):  # as far as that
+            tab_nn.norm_residual(x, x, torch.zeros(sizes))
