@@ -75,11 +75,11 @@ __device__ __forceinline__ f32x4 mfma16_exact(const Exact32 &w, const Exact32 &x
 // instruction's write.)
 __device__ __forceinline__ void to_lds16(i32x4 buffer, uint32_t to, uint32_t lane_offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer) : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds1(i32x4 buffer, uint32_t to, uint32_t lane_offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_ubyte %1, %2, 0 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_ubyte %1, %2, 0 offen lds" ::"s"(to), "v"(lane_offset), "s"(buffer) : "memory", "m0");
 }
 __device__ __forceinline__ uint32_t lds_address(const uint8_t *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)p; }
 
@@ -113,16 +113,10 @@ template <int N> __device__ __forceinline__ ScaleWords<N> scale_words(const uint
     return s;
 }
 
-template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v, int left)
+template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v)
 {
-    if (left >= 4) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
-        *reinterpret_cast<Four *>(y) = Four{{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}};
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i < left) y[i] = (T)v[i];
-    }
+    struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
+    *reinterpret_cast<Four *>(y) = Four{{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}};
 }
 
 // A workgroup of WM x WN waves makes a BM x BN tile of Y, for more rows than linear8_rows takes; bound by the matrix instructions and, the smaller the tile,
@@ -422,7 +416,7 @@ template <int OUT> __global__ __launch_bounds__(256) void linear8_join(const flo
     if (count % 4 == 0) {
         f32x4 sum = *reinterpret_cast<const f32x4 *>(parts + i);
         for (int k = 1; k < n; k++) sum += *reinterpret_cast<const f32x4 *>(parts + k * count + i);
-        store4(static_cast<T *>(y) + i, sum, 4);
+        store4(static_cast<T *>(y) + i, sum);
     } else {
         for (long j = i; j < min(i + 4, count); j++) {
             float sum = parts[j];
