@@ -59,6 +59,35 @@ def test_forward(M, D, rows_per_gate, dtype):
 
 
 @two_types
+@pytest.mark.parametrize("M,D", [(1, 1), (3, 100), (5, 511), (2, 1000), (3, 1025), (3, 4096), (2, 8000), (2, 16384)] + ROWS)
+def test_first_norm(M, D, dtype):
+    x, _, _, _, w = _cuda(*_inputs(M, D, 0, dtype, 5 * D + M))
+    want = ref.norm(x, None, None, None, w, 1.0, ref.EPS)[1]
+    H, = tab_amd.Norm(x, w, ref.EPS, M, D)
+    _within(H, want, want.abs(), "H")
+    QH, SH = tab_amd.Norm(x, w, ref.EPS, M, D, tab_amd.NORM_8BIT)
+    _packed_within(QH, SH, want, want.abs(), M, D)
+    if dtype == torch.float32:  # the plain output is what was packed
+        Q, S = tab_amd.Quantize8(H, M, D)
+        assert torch.equal(Q.view(torch.uint8), QH.view(torch.uint8)) and torch.equal(S.view(torch.uint8), SH.view(torch.uint8))
+
+
+def test_stack_whose_first_block_takes_the_packed_norm():
+    from tab_amd import nn as tab_nn
+    D, M = 200, 40
+    x, _, _, _, _ = _cuda(*_inputs(M, D, 0, torch.float32, 60))
+    w, head = (torch.randn((n, D), generator=torch.Generator("cpu").manual_seed(s)) * D ** -0.5 for n, s in ((D, 61), (30, 62)))
+    stack = tab_nn.ResidualStack([tab_nn.Linear8.from_float(w)], D, head=tab_nn.Linear8.from_float(head)).cuda()
+    with torch.no_grad():
+        got = stack(x)
+        h, = tab_amd.Norm(x, stack.w_pre[0], ref.EPS, M, D)
+        y = tab_amd.Linear8Packed(*tab_amd.Quantize8(h, M, D), stack.blocks[0].QW, stack.blocks[0].SW, M, D, D)
+        _, h = tab_amd.NormResidual(x, y, stack.gate[0], stack.w_post[0], stack.w_pre[1], 1.0, ref.EPS, M, D)
+        want = tab_amd.Linear8Packed(*tab_amd.Quantize8(h, M, D), stack.head.QW, stack.head.SW, M, 30, D)
+    assert torch.equal(got, want)
+
+
+@two_types
 @per_gate
 @rows
 def test_gradients(M, D, rows_per_gate, dtype):
