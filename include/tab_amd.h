@@ -277,7 +277,7 @@ int tab_set_conv_kernel(int kernel, int tile);
  * A packed 8-bit operand of an R x K matrix is
  *   Q  8-bit numbers [R][128 * ceil(K/128)], zeros past K, 16-byte aligned
  *   S  E8M0 bytes [ceil(K/128)][R] (blocks of 1 x 128) or [ceil(K/128)][ceil(R/128)] (blocks of 128 x 128)
- * and stands for Q[r][k] * 2^(S - 127).  Real tensors are fp32, bf16 or fp16, rounded to nearest even where they are written; all sums are
+ * and stands for Q[r][k] * 2^(S - 127), NaN where S is 255.  Real tensors are fp32, bf16 or fp16, rounded to nearest even where they are written; all sums are
  * fp32.  Tensors are aligned to their elements and their rows are contiguous; a row stride (ld...) counts elements.
  */
 enum { TAB_F32 = 0, TAB_BF16 = 1, TAB_F16 = 2 };
