@@ -421,6 +421,17 @@ OptionalTensor as_fp32(const OptionalTensor &w)
     return w && (w->scalar_type() == torch::kBFloat16 || w->scalar_type() == torch::kFloat16) ? OptionalTensor(w->to(torch::kFloat32)) : w;
 }
 
+// A row of the kernels' gate holds for consecutive rows of x.  Torch would broadcast a gate of (1, S, D) over the first dimension of x: refused.
+void check_gate(const Tensor &gate, c10::IntArrayRef x)
+{
+    const int64_t dims = (int64_t)x.size();
+    if (gate.dim() != dims || dims < 3) return;
+    int64_t d = 0;
+    while (d < dims - 1 && gate.size(d) == x[d]) d++;
+    for (; d < dims - 1; d++)
+        TORCH_CHECK(gate.size(d) == 1, "a row of the gate holds for consecutive rows of x: sizes other than 1 must be x's first ones, got ", gate.sizes(), " and ", x);
+}
+
 // nn.norm_residual: x (..., D) and y of its shape
 std::vector<Tensor> norm_residual(const Tensor &x, const OptionalTensor &y, const OptionalTensor &gate, const OptionalTensor &w_post_any, const OptionalTensor &w_pre_any,
                                   double alpha, double eps, int output)
@@ -428,12 +439,7 @@ std::vector<Tensor> norm_residual(const Tensor &x, const OptionalTensor &y, cons
     TORCH_CHECK(x.dim() >= 1 && x.numel() > 0, "x must not be empty, got ", x.sizes());
     TORCH_CHECK(!y || y->sizes() == x.sizes(), "y must have x's shape, got ", y ? y->sizes() : x.sizes(), " and ", x.sizes());
     TORCH_CHECK(y || output != NORM_NONE, "without a block there is nothing to do but the norm");
-    if (gate && gate->dim() == x.dim() && x.dim() > 2) {
-        // (torch would broadcast a gate of (1, S, D) over the first dimension; a row of the kernels' gate holds for consecutive rows of x)
-        int64_t d = 0;
-        while (d < x.dim() - 1 && gate->size(d) == x.size(d)) d++;
-        for (; d < x.dim() - 1; d++) TORCH_CHECK(gate->size(d) == 1, "a row of the gate holds for consecutive rows of x: sizes other than 1 must be x's first ones, got ", gate->sizes(), " and ", x.sizes());
-    }
+    if (gate) check_gate(*gate, x.sizes());
     const auto at = [](const OptionalTensor &t) { return t ? &*t : nullptr; };
     no_tangent({&x, at(y), at(gate), at(w_post_any), at(w_pre_any)});
     const OptionalTensor w_post = as_fp32(w_post_any), w_pre = as_fp32(w_pre_any);
@@ -471,5 +477,6 @@ void bind_layers8(pybind11::module_ &m)
     m.def("NormBackward", &TAB_NormBackward, "gradients of Norm");
     m.def("linear8", &linear8, "nn.linear8");
     m.def("linear8_packed_weight", &linear8_packed_weight, "nn.Linear8.forward");
+    m.def("check_gate", [](const Tensor &gate, const std::vector<int64_t> &x) { check_gate(gate, x); }, "whether a gate of x's dimensions holds for consecutive rows");
     m.def("norm_residual", &norm_residual, "nn.norm_residual");
 }

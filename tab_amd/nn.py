@@ -224,6 +224,9 @@ class ResidualStack(nn.Module):
     def forward(self, x, gates=None):
         if gates is not None and len(gates) != len(self.blocks):
             raise ValueError(f"{len(gates)} gates for {len(self.blocks)} blocks")
+        for gate in () if gates is None else gates:
+            if gate is not None:
+                _C.check_gate(gate, x.shape)
         shape, x = x.shape, x.reshape(-1, x.shape[-1])
         h = norm_residual(x, w_pre=self.w_pre[0], eps=self.eps, output=self._output(0))
         for i, block in enumerate(self.blocks):

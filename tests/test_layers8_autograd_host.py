@@ -39,3 +39,17 @@ def test_gates_that_would_have_to_be_repeated_are_refused():
     for sizes in ((1, 1, 1, 8), (2, 1, 1, 8), (2, 3, 1, 8), (2, 3, 4, 8), (6, 8), (1, 8), (8,)):
         with pytest.raises(RuntimeError, match="CUDA tensor"):  # as far as that
             tab_nn.norm_residual(x, x, torch.zeros(sizes))
+
+
+def test_a_stack_refuses_such_gates_too():
+    stack = tab_nn.ResidualStack([torch.nn.Identity()], 8)
+    x = torch.zeros(2, 4, 8)
+    with pytest.raises(RuntimeError, match="consecutive rows"):
+        stack(x, [torch.zeros(1, 4, 8)])
+    for sizes in ((2, 1, 8), (1, 1, 8), (2, 8), (8, 8)):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            stack(x, [torch.zeros(sizes)])
+    with pytest.raises(TypeError):
+        stack(x, [0.5])
+    with pytest.raises(RuntimeError, match="CUDA tensor"):  # one tensor for all blocks
+        stack(x, torch.zeros(1, 2, 8))
