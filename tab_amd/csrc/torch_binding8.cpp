@@ -415,10 +415,14 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     }
 };
 
-// Weights of a module that was converted to 16 bits, as the kernels take them; the conversion is differentiable.
-OptionalTensor as_fp32(const OptionalTensor &w)
+// Weights and gates as the kernels take them: contiguous (a gate is often a part of a wider modulation), weights of a module that was converted to 16 bits
+// as fp32, and gates of 16 bits that are not x's.  All of it is differentiable.
+OptionalTensor taken(const OptionalTensor &w, torch::ScalarType kept = torch::kFloat32)
 {
-    return w && (w->scalar_type() == torch::kBFloat16 || w->scalar_type() == torch::kFloat16) ? OptionalTensor(w->to(torch::kFloat32)) : w;
+    if (!w) return w;
+    const auto type = w->scalar_type();
+    const bool widen = type != kept && (type == torch::kBFloat16 || type == torch::kFloat16);
+    return (widen ? w->to(torch::kFloat32) : *w).contiguous();
 }
 
 // A row of the kernels' gate holds for consecutive rows of x.  Torch would broadcast a gate of (1, S, D) over the first dimension of x: refused.
@@ -433,16 +437,16 @@ void check_gate(const Tensor &gate, c10::IntArrayRef x)
 }
 
 // nn.norm_residual: x (..., D) and y of its shape
-std::vector<Tensor> norm_residual(const Tensor &x, const OptionalTensor &y, const OptionalTensor &gate, const OptionalTensor &w_post_any, const OptionalTensor &w_pre_any,
+std::vector<Tensor> norm_residual(const Tensor &x, const OptionalTensor &y, const OptionalTensor &any_gate, const OptionalTensor &any_post, const OptionalTensor &any_pre,
                                   double alpha, double eps, int output)
 {
     TORCH_CHECK(x.dim() >= 1 && x.numel() > 0, "x must not be empty, got ", x.sizes());
     TORCH_CHECK(!y || y->sizes() == x.sizes(), "y must have x's shape, got ", y ? y->sizes() : x.sizes(), " and ", x.sizes());
     TORCH_CHECK(y || output != NORM_NONE, "without a block there is nothing to do but the norm");
-    if (gate) check_gate(*gate, x.sizes());
+    if (any_gate) check_gate(*any_gate, x.sizes());
     const auto at = [](const OptionalTensor &t) { return t ? &*t : nullptr; };
-    no_tangent({&x, at(y), at(gate), at(w_post_any), at(w_pre_any)});
-    const OptionalTensor w_post = as_fp32(w_post_any), w_pre = as_fp32(w_pre_any);
+    no_tangent({&x, at(y), at(any_gate), at(any_post), at(any_pre)});
+    const OptionalTensor gate = taken(any_gate, x.scalar_type()), w_post = taken(any_post), w_pre = taken(any_pre);
     if (output != NORM_8BIT && wants_gradient({&x, at(y), at(gate), at(w_post), at(w_pre)}))
         return NormFunction::apply(x, y, gate, w_post, w_pre, alpha, eps, (int64_t)output);
     TORCH_CHECK(!wants_gradient({&x, at(y), at(gate), at(w_post), at(w_pre)}), "the packed output has no gradient: take the plain one and linear8 for training");

@@ -132,8 +132,8 @@ def linear8(x, w, grad_format=E4M3):
 def norm_residual(x, y=None, gate=None, w_post=None, w_pre=None, alpha=1.0, eps=1e-6, output=NORM_PLAIN):
     """tab_amd.NormResidual (with a block's output y) or tab_amd.Norm (without) on tensors (..., D), differentiable in every tensor:
     [R, H], [R] with output=NORM_NONE, [H] without y.  output=NORM_8BIT gives H packed, for inference.  A row of the gate
-    holds for consecutive rows of x, so (B, 1, D) or (B, D) is a gate for each sequence of x (B, S, D).  Weights of 16 bits, as a converted module
-    has, are taken as fp32."""
+    holds for consecutive rows of x, so (B, 1, D) or (B, D) is a gate for each sequence of x (B, S, D).  Gate and weights need not be contiguous;
+    those of 16 bits, as a converted module has, are taken as fp32 (a gate of x's type as it is)."""
     return _C.norm_residual(x, y, gate, w_post, w_pre, float(alpha), float(eps), int(output))
 
 

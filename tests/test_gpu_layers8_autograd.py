@@ -196,3 +196,36 @@ def test_gradients_of_large_and_small_streams(D, size, eps, dtype):
             got = got.cpu().double()
             off, bound = (got - want).abs(), 2.0 ** -18 * mag + ref.UNIT[dtype] * (1 + 2.0 ** -8) * want.abs() + ref.TINY[dtype]
             assert (off <= bound).all(), float((off / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gates_and_weights_that_are_parts_of_wider_tensors(dtype):
+    """A gate out of a modulation, one gate expanded over the sequences, columns of a matrix as weights: the values and the gradients of contiguous ones."""
+    B, S, D = 3, 4, 200
+    x, y, wide, columns = _rand((B, S, D), 50).to(dtype), _rand((B, S, D), 51).to(dtype), _rand((B, 1, 3 * D), 52).to(dtype), _rand((D, 2), 53)
+    dr, dh = _rand((B, S, D), 54).to(dtype).cuda(), _rand((B, S, D), 55).to(dtype).cuda()
+    a = _leaves(x, y, wide, columns)
+    part = a[2].chunk(3, dim=-1)[1]
+    assert not part.is_contiguous()
+    got = tab_nn.norm_residual(a[0], a[1], part, a[3][:, 0], a[3][:, 1], 0.9)
+    c = _leaves(x, y, wide[..., D:2 * D].contiguous(), columns[:, 0].contiguous(), columns[:, 1].contiguous())
+    want = tab_nn.norm_residual(*c, 0.9)
+    for g, e in zip(got, want):
+        assert torch.equal(g, e)
+    dx, dy, dwide, dcolumns = torch.autograd.grad(got, a, (dr, dh))
+    ex, ey, egate, epost, epre = torch.autograd.grad(want, c, (dr, dh))
+    assert torch.equal(dx, ex) and torch.equal(dy, ey) and torch.equal(dcolumns, torch.stack([epost, epre], dim=1))
+    assert torch.equal(dwide[..., D:2 * D], egate) and not dwide[..., :D].any() and not dwide[..., 2 * D:].any()
+    one = wide[:1, :, :D].cuda()
+    with torch.no_grad():
+        for g, e in zip(tab_nn.norm_residual(x.cuda(), y.cuda(), one.expand(B, 1, D)), tab_nn.norm_residual(x.cuda(), y.cuda(), one.contiguous())):
+            assert torch.equal(g, e)
+
+
+def test_gate_of_16_bits_in_a_stream_of_32():
+    x, y, gate = _rand((6, 300), 56), _rand((6, 300), 57), _rand((2, 300), 58).bfloat16()
+    a, c = _leaves(x, y, gate), _leaves(x, y, gate.float())
+    got, want = tab_nn.norm_residual(*a), tab_nn.norm_residual(*c)
+    dh = _rand((6, 300), 59).cuda()
+    for g, e, leaf in zip(torch.autograd.grad(got, a, (dh, dh)), torch.autograd.grad(want, c, (dh, dh)), a):
+        assert g.dtype == leaf.dtype and torch.equal(g, e.to(g.dtype))
