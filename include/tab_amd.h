@@ -277,8 +277,8 @@ int tab_set_conv_kernel(int kernel, int tile);
  * A packed 8-bit operand of an R x K matrix is
  *   Q  8-bit numbers [R][128 * ceil(K/128)], zeros past K, 16-byte aligned
  *   S  E8M0 bytes [ceil(K/128)][R] (blocks of 1 x 128) or [ceil(K/128)][ceil(R/128)] (blocks of 128 x 128)
- * and stands for Q[r][k] * 2^(S - 127), NaN where S is 255.  Real tensors are fp32, bf16 or fp16, rounded to nearest even where they are written; all sums are
- * fp32.  Tensors are aligned to their elements and their rows are contiguous; a row stride (ld...) counts elements.
+ * and stands for Q[r][k] * 2^(S - 127), NaN where S is 255.  Real tensors are fp32, bf16 or fp16, rounded to nearest even where they are written.
+ * Sums are fp32; inside the products towards 16-bit outputs some partial sums have fewer bits (see tab_linear8_packed).  Tensors are aligned to their elements and their rows are contiguous; a row stride (ld...) counts elements.
  */
 enum { TAB_F32 = 0, TAB_BF16 = 1, TAB_F16 = 2 };
 enum { TAB_E4M3 = 0, TAB_E5M2 = 1 }; /* largest numbers 448 and 57344 */
@@ -300,7 +300,8 @@ int tab_quantize8(const void *dev_X, int dtype, int M, int K, long ldx, int bloc
 /*
  * Y (M x N, rows contiguous) = X (M x K, packed) times the transpose of W (N x K, packed in E4M3 with blocks of w_block_rows x 128).  An fp32 Y
  * is the sum of exact products in fp32 (operands below 2^-126 may count as zeros, one that rounds to 2^128 as an infinity); towards a 16-bit Y the products of eight neighbours in K keep
- * 13 bits below the largest of them, some 1.5e-5 of Y's size.
+ * 13 bits below the largest of them, some 1.5e-5 of Y's size: about one output in a hundred is rounded to the other neighbour in bf16, its distance from
+ * the exact product as large as before.  Where that matters, an fp32 Y.
  *   workspace  tab_linear8_packed_workspace_bytes(out_dtype, M, N, K) bytes, 16-byte aligned; 0 bytes: NULL will do
  */
 size_t tab_linear8_packed_workspace_bytes(int out_dtype, int M, int N, int K);
@@ -320,7 +321,7 @@ int tab_linear8(const void *dev_X, int dtype, long ldx, const void *dev_QW, cons
  *   dev_w_post, dev_w_pre  fp32 [D], or NULL (1)
  *   dev_R         M x D
  *   dev_H, dev_S  M x D and NULL; or the packed operand of H, E4M3 with blocks of 1 x 128; or both NULL: not wanted
- * D is at most 16384.
+ * D is at most 16384.  A row whose squares add up beyond fp32 (its rms times sqrt(D) above 1.8e19) has rms(v) = 0.
  */
 int tab_norm_residual(const void *dev_X, long ldx, const void *dev_Y, long ldy, const void *dev_gate, int gate_dtype, int gates,
                       const float *dev_w_post, const float *dev_w_pre, float alpha, float eps, int dtype, int M, int D, void *dev_R, void *dev_H,

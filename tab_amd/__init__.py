@@ -201,8 +201,9 @@ def Quantize8Both(X, M, K, block_rows=1, format=E4M3):
 
 def Linear8(X, QW, SW, M, N, K):
     """X (M x K, quantized on the way as Quantize8 does) times the transpose of the packed weight (N x K, E4M3, blocks of 128 x 128 or of
-    one row): Y (M, N) of X's type.  Sums in fp32.  Up to 32 rows, their packed numbers at most 72 KB, are
-    quantized and multiplied in one launch."""
+    one row): Y (M, N) of X's type.  Sums in fp32; towards a 16-bit Y the products of eight neighbours in K are added with 13 bits below the
+    largest of them (some 1.5e-5 of Y's size, below its rounding), towards an fp32 one with all of theirs: for those from a 16-bit X, quantize it
+    and call Linear8Packed.  Up to 32 rows, their packed numbers at most 72 KB, are quantized and multiplied in one launch."""
     try:
         return _C.Linear8(X, QW, SW, M, N, K)
     except TypeError:
@@ -210,7 +211,8 @@ def Linear8(X, QW, SW, M, N, K):
 
 
 def Linear8Packed(QX, SX, QW, SW, M, N, K, out_dtype=torch.float32):
-    """Linear8 on an activation that is already packed (E4M3 or E5M2, blocks of one row): Y (M, N) of out_dtype."""
+    """Linear8 on an activation that is already packed (E4M3 or E5M2, blocks of one row): Y (M, N) of out_dtype, the sums of an
+    fp32 one with all their bits."""
     try:
         return _C.Linear8Packed(QX, SX, QW, SW, M, N, K, out_dtype)
     except TypeError:

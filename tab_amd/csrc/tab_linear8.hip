@@ -4,7 +4,8 @@
 // 16-bit outputs: v_mfma_scale_f32_16x16x128_f8f6f4.  One instruction is a 16 x 16 tile over one block of K, and it takes the E8M0 bytes of its
 // 16 rows and 16 columns as operands, so the scales cost no vector instruction and the sums stay in one set of fp32 accumulators.  Inside
 // the instruction, products of eight neighbours in K are aligned to the largest of them and keep 13 bits below it (measured): 1.5e-5 of the
-// output's size for normal operands, far below the 2^-8 or 2^-11 of the output's own rounding, but not what an fp32 output is for.
+// output's size for normal operands, far below the 2^-8 or 2^-11 of the output's own rounding, but not what an fp32 output is for.  (512 x 4096 x 4096: 1.2 % of
+// the bf16 outputs are the other neighbour of what the fp32 output rounds to; off the fp32 output by 0.0016633 of its size instead of 0.0016632.)
 // fp32 outputs (EXACT): the numbers times their scales are bf16 numbers exactly (4 of 8 significant bits, the exponent range of fp32), made by one
 // conversion of two numbers, and v_mfma_f32_16x16x32_bf16 multiplies them at half the rate with full fp32 sums.  A number below 2^-126 may
 // count as zero there.
@@ -123,7 +124,8 @@ template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v)
 // by the way of its operands into LDS (54 bytes a clock and CU measured; reads of LDS reach 200).  What cost most was a wave that waits to get a load
 // out, or whose scalar instructions make the load's address, and does not multiply meanwhile.  So a step's operands are read from LDS while the
 // step before is multiplied, loads, reads and products alternate, and a load takes two scalar instructions and one addition.
-//   256 x 256  8192^3 432-456 us, 2.4-2.5 PFLOP/s (a library's fp8 product with one scale a tensor 361); all loads between the products 426-478
+//   256 x 256  8192^3 404-406 us, 2.7 PFLOP/s, in a replayed graph (432-442 with X's quantizer; 430-460 under a profiler's trace; a library's fp8 product with one
+//              scale a tensor 361)
 //   128 x 128  4096 x 2048 x 4096 37-41 us, 1.7-1.9 PFLOP/s
 //   64 x 128   512 x 4096 x 4096 13.8 us, 1.25 PFLOP/s (64 x 64 16.4; both 19 with read and multiplied in turn)
 //   64 x 64    128 x 4096 x 4096 9.0 us (14.0 in turn); fp32 1000 x 776 x 520 6.6 us
@@ -442,8 +444,13 @@ struct RowsParams {
     Div32 div_kb;
 };
 
+// The bound between one launch and quantizer, tiles and join: X in 72 KB of LDS, which up to 16 rows (with 8 KB for the waves' sums) leaves room for two workgroups
+// a CU; with 17 to 32 rows the sums take 16 KB, and a CU holds one.  On both sides of it (bf16, by 4096 columns, a pass among others, us):
+//   one launch   8 x 4096  8.7   12 x 4096 10.4   17 x 4096 13.0   8 x 8000 15.0   32 x 2176 12.3   32 x 1000 7.4   by 1003 columns 24 x 2050 9.0, 32 x 2050 10.4
+//   three        18 x 4096 10.6                                    8 x 9300 12.7   32 x 2304  9.5   33 x 1000 7.0   by 1003 columns 33 x 2050 9.0
+// So the largest X in one launch take up to a fifth longer than three launches would; they meet at about 12 rows of 4096.
 constexpr int kRowsMost = 32;           // rows of X
-constexpr int kRowsLds = 72 << 10;      // bytes of X in LDS: 16 rows of 4096 and two workgroups a CU
+constexpr int kRowsLds = 72 << 10;      // bytes of X in LDS
 constexpr int kRowsWaves = 8;
 
 __host__ __device__ __forceinline__ int rows_stride(int KB) { return KB * kBlock8 + 16; }

@@ -185,8 +185,10 @@ __global__ __launch_bounds__(RowsOfGroup<LANES>::THREADS) void norm_residual(con
 //   s = sum over a gate's rows of t Y q:  dgate = s w_post,  dw_post = sum over gates of gate s
 // p and q are made anew from R and Y, which are here anyway, so the forward pass keeps nothing.  Sums over rows: a group of lanes adds up
 // its own rows in registers and leaves them in the workspace, a second launch adds the groups up in a fixed order.
-// bf16 16384 x 4096 with 16 gates: 162-167 us, 805 MB at 4.8-5.0 TB/s, and 11-13 for the join; fp32 777 x 1531 with a gate for each row: 17.6-17.9 in
-// all (two rows to a group; with three 19.1-19.6).  The next row is loaded before this one's sums are taken, as a row alone is all latency.
+// bf16 16384 x 4096 with 16 gates: 162-167 us, 805 MB at 4.8-5.0 TB/s, and 11-13 for the join; fp32 777 x 1531 with a gate for each row: 14.5 and 4
+// (two rows to a group; with three 16.7 and 4).  A group that keeps a gate's, both weights' and their sums' eight columns a lane beside the row's operands needs more
+// registers than there are for rows beyond 8192 (two runs a lane: 172 to 591 spilled; bf16 4096 x 16384 480 us, of 157 for its bytes, with a gate a row 910 of 210) and,
+// with a gate a row, beyond 2048 in fp32 and 16 bits (16 to 37 spilled; bf16 16384 x 4096 378 us of 210, fp32 470 of 419).  The next row is loaded before this one's sums are taken, as a row alone is all latency.
 
 struct NormGradParams {
     const void *dr, *dh, *r, *y, *gate;

@@ -123,7 +123,8 @@ class TABPackedChain(nn.Module):
 def linear8(x, w, grad_format=E4M3):
     """x (..., K) times the transpose of w (N, K) in 8-bit numbers with a scale per block of 128: y (..., N) of x's type.  Differentiable
     in x and w: dx = dy w and dw = dy^T x are products of the same kind, dy packed in grad_format (E5M2 where its range needs more than
-    a scale per block of 128 gives) along its rows and its columns.  w is packed anew in every call: for weights that stay, see Linear8."""
+    a scale per block of 128 gives) along its rows and its columns.  w is packed anew in every call: for weights that stay, see Linear8.
+    The sums are those of tab_amd.Linear8Packed towards x's type.  Second derivatives and forward mode are errors."""
     if not isinstance(x, torch.Tensor) or not isinstance(w, torch.Tensor):
         raise TypeError("x and w must be torch.Tensors")
     return _C.linear8(x, w, int(grad_format))
