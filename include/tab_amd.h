@@ -339,6 +339,89 @@ int tab_norm_residual_backward(const void *dev_dR, const void *dev_dH, const voi
                                void *dev_dX, void *dev_dY, void *dev_dgate, float *dev_dw_post, float *dev_dw_pre, void *workspace,
                                size_t workspace_bytes, void *stream);
 
+/*
+ * Weights of 4 bits.  E matrices W of M x K, row after row, are packed one by one as
+ *   Q  E2M1 numbers (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives), two a byte with the first in the low bits, [E][M][64 * ceil(K/128)], zeros past K,
+ *      16-byte aligned
+ *   S  E8M0 bytes [E][ceil(K/128)][M][4], one for each group of 32 of a row, 4-byte aligned
+ * A group's scale is the smallest power of two from 2^-126 on with which its largest magnitude fits, a packed number the nearest one to W, half to
+ * even.  The format knows neither infinities nor NaN: a group that holds one has the scale 255, NaN.
+ */
+int tab_quantize4(const void *dev_W, int dtype, int E, int M, int K, long ldw, void *dev_Q, void *dev_S, void *stream);
+
+/*
+ * tab_linear8_packed and tab_linear8 (see there for sums and workspaces) with one such weight (N x K); the packed activation in E4M3.
+ */
+size_t tab_linear4_packed_workspace_bytes(int out_dtype, int M, int N, int K);
+int tab_linear4_packed(const void *dev_QX, const void *dev_SX, const void *dev_QW, const void *dev_SW, int M, int N, int K, void *dev_Y, int out_dtype,
+                       void *workspace, size_t workspace_bytes, void *stream);
+size_t tab_linear4_workspace_bytes(int dtype, int M, int N, int K);
+int tab_linear4(const void *dev_X, int dtype, long ldx, const void *dev_QW, const void *dev_SW, int M, int N, int K, void *dev_Y, void *workspace,
+                size_t workspace_bytes, void *stream);
+
+/*
+ * The router of a layer of E experts (at most 1024): of each of M tokens the k (at most 32) experts with the largest logits, ties to the lower index.
+ *   dev_logits   M x E of type dtype, rows ld elements apart
+ *   normalize    weights are the softmax over the chosen experts (1) or over all of them (0)
+ *   dev_weights  fp32 [M][k], dev_experts int32 [M][k], the largest logit first
+ * An expert at -inf is never chosen: a token with fewer open ones has the weight 0, the expert -1 and the place -1 in what remains.  NaN is chosen first, and
+ * the weights of its token are NaN.  The M * k rows are put in order by expert, then by token:
+ *   dev_offsets  int32 [E + 1]: expert e has the rows offsets[e] .. offsets[e + 1]
+ *   dev_rows     int32 [M * k]: the token of each row, -1 behind offsets[E]
+ *   dev_places   int32 [M][k]: the row of each choice
+ *   workspace    tab_route_workspace_bytes(M, E, k) bytes, 16-byte aligned; 0 bytes: NULL will do
+ */
+size_t tab_route_workspace_bytes(int M, int E, int k);
+int tab_route(const void *dev_logits, int dtype, long ld, int M, int E, int k, int normalize, float *dev_weights, int *dev_experts, int *dev_rows, int *dev_places,
+              int *dev_offsets, void *workspace, size_t workspace_bytes, void *stream);
+/* dev_dlogits (M x E of dtype, rows contiguous) from the gradients of the weights (fp32 [M][k]). */
+int tab_route_backward(const float *dev_dweights, const float *dev_weights, const int *dev_experts, const void *dev_logits, int dtype, long ld, int M, int E, int k,
+                       int normalize, void *dev_dlogits, void *stream);
+
+/*
+ * Products of rows sorted by expert: row r of Y (R x N, rows contiguous) is row rows[r] of X (M x K) times the transpose of its expert's weight; rows behind
+ * offsets[E] are zeros.  Of rows and offsets that a program makes itself: a row outside X counts as zeros; offsets have to be in order, from 0 to at most R
+ * (others leave Y undefined, but nothing outside the tensors is touched).
+ *   dev_rows      int32 [R], or NULL: row r (M is R then)
+ *   w_bits        8: E packed E4M3 weights of N x K, one behind the other, each with its scales (blocks of w_block_rows x 128; see tab_quantize8_experts);
+ *                 4: those of tab_quantize4
+ * tab_experts_linear quantizes X on the way (E4M3, 1 x 128); Y has X's type.  Few rows to an expert take one launch.  tab_experts_linear_packed takes X packed;
+ * full_sums 0 lets an fp32 Y have the sums of a 16-bit one (8-bit weights; see tab_linear8_packed).  X may take at most 3.5 GiB packed, or any size
+ * where few rows take one launch.
+ */
+size_t tab_experts_linear_workspace_bytes(int dtype, int M, int R, int E, int N, int K);
+int tab_experts_linear(const void *dev_X, int dtype, long ldx, int M, const int *dev_rows, const int *dev_offsets, const void *dev_QW, const void *dev_SW, int w_bits,
+                       int w_block_rows, int R, int E, int N, int K, void *dev_Y, void *workspace, size_t workspace_bytes, void *stream);
+size_t tab_experts_linear_packed_workspace_bytes(int out_dtype, int R, int E, int N, int K);
+int tab_experts_linear_packed(const void *dev_QX, int x_format, const void *dev_SX, int M, const int *dev_rows, const int *dev_offsets, const void *dev_QW,
+                              const void *dev_SW, int w_bits, int w_block_rows, int R, int E, int N, int K, void *dev_Y, int out_dtype, int full_sums,
+                              void *workspace, size_t workspace_bytes, void *stream);
+
+/* E weights of N x K, row after row, packed one by one in E4M3 with blocks of 128 x 128, and transposed (K x N) as the gradient of X takes them; either
+ * pair may be NULL. */
+int tab_quantize8_experts(const void *dev_W, int dtype, int E, int N, int K, long ldw, void *dev_Q, void *dev_S, void *dev_QT, void *dev_ST, void *stream);
+
+/*
+ * Rows sorted by expert, packed for the gradients of the weights.  dev_QT, dev_ST: the rows of X as they are sorted, transposed, in blocks of 128 rows that belong
+ * to one expert: K x (128 * tab_run_blocks(R, E)) numbers and [tab_run_blocks(R, E)][K] scales, of which the experts' own blocks are written, one expert's
+ * behind the other's.  dev_Q, dev_S: the sorted rows packed as tab_quantize8 does, those behind offsets[E] not written; or both NULL.
+ */
+int tab_run_blocks(int R, int E);
+int tab_quantize8_by_expert(const void *dev_X, int dtype, long ldx, int M, const int *dev_rows, const int *dev_offsets, int R, int E, int K, int format, void *dev_Q,
+                            void *dev_S, void *dev_QT, void *dev_ST, void *stream);
+/* dW[e] (N x K) = sum over the rows r of expert e of dY[r]^T X[r], from dY (R x N) and X (E4M3) packed by tab_quantize8_by_expert; zeros for an expert without rows. */
+int tab_experts_grad_weight(const void *dev_QD, int d_format, const void *dev_SD, const void *dev_QX, const void *dev_SX, const int *dev_offsets, int R, int E, int N,
+                            int K, void *dev_dW, int out_dtype, void *stream);
+
+/*
+ * The experts' rows back to their tokens: out[t] (M x D) = sum over j of weights[t][j] Y[places[t][j]], Y R x D; a place outside Y is left out.  weights NULL: ones.
+ * out has Y's type, or with an fp32 Y any.  Its gradients (each NULL where it is not wanted): dY[places[t][j]] = weights[t][j] dout[t], zeros from row
+ * used[0] on (NULL: R), and dweights[t][j] = dout[t] . Y[places[t][j]].  No row may be two choices' place, and the rows below used[0] are all somebody's.
+ */
+int tab_combine(const void *dev_Y, int dtype, const int *dev_places, const float *dev_weights, int M, int k, int R, int D, void *dev_out, int out_dtype, void *stream);
+int tab_combine_backward(const void *dev_dout, const void *dev_Y, int dtype, const int *dev_places, const float *dev_weights, const int *dev_used, int M, int k, int R,
+                         int D, void *dev_dY, float *dev_dweights, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -273,6 +273,142 @@ def NormBackward(dH, X, w, eps, M, D):
         return _call_norm(_C.NormBackward, {"dH": dH, "X": X}, {"w": w}, (eps,), (M, D))
 
 
+def Quantize4(X, M, K):
+    """Pack weights X (M x K; fp32, bf16 or fp16; contiguous or rows of a wider matrix) in 4-bit numbers (E2M1) with a power-of-two scale per
+    group of 32 of a row: the smallest one, from 2^-126, with which the group's largest magnitude fits 6.  A packed number is the nearest one to X, half
+    to even.  The format has no infinity and no NaN: a group that holds one has the scale NaN.  Returns [Q, S]: Q float4_e2m1fn_x2
+    (M, 64 * blocks8(K)), two numbers an element, the first in the low bits, zeros past K; S float8_e8m0fnu (blocks8(K), M, 4)."""
+    try:
+        return _C.Quantize4(X, M, K)
+    except TypeError:
+        return _call(_C.Quantize4, {"X": X}, (M, K))
+
+
+def Linear4(X, QW, SW, M, N, K):
+    """Linear8 with a weight that Quantize4 packed: X (M x K) is quantized on the way to 8 bits, Y (M, N) has X's type, sums as there."""
+    try:
+        return _C.Linear4(X, QW, SW, M, N, K)
+    except TypeError:
+        return _call(_C.Linear4, {"X": X, "QW": QW, "SW": SW}, (M, N, K))
+
+
+def Linear4Packed(QX, SX, QW, SW, M, N, K, out_dtype=torch.float32):
+    """Linear4 on an activation that is already packed (E4M3, blocks of one row), as Linear8Packed."""
+    try:
+        return _C.Linear4Packed(QX, SX, QW, SW, M, N, K, out_dtype)
+    except TypeError:
+        if not isinstance(out_dtype, torch.dtype):
+            raise TypeError("out_dtype must be a torch.dtype")
+        return _call(_C.Linear4Packed, {"QX": QX, "SX": SX, "QW": QW, "SW": SW}, (M, N, K), out_dtype)
+
+
+def Route(logits, M, E, k, normalize=True):
+    """The router of a layer of E experts (at most 1024): for each of M tokens the k (at most 32) experts with the largest logits (M x E), ties to
+    the lower index.  Returns [weights, experts, rows, places, offsets]:
+
+        weights  fp32 (M, k)      softmax over the chosen experts, or with normalize=False over all of them
+        experts  int32 (M, k)     the largest logit first
+        rows     int32 (M * k,)   the token of each row, the rows in order by expert, then by token
+        places   int32 (M, k)     the row of each choice
+        offsets  int32 (E + 1,)   expert e has the rows offsets[e] .. offsets[e + 1]
+
+    An expert at -inf is never chosen: a token with fewer open ones (a padded one has none) has weight 0, expert -1 and place -1 in what remains, and the rows
+    behind offsets[E] are -1.  NaN is chosen first and makes its token's weights NaN."""
+    try:
+        return _C.Route(logits, M, E, k, normalize)
+    except TypeError:
+        return _call(_C.Route, {"logits": logits}, (M, E, k), bool(normalize))
+
+
+def RouteBackward(dweights, weights, experts, logits, M, E, k, normalize=True):
+    """Gradient of Route: that of the logits (M, E) from those of the weights (fp32)."""
+    try:
+        return _C.RouteBackward(dweights, weights, experts, logits, M, E, k, normalize)
+    except TypeError:
+        return _call(_C.RouteBackward, {"dweights": dweights, "weights": weights, "experts": experts, "logits": logits}, (M, E, k), bool(normalize))
+
+
+def QuantizeExperts(W, E, N, K, bits=8, transposed=False):
+    """Pack the weights W (E, N, K) of E experts one by one: bits=8 as Quantize8 does in blocks of 128 x 128, [Q (E, N, 128 * blocks8(K)),
+    S (E, blocks8(K), blocks8(N))], with transposed=True also [QT, ST] of each one transposed; bits=4 as Quantize4 does."""
+    try:
+        return _C.QuantizeExperts(W, E, N, K, bits, transposed)
+    except TypeError:
+        return _call(_C.QuantizeExperts, {"W": W}, (E, N, K, bits), bool(transposed))
+
+
+def _call_rows(fn, before, rows, after, ints, *rest):
+    """As _call, where rows may be None."""
+    for name, t in {**before, "rows": rows, **after}.items():
+        if not isinstance(t, torch.Tensor) and not (t is None and name == "rows"):
+            raise TypeError(f"{name} must be a torch.Tensor" + (" or None" if name == "rows" else ""))
+    return fn(*before.values(), rows, *after.values(), *(int(v) for v in ints), *rest)
+
+
+def ExpertsLinear(X, rows, offsets, QW, SW, M, R, E, N, K):
+    """Rows sorted by expert times their expert's weight: Y (R, N) of X's type, Y[r] = X[rows[r]] QW[e]^T for offsets[e] <= r < offsets[e + 1], zeros
+    behind offsets[E].  X (M x K) is quantized on the way as Linear8 does; rows and offsets are Route's, rows None where X is sorted already (M = R).  QW, SW:
+    the experts' weights from QuantizeExperts, 8 or 4 bits.  Few rows to an expert take one launch; otherwise X may take at most 3.5 GiB packed."""
+    try:
+        return _C.ExpertsLinear(X, rows, offsets, QW, SW, M, R, E, N, K)
+    except TypeError:
+        return _call_rows(_C.ExpertsLinear, {"X": X}, rows, {"offsets": offsets, "QW": QW, "SW": SW}, (M, R, E, N, K))
+
+
+def ExpertsLinearPacked(QX, SX, rows, offsets, QW, SW, M, R, E, N, K, out_dtype=torch.float32):
+    """ExpertsLinear on an activation that is already packed (blocks of one row): Y (R, N) of out_dtype."""
+    try:
+        return _C.ExpertsLinearPacked(QX, SX, rows, offsets, QW, SW, M, R, E, N, K, out_dtype)
+    except TypeError:
+        if not isinstance(out_dtype, torch.dtype):
+            raise TypeError("out_dtype must be a torch.dtype")
+        return _call_rows(_C.ExpertsLinearPacked, {"QX": QX, "SX": SX}, rows, {"offsets": offsets, "QW": QW, "SW": SW}, (M, R, E, N, K), out_dtype)
+
+
+def run_blocks(R, E):
+    """Blocks of 128 rows that R rows take at most when each of E experts' rows begin at a new one."""
+    return _lib.tab_run_blocks(int(R), int(E))
+
+
+def Quantize8ByExpert(X, rows, offsets, M, R, E, K, format=E4M3, sorted=False):
+    """The R rows by expert of X (M x K), packed for the gradients of the weights: [QT, ST], transposed, in blocks of 128 rows that belong to one
+    expert, QT (K, 128 * run_blocks(R, E)), ST (run_blocks(R, E), K); with sorted=True [Q, S, QT, ST], Q and S as Quantize8 of the sorted rows (those
+    behind offsets[E] are not written)."""
+    try:
+        return _C.Quantize8ByExpert(X, rows, offsets, M, R, E, K, format, sorted)
+    except TypeError:
+        return _call_rows(_C.Quantize8ByExpert, {"X": X}, rows, {"offsets": offsets}, (M, R, E, K, format), bool(sorted))
+
+
+def ExpertsGradWeight(QD, SD, QX, SX, offsets, R, E, N, K, out_dtype=torch.float32):
+    """Gradients of the experts' weights (E, N, K): dY_e^T X_e from dY (R x N) and X (R x K, E4M3), both packed by Quantize8ByExpert; zeros for an
+    expert without rows."""
+    try:
+        return _C.ExpertsGradWeight(QD, SD, QX, SX, offsets, R, E, N, K, out_dtype)
+    except TypeError:
+        if not isinstance(out_dtype, torch.dtype):
+            raise TypeError("out_dtype must be a torch.dtype")
+        return _call(_C.ExpertsGradWeight, {"QD": QD, "SD": SD, "QX": QX, "SX": SX, "offsets": offsets}, (R, E, N, K), out_dtype)
+
+
+def Combine(Y, places, weights, M, k, R, D):
+    """The experts' rows back to their tokens: out (M, D) of Y's type, out[t] = sum over j of weights[t, j] Y[places[t, j]], Y (R, D), weights fp32 or None
+    (ones); a place that is no row of Y is left out."""
+    try:
+        return _C.Combine(Y, places, weights, M, k, R, D)
+    except TypeError:
+        return _call_norm(_C.Combine, {"Y": Y, "places": places}, {"weights": weights}, (), (M, k, R, D))
+
+
+def CombineBackward(dout, Y, places, weights, offsets, M, k, R, D):
+    """Gradients of Combine: [dY, dweights], the latter None without weights.  Rows from offsets[-1] on (offsets None: R) are zeros; those below it have to be
+    the place of one choice each, as Route makes them."""
+    try:
+        return _C.CombineBackward(dout, Y, places, weights, offsets, M, k, R, D)
+    except TypeError:
+        return _call_norm(_C.CombineBackward, {"dout": dout, "Y": Y, "places": places}, {"weights": weights, "offsets": offsets}, (), (M, k, R, D))
+
+
 CONV_AUTO, CONV_MATRIX, CONV_POPCOUNT = 0, 1, 2
 
 
@@ -290,4 +426,6 @@ __all__ = ["Quantize", "QuantizeNCHW", "QuantizeActivation", "conv2d_launches", 
            "packed_channels", "out_shape", "version", "TNN", "TBN", "BTN", "BNN", "set_conv_kernel",
            "CONV_AUTO", "CONV_MATRIX", "CONV_POPCOUNT",
            "Quantize8", "Quantize8Transposed", "Quantize8Both", "Linear8", "Linear8Packed", "blocks8", "E4M3", "E5M2",
-           "Norm", "NormResidual", "NormResidualBackward", "NormBackward", "NORM_NONE", "NORM_PLAIN", "NORM_8BIT"]
+           "Norm", "NormResidual", "NormResidualBackward", "NormBackward", "NORM_NONE", "NORM_PLAIN", "NORM_8BIT",
+           "Quantize4", "Linear4", "Linear4Packed", "Route", "RouteBackward", "QuantizeExperts", "ExpertsLinear", "ExpertsLinearPacked", "run_blocks",
+           "Quantize8ByExpert", "ExpertsGradWeight", "Combine", "CombineBackward"]

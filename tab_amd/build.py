@@ -8,8 +8,10 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libtab_amd.so")
 SOURCES = ["tab_capi.hip", "tab_conv.hip", "tab_conv_mfma_tnn.hip", "tab_conv_mfma_tbn.hip", "tab_conv_mfma_btn.hip",
            "tab_conv_mfma_bnn.hip", "tab_conv_mfma_drf.hip", "tab_conv_mfma_rtn.hip", "tab_conv_fused1x1.hip", "tab_conv_small.hip", "tab_quantize.hip", "tab_quantize_item.hip",
-           "tab_capi8.hip", "tab_quantize8.hip", "tab_linear8.hip", "tab_norm_residual.hip"]
-EXTENSION_SOURCES = ["torch_binding.cpp", "torch_binding8.cpp"]
+           "tab_capi8.hip", "tab_quantize8.hip", "tab_linear8.hip", "tab_norm_residual.hip",
+           "tab_capi_experts.hip", "tab_quantize4.hip", "tab_linear4.hip", "tab_experts8.hip", "tab_experts4.hip", "tab_experts_grad.hip", "tab_route.hip",
+           "tab_combine.hip"]
+EXTENSION_SOURCES = ["torch_binding.cpp", "torch_binding8.cpp", "torch_binding_experts.cpp"]
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -packed-fp32-ops: keep the compiler from forming packed-FP32 VALU ops from float code.

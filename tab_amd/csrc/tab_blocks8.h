@@ -247,6 +247,7 @@ struct Quantize8Args {
     uint8_t *q, *s, *qt, *st;  // either pair may be null
     int M, K;
     long ldx;  // elements between rows of x
+    int matrices = 1;  // with blocks of 128 x 128: M x K each, the rows of one behind those of the other
 };
 // workgroups of a launch (of 256 threads; a launch may hold 2^32 threads)
 long quantize8_tiles(int block_rows, bool transposed, int M, int K);
@@ -264,6 +265,9 @@ long linear8_threads(int out_dtype, int M, int N, int KB);  // of the launch
 int linear8_way(int out_dtype, int M, int N, int KB);  // 0: few rows; else (the tile's rows + columns) / 2 * 100 + the parts of K
 hipError_t launch_linear8(int out_dtype, int x_format, const Linear8Args &a, void *workspace, hipStream_t stream);
 
+// Rows sorted by expert (tab_experts.h): M rows, in QT by blocks of 128 that belong to one expert
+hipError_t launch_quantize8_by_expert(int dtype, int format, const Quantize8Args &a, const int *offsets, const int *rows, int E, int x_rows, hipStream_t stream);
+
 // The product that quantizes a few rows of x itself.
 bool linear8_rows_supported(int M, int K);
 struct Linear8RowsArgs {
@@ -275,6 +279,19 @@ struct Linear8RowsArgs {
     long ldx;
 };
 hipError_t launch_linear8_rows(int dtype, const Linear8RowsArgs &a, hipStream_t stream);
+
+// Weights of 4 bits (tab_quantize4.hip, tab_linear4.hip): E matrices of M x K, row after row.  A packed one is Q, two E2M1 numbers a byte (the first in the
+// low bits), [M][64 * ceil(K / 128)] with zeros past K, and S, E8M0 bytes of groups of 32, [ceil(K / 128)][M][4].
+struct Quantize4Args {
+    const void *x;
+    uint8_t *q, *s;
+    int E, M, K;
+    long ldx;
+};
+long quantize4_tiles(long rows, int K);  // workgroups of 256 threads
+hipError_t launch_quantize4(int dtype, const Quantize4Args &a, hipStream_t stream);
+hipError_t launch_linear4(int out_dtype, const Linear8Args &a, void *workspace, hipStream_t stream);  // (w_block_rows is not read)
+hipError_t launch_linear4_rows(int dtype, const Linear8RowsArgs &a, hipStream_t stream);
 
 struct NormArgs {
     const void *x, *y, *gate;      // y and gate may be null

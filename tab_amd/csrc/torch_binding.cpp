@@ -10,6 +10,7 @@
 using namespace tab_torch;
 
 void bind_layers8(pybind11::module_ &m);  // torch_binding8.cpp
+void bind_experts(pybind11::module_ &m);  // torch_binding_experts.cpp
 
 namespace {
 
@@ -634,6 +635,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("Conv2dPacked", &TAB_Conv2dPacked, "Conv2d on an already packed activation");
     m.def("Conv2dPackedOut", &TAB_Conv2dPackedOut, "Conv2dPacked with the output quantized and packed in the epilogue");
     bind_layers8(m);
+    bind_experts(m);
     make_fast<&TAB_Conv2d, 4, 12>(m, "Conv2d");
     make_fast<&TAB_Conv2d, 4, 12, 1>(m, "TAB_Conv2d");
     make_fast<&TAB_Quantize, 2, 5>(m, "Quantize");

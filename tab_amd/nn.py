@@ -1,15 +1,18 @@
 """Layer wrappers around the two operators: the caller the reference's demo notebook gestures
 at (it imports torch.nn and autograd.Function, TAB Demo CUDA.ipynb cell 1, but ships none).
 Inference only (the operators have no backward).  Beside them the 8-bit layers and the norms around a block (linear8,
-norm_residual, Linear8, ResidualStack), which have one.
+norm_residual, Linear8, ResidualStack), which have one, layers of 4-bit weights for inference (Linear4), and layers of experts (route, experts_linear8, combine,
+MixtureOfExperts).
 
     layer = TABConv2d.from_float(weight_kn_c_kh_kw, conv_type=tab_amd.TNN, stride=1, padding=1)
     y = layer(x)            # x: (N, C, H, W) fp32 on the GPU -> (N, KN, OH, OW), logical NCHW
 """
+from typing import NamedTuple
+
 import torch
 from torch import nn
 
-from . import _C, BNN, BTN, E4M3, NORM_8BIT, NORM_PLAIN, TBN, TNN, Linear8Packed, Quantize, Quantize8, Threshold
+from . import _C, BNN, BTN, E4M3, NORM_8BIT, NORM_PLAIN, TBN, TNN, Linear4Packed, Linear8Packed, Quantize, Quantize4, Quantize8, QuantizeExperts, Threshold
 
 _ACT_BITS = {TNN: 2, TBN: 2, BTN: 1, BNN: 1}
 _WEIGHT_BITS = {TNN: 2, TBN: 1, BTN: 2, BNN: 1}
@@ -138,7 +141,26 @@ def norm_residual(x, y=None, gate=None, w_post=None, w_pre=None, alpha=1.0, eps=
     return _C.norm_residual(x, y, gate, w_post, w_pre, float(alpha), float(eps), int(output))
 
 
-class Linear8(nn.Module):
+# Types of packed weights: what they hold is bytes, whatever a module is converted to
+_PACKED_TYPES = (torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.float4_e2m1fn_x2)
+
+
+class _PackedWeight(nn.Module):
+    """A layer whose buffers are packed numbers."""
+
+    def _apply(self, fn, recurse=True):
+        """What moves or converts the module moves the packed weight, whose types are its format: fn sees their bytes, and a conversion to another type leaves
+        them as they are."""
+        def bytes_alone(t):
+            if t.dtype not in _PACKED_TYPES:
+                return fn(t)
+            moved = fn(t.view(torch.uint8))
+            return moved.view(t.dtype) if moved.dtype == torch.uint8 else t.to(moved.device)
+
+        return super()._apply(bytes_alone, recurse)
+
+
+class Linear8(_PackedWeight):
     """Fully connected layer on 8-bit numbers, for the layers of a low-bit network that keep more than two bits.  Holds the packed weight
     (QW, SW) as buffers.  Input (..., in_features) of fp32, bf16 or fp16, or the pair (QH, SH) that a norm packed (then `rows` x out_features
     of out_dtype); output (..., out_features)."""
@@ -156,17 +178,6 @@ class Linear8(nn.Module):
         QW, SW = Quantize8(weight.detach().cuda().contiguous(), N, K, 128)
         return cls(QW, SW, K, N, out_dtype)
 
-    def _apply(self, fn, recurse=True):
-        """What moves or converts the module moves the packed weight, whose types are its format: fn sees their bytes, and a conversion to another type leaves
-        them as they are."""
-        def bytes_alone(t):
-            if t.dtype not in (torch.float8_e4m3fn, torch.float8_e8m0fnu):
-                return fn(t)
-            moved = fn(t.view(torch.uint8))
-            return moved.view(t.dtype) if moved.dtype == torch.uint8 else t.to(moved.device)
-
-        return super()._apply(bytes_alone, recurse)
-
     def forward(self, x):
         if isinstance(x, (tuple, list)):
             QX, SX = x
@@ -175,6 +186,120 @@ class Linear8(nn.Module):
 
     def extra_repr(self):
         return f"{self.in_features}, {self.out_features}"
+
+
+class Linear4(Linear8):
+    """Linear8 with a weight of 4 bits and a scale per group of 32, for inference where the weights' bytes are what counts.  Inputs and outputs as there."""
+
+    @classmethod
+    def from_float(cls, weight, out_dtype=torch.float32):
+        """Pack a weight of PyTorch's shape (out_features, in_features) on the GPU."""
+        N, K = weight.shape
+        QW, SW = Quantize4(weight.detach().cuda().contiguous(), N, K)
+        return cls(QW, SW, K, N, out_dtype)
+
+    def forward(self, x):
+        if isinstance(x, (tuple, list)):
+            QX, SX = x
+            return Linear4Packed(QX, SX, self.QW, self.SW, QX.shape[0], self.out_features, self.in_features, self.out_dtype)
+        return _C.linear4_packed_weight(x, self.QW, self.SW, self.out_features, self.in_features)
+
+
+class Routing(NamedTuple):
+    """What tab_amd.Route returns: a step's choice of experts, and the order of its rows."""
+
+    weights: torch.Tensor
+    experts: torch.Tensor
+    rows: torch.Tensor
+    places: torch.Tensor
+    offsets: torch.Tensor
+
+
+def route(logits, k, normalize=True):
+    """tab_amd.Route on logits (..., E), a Routing of their tokens; its weights are differentiable in the logits."""
+    return Routing(*_C.route(logits, int(k), bool(normalize)))
+
+
+def experts_linear8(x, w, routing, gather=True, grad_format=E4M3):
+    """Rows sorted by expert times their expert's weight w (E, N, K) in 8-bit numbers: y (rows, N) of x's type, zeros in the rows of no expert.
+    x (..., K) holds the routing's tokens, or with gather=False its sorted rows, as a product before left them.  Differentiable in x and w as linear8 is: the
+    rows of a token are added up in fp32, blocks of 128 rows under one scale belong to one expert.  w is packed anew in every call: for weights that stay,
+    see PackedExperts."""
+    return _C.experts_linear8(x, w, routing.rows, routing.places, routing.offsets, bool(gather), int(grad_format))
+
+
+def combine(y, routing):
+    """The rows y (rows, D) of a routing back to its tokens, times their weights: (tokens, D).  Differentiable in y and in the weights."""
+    return _C.combine(y, routing.weights, routing.places, routing.offsets)
+
+
+class Experts8(nn.Module):
+    """The weights (E, out_features, in_features) of a layer of experts in training; forward is experts_linear8."""
+
+    def __init__(self, weight, grad_format=E4M3):
+        super().__init__()
+        self.weight = nn.Parameter(weight)
+        self.grad_format = int(grad_format)
+
+    def forward(self, x, routing, gather=True):
+        return experts_linear8(x, self.weight, routing, gather, self.grad_format)
+
+    def packed(self, bits=8):
+        """The layer for inference."""
+        return PackedExperts.from_float(self.weight, bits)
+
+    def extra_repr(self):
+        return "{}, {}, experts={}".format(self.weight.shape[2], self.weight.shape[1], self.weight.shape[0])
+
+
+class PackedExperts(_PackedWeight):
+    """A layer of experts for inference, its weights packed in 8 or 4 bits (QW, SW, buffers).  forward(x, routing) multiplies the routing's tokens x
+    (..., in_features) by their experts' weights, with gather=False its sorted rows: (rows, out_features) of x's type."""
+
+    def __init__(self, QW, SW, num_experts, in_features, out_features):
+        super().__init__()
+        self.num_experts, self.in_features, self.out_features = int(num_experts), int(in_features), int(out_features)
+        self.register_buffer("QW", QW)
+        self.register_buffer("SW", SW)
+
+    @classmethod
+    def from_float(cls, weight, bits=8):
+        """Pack weights (E, out_features, in_features) on the GPU."""
+        E, N, K = weight.shape
+        QW, SW = QuantizeExperts(weight.detach().cuda().contiguous(), E, N, K, bits)
+        return cls(QW, SW, E, K, N)
+
+    def forward(self, x, routing, gather=True):
+        return _C.experts_packed_weight(x, self.QW, self.SW, routing.rows, routing.places, routing.offsets, bool(gather), self.num_experts, self.out_features, self.in_features)
+
+    def extra_repr(self):
+        return f"{self.in_features}, {self.out_features}, experts={self.num_experts}"
+
+
+class MixtureOfExperts(nn.Module):
+    """A block whose weights are chosen by token: router(x) gives logits (tokens, E), the k largest choose the experts, each of which is `up`, an activation
+    and `down` (Experts8 or PackedExperts; down may be None), and a token's rows are added up by their weights.  Maps (..., D) to (..., D_out), so it is a block
+    of ResidualStack too."""
+
+    def __init__(self, router, up, down=None, k=2, normalize=True, activation=None):
+        super().__init__()
+        self.router, self.up, self.down, self.activation = router, up, down, activation
+        self.k, self.normalize = int(k), bool(normalize)
+
+    def forward(self, x):
+        tokens = x.reshape(-1, x.shape[-1])
+        routing = route(self.router(tokens), self.k, self.normalize)
+        y = self.up(tokens, routing)
+        if self.activation is not None:
+            y = self.activation(y)
+        if self.down is not None:
+            y = self.down(y, routing, gather=False)
+        return combine(y, routing).reshape(*x.shape[:-1], y.shape[-1])
+
+    def packed(self, bits=8):
+        """The block for inference: its experts' weights packed, the router as it is."""
+        down = None if self.down is None else self.down.packed(bits)
+        return MixtureOfExperts(self.router, self.up.packed(bits), down, self.k, self.normalize, self.activation)
 
 
 class _NoGradient(torch.autograd.Function):
@@ -196,8 +321,8 @@ class ResidualStack(nn.Module):
         y_i = block_i(h_i),   x_{i+1} = alpha x_i + gate_i * norm(y_i; w_post_i),   h_{i+1} = norm(x_{i+1}; w_pre_{i+1})
 
     Every block is followed by one NormResidual launch (norm, gate, residual, next norm); the output is the last norm, so that a head can
-    follow.  Blocks map (rows, D) to (rows, D): TABLinear layers, Linear8, or functions of linear8 in training; TABLinear's input is fp32 also
-    in a stream of 16 bits.  With a Linear8 as the next block and no gradient wanted, the norm packs its output for it.  `gates` of a call: one
+    follow.  Blocks map (rows, D) to (rows, D): TABLinear layers, Linear8, Linear4, MixtureOfExperts, or functions of linear8 in training; TABLinear's input is fp32 also
+    in a stream of 16 bits.  With a Linear8 or Linear4 as the next block and no gradient wanted, the norm packs its output for it.  `gates` of a call: one
     (G, D) tensor or None a block, in place of the learned gate per channel.  TABLinear layers have no backward pass: a gradient that would
     have to go through one is an error."""
 
