@@ -389,10 +389,10 @@ int tab_route_backward(const float *dev_dweights, const float *dev_weights, cons
  * full_sums 0 lets an fp32 Y have the sums of a 16-bit one (8-bit weights; see tab_linear8_packed).  X may take at most 3.5 GiB packed, or any size
  * where few rows take one launch.
  */
-size_t tab_experts_linear_workspace_bytes(int dtype, int M, int R, int E, int N, int K);
+size_t tab_experts_linear_workspace_bytes(int dtype, int w_bits, int M, int R, int E, int N, int K);
 int tab_experts_linear(const void *dev_X, int dtype, long ldx, int M, const int *dev_rows, const int *dev_offsets, const void *dev_QW, const void *dev_SW, int w_bits,
                        int w_block_rows, int R, int E, int N, int K, void *dev_Y, void *workspace, size_t workspace_bytes, void *stream);
-size_t tab_experts_linear_packed_workspace_bytes(int out_dtype, int R, int E, int N, int K);
+size_t tab_experts_linear_packed_workspace_bytes(int out_dtype, int full_sums, int w_bits, int R, int E, int N, int K);
 int tab_experts_linear_packed(const void *dev_QX, int x_format, const void *dev_SX, int M, const int *dev_rows, const int *dev_offsets, const void *dev_QW,
                               const void *dev_SW, int w_bits, int w_block_rows, int R, int E, int N, int K, void *dev_Y, int out_dtype, int full_sums,
                               void *workspace, size_t workspace_bytes, void *stream);

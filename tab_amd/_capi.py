@@ -58,9 +58,9 @@ SIGNATURES = {
     "tab_route_workspace_bytes": (_sz, [_int] * 3),
     "tab_route": (_int, [_vp, _int, ctypes.c_long] + [_int] * 4 + [_vp] * 6 + [_sz, _vp]),
     "tab_route_backward": (_int, [_vp] * 4 + [_int, ctypes.c_long] + [_int] * 4 + [_vp, _vp]),
-    "tab_experts_linear_workspace_bytes": (_sz, [_int] * 6),
+    "tab_experts_linear_workspace_bytes": (_sz, [_int] * 7),
     "tab_experts_linear": (_int, [_vp, _int, ctypes.c_long, _int] + [_vp] * 4 + [_int] * 6 + [_vp, _vp, _sz, _vp]),
-    "tab_experts_linear_packed_workspace_bytes": (_sz, [_int] * 5),
+    "tab_experts_linear_packed_workspace_bytes": (_sz, [_int] * 7),
     "tab_experts_linear_packed": (_int, [_vp, _int, _vp, _int] + [_vp] * 4 + [_int] * 6 + [_vp, _int, _int, _vp, _sz, _vp]),
     "tab_quantize8_experts": (_int, [_vp, _int, _int, _int, _int, ctypes.c_long] + [_vp] * 5),
     "tab_run_blocks": (_int, [_int] * 2),

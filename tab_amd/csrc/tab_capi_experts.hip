@@ -36,7 +36,7 @@ int check_runs(int M, const int *rows, const int *offsets, int R, int E)
     return TAB_OK;
 }
 
-int check_experts(int M, const int *rows, const int *offsets, int R, int E, int N, int K, int out_dtype, int w_bits, int w_block_rows)
+int check_experts(int M, const int *rows, const int *offsets, int R, int E, int N, int K, int out_dtype, bool full_sums, int w_bits, int w_block_rows)
 {
     TAB_CHECK(check_type(out_dtype, "out_dtype"));
     TAB_CHECK(check_weight_bits(w_bits, w_block_rows));
@@ -44,7 +44,7 @@ int check_experts(int M, const int *rows, const int *offsets, int R, int E, int 
     if (N < 1 || K < 1) return fail(TAB_ERR_BAD_ARGUMENT, "N and K must be positive");
     const int KB = tab::blocks8(K);
     if (N > kMostRows || KB > tab::kBlocks8Most) return fail(TAB_ERR_BAD_SHAPE, "product too large for 32-bit offsets into a tile");
-    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, R, E, N, KB);
+    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, full_sums, w_bits, R, E, N, KB);
     if (plan.workgroups * 512 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "product too large for one launch");
     if (!plan.few && (unsigned long)M * (unsigned long)KB * tab::kBlock8 > 0xe0000000ul)
         return fail(TAB_ERR_BAD_SHAPE, "X takes more than 3.5 GiB packed: too large for 32-bit offsets");
@@ -189,9 +189,9 @@ int tab_quantize8_by_expert(const void *dev_X, int dtype, long ldx, int M, const
     return e == hipSuccess ? TAB_OK : device_fail(e, "quantize8 launch");
 }
 
-size_t tab_experts_linear_packed_workspace_bytes(int out_dtype, int R, int E, int N, int K)
+size_t tab_experts_linear_packed_workspace_bytes(int out_dtype, int full_sums, int w_bits, int R, int E, int N, int K)
 {
-    return R < 1 || E < 1 || N < 1 || K < 1 ? 0 : parts_bytes(tab::experts_plan(out_dtype, R, E, N, tab::blocks8(K)), R, N);
+    return R < 1 || E < 1 || N < 1 || K < 1 ? 0 : parts_bytes(tab::experts_plan(out_dtype, full_sums != 0, w_bits, R, E, N, tab::blocks8(K)), R, N);
 }
 
 int tab_experts_linear_packed(const void *dev_QX, int x_format, const void *dev_SX, int M, const int *dev_rows, const int *dev_offsets, const void *dev_QW,
@@ -199,43 +199,43 @@ int tab_experts_linear_packed(const void *dev_QX, int x_format, const void *dev_
                               void *workspace, size_t workspace_bytes, void *stream)
 {
     TAB_CHECK(check_format(x_format));
-    TAB_CHECK(check_experts(M, dev_rows, dev_offsets, R, E, N, K, out_dtype, w_bits, w_block_rows));
+    TAB_CHECK(check_experts(M, dev_rows, dev_offsets, R, E, N, K, out_dtype, full_sums != 0, w_bits, w_block_rows));
     if (w_bits == 4 && x_format != TAB_E4M3) return fail(TAB_ERR_BAD_ARGUMENT, "weights of 4 bits take activations in E4M3");
     TAB_CHECK(check_packed(dev_QX, dev_SX, "QX or SX"));
     TAB_CHECK(check_packed(dev_QW, dev_SW, "QW or SW"));
     if (w_bits == 4 && (uintptr_t)dev_SW % 4) return fail(TAB_ERR_BAD_ARGUMENT, "SW must be aligned to 4 bytes");
     TAB_CHECK(check_rows(dev_Y, out_dtype, 1, N, N, "Y"));
-    TAB_CHECK(check_workspace(workspace, workspace_bytes, tab_experts_linear_packed_workspace_bytes(out_dtype, R, E, N, K)));
-    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, R, E, N, tab::blocks8(K));
+    TAB_CHECK(check_workspace(workspace, workspace_bytes, tab_experts_linear_packed_workspace_bytes(out_dtype, full_sums, w_bits, R, E, N, K)));
+    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, full_sums != 0, w_bits, R, E, N, tab::blocks8(K));
     const tab::ExpertsArgs a = experts_args(dev_QX, dev_SX, 0, M, dev_rows, dev_offsets, dev_QW, dev_SW, w_block_rows, R, E, N, K, dev_Y);
     const hipError_t e = w_bits == 4 ? tab::launch_experts4(out_dtype, plan, a, workspace, static_cast<hipStream_t>(stream))
                                      : tab::launch_experts8(out_dtype, full_sums != 0, x_format, plan, a, workspace, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? TAB_OK : device_fail(e, "experts launch");
 }
 
-size_t tab_experts_linear_workspace_bytes(int dtype, int M, int R, int E, int N, int K)
+size_t tab_experts_linear_workspace_bytes(int dtype, int w_bits, int M, int R, int E, int N, int K)
 {
     if (M < 1 || R < 1 || E < 1 || N < 1 || K < 1) return 0;
-    const tab::ExpertsPlan plan = tab::experts_plan(dtype, R, E, N, tab::blocks8(K));
+    const tab::ExpertsPlan plan = tab::experts_plan(dtype, true, w_bits, R, E, N, tab::blocks8(K));
     return plan.few ? 0 : packed_bytes(M, K) + parts_bytes(plan, R, N);
 }
 
 int tab_experts_linear(const void *dev_X, int dtype, long ldx, int M, const int *dev_rows, const int *dev_offsets, const void *dev_QW, const void *dev_SW, int w_bits,
                        int w_block_rows, int R, int E, int N, int K, void *dev_Y, void *workspace, size_t workspace_bytes, void *stream)
 {
-    TAB_CHECK(check_experts(M, dev_rows, dev_offsets, R, E, N, K, dtype, w_bits, w_block_rows));
+    TAB_CHECK(check_experts(M, dev_rows, dev_offsets, R, E, N, K, dtype, true, w_bits, w_block_rows));
     TAB_CHECK(check_rows(dev_X, dtype, M, K, ldx, "X"));
     TAB_CHECK(check_packed(dev_QW, dev_SW, "QW or SW"));
     if (w_bits == 4 && (uintptr_t)dev_SW % 4) return fail(TAB_ERR_BAD_ARGUMENT, "SW must be aligned to 4 bytes");
     TAB_CHECK(check_rows(dev_Y, dtype, 1, N, N, "Y"));
-    const tab::ExpertsPlan plan = tab::experts_plan(dtype, R, E, N, tab::blocks8(K));
+    const tab::ExpertsPlan plan = tab::experts_plan(dtype, true, w_bits, R, E, N, tab::blocks8(K));
     if (plan.few) {
         const tab::ExpertsArgs a = experts_args(dev_X, nullptr, ldx, M, dev_rows, dev_offsets, dev_QW, dev_SW, w_block_rows, R, E, N, K, dev_Y);
         const hipError_t e = w_bits == 4 ? tab::launch_experts4_few(dtype, plan, a, static_cast<hipStream_t>(stream)) : tab::launch_experts8_few(dtype, plan, a, static_cast<hipStream_t>(stream));
         return e == hipSuccess ? TAB_OK : device_fail(e, "experts launch");
     }
     TAB_CHECK(check_quantize(M, K, 1, false));
-    TAB_CHECK(check_workspace(workspace, workspace_bytes, tab_experts_linear_workspace_bytes(dtype, M, R, E, N, K)));
+    TAB_CHECK(check_workspace(workspace, workspace_bytes, tab_experts_linear_workspace_bytes(dtype, w_bits, M, R, E, N, K)));
     uint8_t *const q = static_cast<uint8_t *>(workspace), *const s = q + packed_numbers(M, K);
     const size_t packed = packed_bytes(M, K);
     TAB_CHECK(tab_quantize8(dev_X, dtype, M, K, ldx, 1, TAB_E4M3, q, s, nullptr, nullptr, stream));
@@ -304,10 +304,13 @@ int tab_combine_backward(const void *dev_dout, const void *dev_Y, int dtype, con
 
 /* Test hook, absent from include/tab_amd.h: how a product over experts would be computed: 0 as few rows, else (the tile's rows + columns) / 2 * 100 + the
  * parts of K. */
-int tab_internal_experts_way(int out_dtype, int R, int E, int N, int K)
+int tab_internal_experts_way(int out_dtype, int w_bits, int R, int E, int N, int K)
 {
-    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, R, E, N, tab::blocks8(K));
+    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, true, w_bits, R, E, N, tab::blocks8(K));
     return plan.few ? 0 : (plan.rows + plan.columns) / 2 * 100 + plan.parts;
 }
+
+/* The same of the gradients of the weights: the tile. */
+int tab_internal_experts_grad_way(int out_dtype, int R, int E, int N, int K) { return tab::experts_grad_way(out_dtype, R, E, N, K); }
 
 }  // extern "C"

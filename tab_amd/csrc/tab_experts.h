@@ -37,48 +37,50 @@ __device__ __forceinline__ void run_bounds(const int *offsets, int E, int rows, 
     a = e <= E ? min(max(offsets[e], 0), rows) : rows;
     b = e < E ? min(max(offsets[e + 1], a), rows) : rows;
 }
-template <int TILE> __device__ __forceinline__ int run_tiles(int a, int b) { return (int)(((uint32_t)(b - a) + (uint32_t)(TILE - 1)) / (uint32_t)TILE); }
+// Tiles of 2^log_tile rows
+__device__ __forceinline__ int run_tiles(int a, int b, int log_tile) { return (int)(((uint32_t)(b - a) + (1u << log_tile) - 1u) >> log_tile); }
+constexpr int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
 
 // Tiles of all runs, with or without those behind the last expert.  By whole waves.
-template <int TILE> __device__ __forceinline__ uint32_t count_runs(const int *offsets, int E, int rows, bool behind, int lane)
+__device__ __forceinline__ uint32_t count_runs(const int *offsets, int E, int rows, bool behind, int log_tile, int lane)
 {
     uint32_t all = 0;
     const int last = behind ? E : E - 1;
     for (int base = 0; base <= last; base += 64) {
         int a, b;
         run_bounds(offsets, E, rows, base + lane, a, b);
-        all += (uint32_t)__builtin_amdgcn_readlane(wave_scan(base + lane <= last ? run_tiles<TILE>(a, b) : 0), 63);
+        all += (uint32_t)__builtin_amdgcn_readlane(wave_scan(base + lane <= last ? run_tiles(a, b, log_tile) : 0), 63);
     }
     return all;
 }
 
 // Tile `id`: its expert, its first row and the end of the expert's rows.  By whole waves.
-template <int TILE> __device__ __forceinline__ Run find_run(const int *offsets, int E, int rows, uint32_t id, int lane)
+__device__ __forceinline__ Run find_run(const int *offsets, int E, int rows, uint32_t id, int log_tile, int lane)
 {
     uint32_t before = 0;
     for (int base = 0; base <= E; base += 64) {
         int a, b;
         run_bounds(offsets, E, rows, base + lane, a, b);
-        const int mine = run_tiles<TILE>(a, b), sum = wave_scan(mine);
+        const int mine = run_tiles(a, b, log_tile), sum = wave_scan(mine);
         const uint64_t past = __ballot(before + (uint32_t)sum > id);
         if (past) {
             const int l = __builtin_ctzll(past);
             const uint32_t first = before + (uint32_t)(__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
-            return {base + l, __builtin_amdgcn_readlane(a, l) + (int)((id - first) * (uint32_t)TILE), __builtin_amdgcn_readlane(b, l)};
+            return {base + l, __builtin_amdgcn_readlane(a, l) + (int)((id - first) << log_tile), __builtin_amdgcn_readlane(b, l)};
         }
         before += (uint32_t)__builtin_amdgcn_readlane(sum, 63);
     }
     return {-1, 0, 0};
 }
 
-// Expert e's blocks of TILE rows, where every expert's rows begin at a new one: first and end.  By whole waves.
-template <int TILE> __device__ __forceinline__ Run run_of(const int *offsets, int E, int rows, int expert, int lane)
+// Expert e's blocks of 2^log_tile rows, where every expert's rows begin at a new one: first and end.  By whole waves.
+__device__ __forceinline__ Run run_of(const int *offsets, int E, int rows, int expert, int log_tile, int lane)
 {
     int before = 0;
     for (int base = 0;; base += 64) {
         int a, b;
         run_bounds(offsets, E, rows, base + lane, a, b);
-        const int mine = run_tiles<TILE>(a, b), sum = wave_scan(mine);
+        const int mine = run_tiles(a, b, log_tile), sum = wave_scan(mine);
         if (expert < base + 64) {
             const int end = before + __builtin_amdgcn_readlane(sum, expert - base);
             return {expert, end - __builtin_amdgcn_readlane(mine, expert - base), end};
@@ -99,14 +101,14 @@ struct ExpertsArgs {
     int w_block_rows;               // 8 bits: rows of QW under one scale, 1 or 128
     long ldx;                       // elements between rows of x that are not packed
 };
-// How a call is computed: few rows of X quantized and multiplied in one launch, or tiles of a packed X, K in parts
+// How a call is computed: few rows to an expert quantized and multiplied in one launch, or tiles of a packed X, K in parts
 struct ExpertsPlan {
     bool few;
-    int most;                       // rows of X that a workgroup of that launch holds at once
-    int rows, columns, parts, kb_per_part;
+    int rows, columns;              // of a tile; few: rows of X in a workgroup's LDS (a power of two) and of the weight that it takes
+    int parts, kb_per_part;         // few: waves that share 16 rows of the weight, and 0
     long workgroups;
 };
-ExpertsPlan experts_plan(int out_dtype, int R, int E, int N, int KB);
+ExpertsPlan experts_plan(int out_dtype, bool full_sums, int bits, int R, int E, int N, int KB);
 // full_sums: of an fp32 Y, as of one from fp32 activations; else those towards 16 bits
 hipError_t launch_experts8(int out_dtype, bool full_sums, int x_format, const ExpertsPlan &plan, const ExpertsArgs &a, void *workspace, hipStream_t stream);
 hipError_t launch_experts4(int out_dtype, const ExpertsPlan &plan, const ExpertsArgs &a, void *workspace, hipStream_t stream);
@@ -121,6 +123,7 @@ struct ExpertsGradArgs {
     int R, E, M, N, KB;
 };
 long experts_grad_workgroups(int out_dtype, int R, int E, int M, int N);
+int experts_grad_way(int out_dtype, int R, int E, int M, int N);  // (the tile's rows + columns) / 2
 hipError_t launch_experts_grad(int out_dtype, int d_format, const ExpertsGradArgs &a, hipStream_t stream);
 
 struct RouteArgs {

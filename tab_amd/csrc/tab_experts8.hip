@@ -3,31 +3,43 @@
 
 namespace tab {
 
-// Few rows to an expert: the launch whose workgroups hold an expert's rows in LDS and stream its weight; `columns` is then the groups of 16 rows of a weight
-// that a workgroup takes, `parts` the workgroups to an expert.
-ExpertsPlan experts_plan(int out, int R, int E, int N, int KB)
+namespace {
+
+// The experts that R rows come to, where each takes any
+double chosen_experts(int R, int E) { return E > 1 ? E * (1 - __builtin_pow(1 - 1.0 / E, R)) : 1; }
+
+}  // namespace
+
+// The least of what the ways take, us: few rows to an expert in one launch (waves stream KB of the weights, workgroups take turns on the CUs), or the launches of
+// the quantizer and of tiles (as plan8 has them, by the tiles that the chosen experts come to).  Constants fitted to every way of 460 products of 1 .. 20000
+// rows over 1 .. 137 experts of 64 .. 5000 columns and K, 8 and 4 bits, on an MI355X; what the rule picks takes 3 % longer than the best of them in the
+// mean, 1.65 times at most (15 rows of 31 experts of 2048 x 3456).
+ExpertsPlan experts_plan(int out, bool full_sums, int bits, int R, int E, int N, int KB)
 {
+    const bool exact = out == 0 && full_sums;
+    const double chosen = chosen_experts(R, E), weight_mb = chosen * N * (double)KB * (kBlock8 * bits / 8 * 1e-6);
     ExpertsPlan plan = {};
-    const int active = E < R ? E : R;
-    if ((long)R <= 8L * active && rows_fit(1, KB)) {
-        int most = R < 16 ? R : 16;
-        while (!rows_fit(most, KB)) most--;
-        const int groups = (N + 15) / 16;
-        const long experts = E + 1L < R ? E + 1L : R;
-        const long each = (groups * experts + 1023) / 1024;
-        plan = {true, most, 0, (int)each, (int)((groups + each - 1) / each), 0, 0};
-        plan.workgroups = experts * plan.parts;
-        return plan;
-    }
-    // as plan8, by the tiles that `active` experts of like numbers of rows come to
-    constexpr TileTimes kFast[] = {{64, 64, 3, 0.05, 0.174, 0.8}, {64, 128, 2, 0.171, 0.242, 1.37}, {128, 128, 2, 0.571, 0.473, 1.69}, {256, 256, 1, 1.235, 1.125, 6.25}};
-    constexpr TileTimes kExact[] = {{64, 64, 3, 0.371, 0.242, 0.7}, {64, 128, 2, 0.553, 0.336, 1.32}, {128, 128, 2, 1.22, 0.716, 1.65}};
-    const double join = out == 0 ? 2.5 : 1.9, join_part = out == 0 ? 0.936e-6 : 0.747e-6, join_out = out == 0 ? 0.008e-6 : 0;
     double least = 1e30;
-    for (int i = 0; i < (out == 0 ? 3 : 4); i++) {
-        const TileTimes &tile = out == 0 ? kExact[i] : kFast[i];
+    if ((long)R <= 40L * (E < R ? E : R) && rows_fit(1, KB)) {
+        int most = 16;
+        while (!rows_fit(most, KB)) most /= 2;
+        const double crowd = (double)R / E - 2.6, runs = chosen * (crowd > 0 ? 1 + crowd / most : 1);
+        for (int split = 1; split <= kRowsWaves && split <= KB; split *= 2) {
+            const long groups = (N + 15) / 16;
+            const double wave_kb = 16e-3 * KB * kBlock8 * bits / 8 / split, workgroups = runs * (double)((groups * split + kRowsWaves - 1) / kRowsWaves);
+            const double all = wave_kb / 4.46 + workgroups / 256 * (1.44 + wave_kb / 4.09), t = 4.24 + (weight_mb / 5.94 > all ? weight_mb / 5.94 : all);
+            if (t < least) {
+                least = t;
+                const int columns = kRowsWaves / split * 16;
+                plan = {true, most, columns, split, 0, run_tiles_most(R, E, most) * ((N + columns - 1L) / columns)};
+            }
+        }
+    }
+    const double join = out == 0 ? 2.5 : 1.9, join_part = out == 0 ? 0.936e-6 : 0.747e-6, mb = weight_mb + R * (double)N * (out == 0 ? 4e-6 : 2e-6);
+    for (int i = 0; i < (exact ? 3 : 4); i++) {
+        const TileTimes &tile = exact ? kExpertExact[i] : kExpertTiles[i];
         const long columns = ((long)N + tile.columns - 1) / tile.columns, most = run_tiles_most(R, E, tile.rows) * columns;
-        const double rows = R <= (long)active * tile.rows / 2 ? active : (double)R / tile.rows + 0.5 * active;
+        const double spread = (double)R / tile.rows + 0.79 * chosen, rows = spread > chosen ? spread : chosen;
         for (int parts = 1; parts <= 16 && parts <= KB; parts *= 2) {
             if (parts > 1 && rows * (double)columns * parts > 2048) break;
             const int steps = (KB + parts - 1) / parts;
@@ -35,10 +47,11 @@ ExpertsPlan experts_plan(int out, int R, int E, int N, int KB)
             const double each = __builtin_ceil(rows * (double)columns * parts / 256), rounds = __builtin_ceil(each / tile.held);
             const double alone = tile.alone * rounds, among = tile.among * each;
             double t = steps * (alone > among ? alone : among) + tile.out * each * (parts > 1 || out == 0 ? 2 : 1);
-            if (parts > 1) t += join + (parts * join_part + join_out) * (double)R * (double)N;
+            if (parts > 1) t += join + parts * join_part * (double)R * (double)N;
+            t = 7 + (t > mb / 5.73 ? t : mb / 5.73);
             if (t < least) {
                 least = t;
-                plan = {false, 0, tile.rows, tile.columns, parts, steps, most * parts};
+                plan = {false, tile.rows, tile.columns, parts, steps, most * parts};
             }
         }
     }

@@ -32,6 +32,7 @@ struct TileParams {
     int M, N, KB, w_scale_rows;  // w_scale_rows: scales of QW per block of K, N or ceil(N / 128)
     int kb_per_part;             // blocks of K of a part; with more than one part y is [parts][M][N] fp32
     int tiles_m, tiles_n;
+    int streamed;                // y is written past the caches (see streamed())
 };
 
 // A launch over the experts of a layer.  Rows (kRowsByExpert): row r of Y belongs to the expert e with offsets[e] <= r < offsets[e + 1], is multiplied by
@@ -190,18 +191,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     const uint32_t most = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n, part = blockIdx.x / most, b = blockIdx.x - part * most;
     uint32_t all_m = (uint32_t)p.tiles_m;
     if constexpr (BY == kRowsByExpert) {
-        all_m = count_runs<BM>(p.offsets, p.E, p.M, true, lane);
+        all_m = count_runs(p.offsets, p.E, p.M, true, log2_of(BM), lane);
         if (b >= all_m * (uint32_t)p.tiles_n) return;
     }
-    uint32_t tiles = all_m * (uint32_t)p.tiles_n;
-    if constexpr (BY == kKByExpert) tiles *= (uint32_t)p.E;
-    const uint32_t share = tiles / 8;
-    uint32_t id = BY == kKByExpert ? blockIdx.x : b;
-    if (id < share * 8) id = (id & 7) * share + (id >> 3);
-    uint32_t expert = 0;
+    const uint32_t tiles = all_m * (uint32_t)p.tiles_n;
+    uint32_t share = tiles / 8, id = b, expert = 0;
     if constexpr (BY == kKByExpert) {
-        expert = id / most;
-        id -= expert * most;
+        // every XCD takes an eighth of each expert's tiles (the experts' runs of blocks differ, and with them their tiles' times), rounded up
+        share = (most + 7) / 8;
+        expert = blockIdx.x / (share * 8);
+        id = blockIdx.x - expert * (share * 8);
+        id = (id & 7) * share + (id >> 3);
+        if (id >= most) return;
+    } else if (id < share * 8) {
+        id = (id & 7) * share + (id >> 3);
     }
     const uint32_t in_group = 8 * (uint32_t)p.tiles_n, group = id / in_group, rest = id - group * in_group;
     const uint32_t rows = min(8u, all_m - group * 8), tile_n = rest / rows, tile_m = group * 8 + rest - tile_n * rows;
@@ -209,14 +212,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     const int n0 = (int)tile_n * BN;
     int kb0 = (int)part * p.kb_per_part, kb1 = min(p.KB, kb0 + p.kb_per_part);
     if constexpr (BY == kRowsByExpert) {
-        const Run run = find_run<BM>(p.offsets, p.E, p.M, tile_m, lane);
+        const Run run = find_run(p.offsets, p.E, p.M, tile_m, log2_of(BM), lane);
         expert = (uint32_t)run.expert, m0 = run.first, end_m = run.end;
         if (run.expert == p.E) expert = 0, kb1 = kb0;  // rows of no expert: zeros
     }
     if constexpr (BY == kKByExpert) {
-        const Run run = run_of<kBlock8>(p.offsets, p.E, p.x_rows, (int)expert, lane);
+        const Run run = run_of(p.offsets, p.E, p.x_rows, (int)expert, log2_of(kRunBlock), lane);
         kb0 = min(run.first, p.KB), kb1 = min(run.end, p.KB);
     }
+
+    // Every expert begins at another block of K: rows of 4096 numbers are as many bytes apart, so that all tiles at the same block would ask the same few
+    // channels of the memory (32 experts of 2048 x 4096, 512 rows each: 149 us, now TURNED)
+    const int turn = BY == kRowsByExpert && p.kb_per_part == p.KB ? (int)expert % p.KB : 0;
 
     const int wave = __builtin_amdgcn_readfirstlane(t / 64), wm = wave / WN, wn = wave % WN, l16 = lane % 16, quarter = lane / 16;
     const int row_bytes = p.KB * kBlock8, w_row_bytes = p.KB * kWBlock, rows_x = min(BM, end_m - m0), rows_w = min(BN, p.N - n0);
@@ -226,8 +233,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     // load i of a wave is eight rows of an operand's tile, eight lanes a row: of W the waves take turns, of X those that multiply the rows
     const int first_x = wm * (BM / WM) + wn * 8, first_w = wave * W_ROWS;
     const uint32_t x_at = (uint32_t)(first_x + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
-    const uint32_t w_at = (uint32_t)(first_w + lane / W_LANES) * (uint32_t)w_row_bytes +
-                          (uint32_t)(WBITS == 4 ? (lane % 4) ^ (lane / 16) : (lane % 8) ^ (lane / 8)) * 16;
+    uint32_t w_at = (uint32_t)(first_w + lane / W_LANES) * (uint32_t)w_row_bytes + (uint32_t)(turn * kWBlock) +
+                    (uint32_t)(WBITS == 4 ? (lane % 4) ^ (lane / 16) : (lane % 8) ^ (lane / 8)) * 16;
     // row `row` of the tile in the buffer of all of X, in units of `unit` bytes
     auto gathered = [&](int row, int unit) {
         if constexpr (GATHER) {
@@ -240,19 +247,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     uint32_t x_from[GATHER ? A_LOADS : 1];
     if constexpr (GATHER) {
 #pragma unroll
-        for (int i = 0; i < A_LOADS; i++) x_from[i] = gathered(first_x + i * 8 * WN + lane / 8, row_bytes) + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
+        for (int i = 0; i < A_LOADS; i++) x_from[i] = gathered(first_x + i * 8 * WN + lane / 8, row_bytes) + (uint32_t)(turn * kBlock8) + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
     }
     // A lane loads one scale: place t of X's, then of W's (of eight waves the first four load one of each).  The scales of a lane's groups of 16 rows are
     // side by side.  (A wave's scales are all of X or all of W.)
     const bool row_scales = p.w_scale_rows == p.N;
+    const int first = kb0 + turn;
     struct Scales { const uint8_t *at; int step, rows; uint32_t offset; };
     auto scales_of = [&](bool x, int place, bool any) {
         const int groups = x ? TM : TN, row = place / (16 * groups) * (16 * groups) + place % groups * 16 + place / groups % 16;
         if constexpr (GATHER)
-            if (x) return Scales{p.sx + (long)kb0 * p.x_rows, p.x_rows, !any ? 0 : p.x_rows, gathered(row, 1)};
-        if (WBITS == 4 && !x) return Scales{sw + ((long)kb0 * p.N + n0) * 4, p.N * 4, any ? rows_w * 4 : 0, (uint32_t)row * 4};
+            if (x) return Scales{p.sx + (long)first * p.x_rows, p.x_rows, !any ? 0 : p.x_rows, gathered(row, 1)};
+        if (WBITS == 4 && !x) return Scales{sw + ((long)first * p.N + n0) * 4, p.N * 4, any ? rows_w * 4 : 0, (uint32_t)row * 4};
         const int step = x ? p.M : p.w_scale_rows;
-        return Scales{(x ? p.sx + m0 : sw + (row_scales ? n0 : n0 / kBlock8)) + (long)kb0 * step, step,
+        return Scales{(x ? p.sx + m0 : sw + (row_scales ? n0 : n0 / kBlock8)) + (long)first * step, step,
                       !any ? 0 : x ? rows_x : row_scales ? rows_w : (n0 + rows_w - 1) / kBlock8 - n0 / kBlock8 + 1,
                       (uint32_t)(x || row_scales ? row : (n0 + row) / kBlock8 - n0 / kBlock8)};
     };
@@ -268,6 +276,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     auto load = [&](int stage, int kb, int i) {
         const bool live = kb < kb1;
         const uint32_t to = lds_at + (uint32_t)stage;
+        if (BY == kRowsByExpert && (i == 0 || i == A_LOADS || i >= LOADS) && kb == p.KB - turn) {  // back to the first block
+            if (i == 0) {
+#pragma unroll
+                for (uint32_t &from : x_from) from -= (uint32_t)row_bytes;
+            }
+            if (i == A_LOADS) w_at -= (uint32_t)w_row_bytes;
+            if (i >= LOADS) {
+                Scales &of = i == LOADS ? scales : more_scales;
+                of.at -= (long)p.KB * of.step;
+            }
+        }
         if (i < A_LOADS) {
             to_lds16(sized(x_rows, live), to + (uint32_t)(first_x + i * 8 * WN) * kBlock8,
                      GATHER ? x_from[GATHER ? i : 0] + (uint32_t)(kb * kBlock8) : x_at + (uint32_t)(i * 8 * WN * row_bytes + kb * kBlock8));
@@ -302,7 +321,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     auto w_fragment = [&](const uint8_t *from, int group) {
         if constexpr (WBITS == 8) return fragment(from, group);
         const i32x4 all = *reinterpret_cast<const i32x4 *>(from + group * 16 * kWBlock + at4);
-        return (i32x8)__builtin_shufflevector(all, all, 0, 1, 2, 3, 0, 1, 2, 3);  // (four words of it are read)
+        return (i32x8)__builtin_shufflevector(all, all, 0, 1, 2, 3, -1, -1, -1, -1);  // (four words are read)
     };
     struct Operands {  // a wave's part of a step
         i32x8 wq[TN], xq[TM];
@@ -374,6 +393,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
         // waves load W and the scales of step s + 2 (which slot 2s + 4 reads), and 2s + 3, in which the others load their rows of X (for slot 2s + 5).
         // Few loads go out between the products: a wave that waits to get one out does not multiply.
         static_assert(STAGES == 2, "two steps in LDS");
+        // (An expert's last tile is rarely full: with at most half the rows the second four waves have nothing to multiply.  Leaving groups of 16 rows out one by
+        // one instead cost full tiles 3-5 %.)
+        constexpr bool HALF = BY == kRowsByExpert;
         Operands o;
         if (wm == 0) {
 #pragma unroll
@@ -412,7 +434,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
                 all_read();
                 barrier();
                 __builtin_amdgcn_s_setprio(1);
-                multiply(o, 0, [](int) {});
+                if (!HALF || rows_x > BM / 2) multiply(o, 0, [](int) {});
                 __builtin_amdgcn_s_setprio(0);
                 wait_loads<0>();
                 barrier();
@@ -501,7 +523,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
             const int m = m0 + (wm * TM + i) * 16 + row, n = n0 + wn * TN * 16 + column;
             if (m >= end_m) continue;
             T *const to = y + (long)m * p.N + n;
-            if (n + V <= p.N) {
+            if (p.streamed) {  // (rows are whole cache lines)
+                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                if (n < p.N) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4 *>(to));
+            } else if (n + V <= p.N) {
                 *reinterpret_cast<Piece *>(to) = v;
             } else {
 #pragma unroll
@@ -547,13 +572,6 @@ struct RowsParams {
     long ldx;
     Div32 div_kb;
 };
-// Rows by expert: `each` workgroups to an expert, which go through its rows of X by `most`
-struct ExpertRowsParams : RowsParams {
-    const int *offsets, *rows;
-    int E, x_rows, each, most;
-};
-template <int BY> struct RowsParamsOf { using type = ExpertRowsParams; };
-template <> struct RowsParamsOf<kOneWeight> { using type = RowsParams; };
 
 // The bound between one launch and quantizer, tiles and join: X in 72 KB of LDS, which up to 16 rows (with 8 KB for the waves' sums) leaves room for two workgroups
 // a CU; with 17 to 32 rows the sums take 16 KB, and a CU holds one.  On both sides of it (bf16, by 4096 columns, a pass among others, us):
@@ -567,8 +585,26 @@ constexpr int kRowsWaves = 8;
 __host__ __device__ __forceinline__ int rows_stride(int KB) { return KB * kBlock8 + 16; }
 __host__ __device__ __forceinline__ int rows_lds(int M, int KB) { return M * (rows_stride(KB) + KB * 4); }  // numbers, then scales as words [KB][M]
 
-template <int INPUT, int FORMAT, int OUT, int MT, int WBITS = 8, int BY = kOneWeight>
-__global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const typename RowsParamsOf<BY>::type p)
+// A lane's part of a block of W
+template <int WBITS> __device__ __forceinline__ i32x8 w_numbers(i32x4 low, i32x4 high)
+{
+    if constexpr (WBITS == 8) return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+    else return __builtin_shufflevector(low, low, 0, 1, 2, 3, -1, -1, -1, -1);
+}
+
+// 16 rows of W by 16 rows of X in LDS, one block of K: x is the lane's row's block.  (Which numbers a lane takes: as in the tiles.)
+template <int FORMAT, int OUT, int WBITS> __device__ __forceinline__ f32x4 times_rows(i32x8 w, uint32_t w_scale, const uint8_t *x, uint32_t x_scale, int quarter, f32x4 c)
+{
+    constexpr bool PAIRS = OUT == 0 && WBITS == 4;
+    x += quarter * (PAIRS ? 32 : 16);
+    const i32x4 low = *reinterpret_cast<const i32x4 *>(x), high = *reinterpret_cast<const i32x4 *>(x + (PAIRS ? 16 : 64));
+    const i32x8 xf = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+    if constexpr (OUT == 0) return mfma16_exact(WBITS == 4 ? exact32_of4(w, w_scale) : exact32<0>(w, w_scale), exact32<FORMAT>(xf, x_scale), c);
+    else return mfma16<FORMAT, WBITS>(w, xf, c, w_scale, x_scale);
+}
+
+template <int INPUT, int FORMAT, int OUT, int MT, int WBITS = 8>
+__global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams p)
 {
     using T = typename Element<OUT>::type;
     constexpr int WAVES = kRowsWaves, AHEAD = 4, kWBlock = kBlock8 * WBITS / 8;
@@ -576,134 +612,90 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const typename R
     __shared__ __attribute__((aligned(16))) float sums[WAVES * MT * 256];
     const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64), l16 = lane % 16, quarter = lane / 16;
     const int stride = rows_stride(p.KB);
+    uint32_t *const scales = reinterpret_cast<uint32_t *>(packed + p.M * stride);
     const bool w_rows = p.w_scale_rows == p.N;
-    const int groups = (p.N + 15) / 16;
-    int first_row = 0, end_row = p.M, most = p.M, share = (int)blockIdx.x;
-    const uint8_t *qw = p.qw, *sw = p.sw;
-    if constexpr (BY == kRowsByExpert) {
-        const int place = share / p.each;
-        share -= place * p.each;
-        const Run run = find_run<1 << 30>(p.offsets, p.E, p.M, (uint32_t)place, lane);
-        if (run.expert < 0) return;
-        first_row = run.first, end_row = run.end, most = p.most;
-        if (run.expert == p.E) {  // rows of no expert: zeros
-            const int n0 = share * p.groups_each * 16, columns = min(p.groups_each * 16, p.N - n0);
-            for (int m = first_row; m < end_row; m++)
-                for (int n = t; n < columns; n += 64 * WAVES) static_cast<T *>(p.y)[(long)m * p.N + n0 + n] = (T)0.f;
-            return;
-        }
-        qw += (long)run.expert * p.N * p.KB * kWBlock;
-        sw += (long)run.expert * p.KB * p.w_scale_rows * (WBITS == 4 ? 4 : 1);
-    }
     // block u of the AHEAD that a wave takes from `first` on: every eighth one, or (of 4 bits) every eighth pair, which is a cache line
     auto block_of = [](int first, int u) { return WBITS == 4 ? first + u / 2 * (2 * WAVES) + u % 2 : first + u * WAVES; };
     const int wave_first = WBITS == 4 ? 2 * wave : wave;
-    i32x4 w_low[AHEAD], w_high[AHEAD];
+    i32x4 w_low[AHEAD], w_high[WBITS == 8 ? AHEAD : 1];
     uint32_t w_scale[AHEAD];
     auto load = [&](int n0, int first) {
         const int row = min(n0 + l16, p.N - 1);
-        const uint8_t *const w = qw + (long)row * p.KB * kWBlock + quarter * 16, *const s = WBITS == 4 ? sw + row * 4 + quarter : sw + (w_rows ? row : row / kBlock8);
+        const uint8_t *const w = p.qw + (long)row * p.KB * kWBlock + quarter * 16, *const s = WBITS == 4 ? p.sw + row * 4 + quarter : p.sw + (w_rows ? row : row / kBlock8);
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             const long kb = min(block_of(first, u), p.KB - 1);
             w_low[u] = *reinterpret_cast<const i32x4 *>(w + kb * kWBlock);
             if constexpr (WBITS == 8) w_high[u] = *reinterpret_cast<const i32x4 *>(w + kb * kWBlock + 64);
-            else w_high[u] = w_low[u];  // (not read)
             w_scale[u] = s[kb * p.w_scale_rows * (WBITS == 4 ? 4 : 1)];
         }
     };
-    const int group0 = share * p.groups_each, group1 = min(groups, group0 + p.groups_each);
-    do {
-        const int rows = BY == kRowsByExpert ? min(most, end_row - first_row) : p.M;
-        uint32_t *const scales = reinterpret_cast<uint32_t *>(packed + rows * stride);
-        load(group0 * 16, wave_first);
+    const int groups = (p.N + 15) / 16, group0 = (int)blockIdx.x * p.groups_each, group1 = min(groups, group0 + p.groups_each);
+    load(group0 * 16, wave_first);
 
-        // X into LDS: blocks in the order of memory, 16 lanes a block, AT_ONCE of them on their way
-        constexpr int AT_ONCE = 8, STEP = 64 * WAVES / 16;
-        const int blocks = rows * p.KB;
-        for (int first = t / 16; first < blocks; first += AT_ONCE * STEP) {
-            using X = typename Element<INPUT == 3 ? 0 : INPUT>::type;
-            Words<X> v[AT_ONCE];
+    // X into LDS: blocks in the order of memory, 16 lanes a block, AT_ONCE of them on their way
+    constexpr int AT_ONCE = 8, STEP = 64 * WAVES / 16;
+    const int blocks = p.M * p.KB;
+    for (int first = t / 16; first < blocks; first += AT_ONCE * STEP) {
+        using X = typename Element<INPUT == 3 ? 0 : INPUT>::type;
+        Words<X> v[AT_ONCE];
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; u++) {
-                const int block = first + u * STEP, m = (int)div32(block, p.div_kb), kb = block - m * p.KB;
-                if (block >= blocks) break;
-                if constexpr (BY == kRowsByExpert) {
-                    const int at = first_row + m, from = p.rows ? p.rows[at] : at;
-                    const bool there = from >= 0 && from < p.x_rows;
-                    if constexpr (INPUT == 3) {
-                        v[u] = {};
-                        if (there) {
-                            const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p.x) + ((long)from * p.KB + kb) * kBlock8 + l16 * 8);
-                            v[u].w[0] = w.x, v[u].w[1] = w.y, v[u].w[2] = p.sx[(long)kb * p.x_rows + from];
-                        }
-                    } else {
-                        v[u] = load_words(static_cast<const X *>(p.x) + from * p.ldx, kb * kBlock8 + l16 * 8, there ? p.K : 0);
-                    }
-                } else if constexpr (INPUT == 3) {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p.x) + (long)block * kBlock8 + l16 * 8);
-                    v[u].w[0] = w.x, v[u].w[1] = w.y, v[u].w[2] = p.sx[(long)kb * p.M + m];
-                } else {
-                    v[u] = load_words(static_cast<const X *>(p.x) + m * p.ldx, kb * kBlock8 + l16 * 8, p.K);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; u++) {
-                const int block = first + u * STEP, m = (int)div32(block, p.div_kb), kb = block - m * p.KB;
-                if (block >= blocks) break;
-                uint32_t byte;
-                uint2 w;
-                if constexpr (INPUT == 3) w = {v[u].w[0], v[u].w[1]}, byte = v[u].w[2];
-                else w = pack_run<X, FORMAT>(v[u], byte);
-                *reinterpret_cast<uint2 *>(packed + m * stride + kb * kBlock8 + l16 * 8) = w;
-                if (l16 == 0) scales[kb * rows + m] = byte;
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int block = first + u * STEP, m = (int)div32(block, p.div_kb), kb = block - m * p.KB;
+            if (block >= blocks) break;
+            if constexpr (INPUT == 3) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p.x) + (long)block * kBlock8 + l16 * 8);
+                v[u].w[0] = w.x, v[u].w[1] = w.y, v[u].w[2] = p.sx[(long)kb * p.M + m];
+            } else {
+                v[u] = load_words(static_cast<const X *>(p.x) + m * p.ldx, kb * kBlock8 + l16 * 8, p.K);
             }
         }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int block = first + u * STEP, m = (int)div32(block, p.div_kb), kb = block - m * p.KB;
+            if (block >= blocks) break;
+            uint32_t byte;
+            uint2 w;
+            if constexpr (INPUT == 3) w = {v[u].w[0], v[u].w[1]}, byte = v[u].w[2];
+            else w = pack_run<X, FORMAT>(v[u], byte);
+            *reinterpret_cast<uint2 *>(packed + m * stride + kb * kBlock8 + l16 * 8) = w;
+            if (l16 == 0) scales[kb * p.M + m] = byte;
+        }
+    }
+    __syncthreads();
+
+    for (int group = group0; group < group1; group++) {
+        const int n0 = group * 16;
+        f32x4 acc[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int first = wave_first; first < p.KB; first += AHEAD * WAVES) {
+            if (first != wave_first) load(n0, first);
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                const int kb = block_of(first, u);
+                if (kb >= p.KB) break;  // (the same for the whole wave)
+                const i32x8 wf = w_numbers<WBITS>(w_low[u], w_high[WBITS == 8 ? u : 0]);
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    const int m = min(i * 16 + l16, p.M - 1);  // (columns past M repeat the last one and are not stored)
+                    acc[i] = times_rows<FORMAT, OUT, WBITS>(wf, w_scale[u], packed + m * stride + kb * kBlock8, scales[kb * p.M + m], quarter, acc[i]);
+                }
+            }
+        }
+        if (group + 1 < group1) load(n0 + 16, wave_first);  // the next group's first blocks, on their way while the sums meet
+#pragma unroll
+        for (int i = 0; i < MT; i++) *reinterpret_cast<f32x4 *>(sums + (wave * MT + i) * 256 + l16 * 16 + quarter * 4) = acc[i];
         __syncthreads();
-
-        for (int group = group0; group < group1; group++) {
-            const int n0 = group * 16;
-            f32x4 acc[MT];
+        for (int i = t; i < MT * 256; i += 64 * WAVES) {
+            const int m = i / 16, n = n0 + i % 16;
+            float sum = sums[i];
 #pragma unroll
-            for (int i = 0; i < MT; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (int first = wave_first; first < p.KB; first += AHEAD * WAVES) {
-                if (first != wave_first) load(n0, first);
-#pragma unroll
-                for (int u = 0; u < AHEAD; u++) {
-                    const int kb = block_of(first, u);
-                    if (kb >= p.KB) break;  // (the same for the whole wave)
-                    const i32x8 wf = __builtin_shufflevector(w_low[u], w_high[u], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        constexpr bool PAIRS = OUT == 0 && WBITS == 4;  // (which numbers a lane takes: as in the tiles)
-                        const int m = min(i * 16 + l16, rows - 1);  // (columns past the last row repeat it and are not stored)
-                        const uint8_t *const x = packed + m * stride + kb * kBlock8 + quarter * (PAIRS ? 32 : 16);
-                        const i32x4 low = *reinterpret_cast<const i32x4 *>(x), high = *reinterpret_cast<const i32x4 *>(x + (PAIRS ? 16 : 64));
-                        const i32x8 xf = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
-                        const uint32_t x_scale = scales[kb * rows + m];
-                        if constexpr (OUT == 0) acc[i] = mfma16_exact(WBITS == 4 ? exact32_of4(wf, w_scale[u]) : exact32<0>(wf, w_scale[u]), exact32<FORMAT>(xf, x_scale), acc[i]);
-                        else acc[i] = mfma16<FORMAT, WBITS>(wf, xf, acc[i], w_scale[u], x_scale);
-                    }
-                }
-            }
-            if (group + 1 < group1) load(n0 + 16, wave_first);  // the next group's first blocks, on their way while the sums meet
-#pragma unroll
-            for (int i = 0; i < MT; i++) *reinterpret_cast<f32x4 *>(sums + (wave * MT + i) * 256 + l16 * 16 + quarter * 4) = acc[i];
-            __syncthreads();
-            for (int i = t; i < MT * 256; i += 64 * WAVES) {
-                const int m = i / 16, n = n0 + i % 16;
-                float sum = sums[i];
-#pragma unroll
-                for (int k = 1; k < WAVES; k++) sum += sums[k * MT * 256 + i];
-                if (m < rows && n < p.N) static_cast<T *>(p.y)[(long)(first_row + m) * p.N + n] = (T)sum;
-            }
-            if (group + 1 < group1) __syncthreads();
+            for (int k = 1; k < WAVES; k++) sum += sums[k * MT * 256 + i];
+            if (m < p.M && n < p.N) static_cast<T *>(p.y)[(long)m * p.N + n] = (T)sum;
         }
-        if constexpr (BY == kRowsByExpert) {
-            first_row += rows;
-            if (first_row < end_row) __syncthreads();  // the sums are read before X is written over and the next ones come
-        }
-    } while (BY == kRowsByExpert && first_row < end_row);
+        if (group + 1 < group1) __syncthreads();
+    }
 }
 
 inline bool rows_fit(int M, int KB) { return M <= kRowsMost && KB <= kRowsLds / kBlock8 && rows_lds(M, KB) <= kRowsLds; }
@@ -731,6 +723,9 @@ struct Plan8 {
 // up by a launch of their own.  Constants fitted to every (tile, parts) of 60 products of 33 .. 16384 rows, 64 .. 8192 columns and K on an MI355X;
 // what the rule picks takes 0.6 % (16-bit output) and 0.3 % (fp32) longer than the best of them in the mean, at most 14 % (40 x 64 x 8192).
 struct TileTimes { int rows, columns, held; double alone, among, out; };
+// The same of tiles over experts (16-bit sums, and full ones); their ways out are shorter, past the caches
+constexpr TileTimes kExpertTiles[] = {{64, 64, 3, 0.092, 0.165, 0.46}, {64, 128, 2, 0.237, 0.235, 0.725}, {128, 128, 2, 0.509, 0.41, 0.923}, {256, 256, 1, 0.96, 0.945, 2.854}};
+constexpr TileTimes kExpertExact[] = {{64, 64, 3, 0.371, 0.242, 0.7}, {64, 128, 2, 0.553, 0.336, 1.32}, {128, 128, 2, 1.22, 0.716, 1.65}};
 
 inline Plan8 plan8(int out, int M, int N, int KB)
 {
@@ -757,6 +752,15 @@ inline Plan8 plan8(int out, int M, int N, int KB)
         }
     }
     return best;
+}
+
+// Whether Y (`count` elements of type `out` in rows of N) is written past the caches: from 8 MB on, where its rows are whole cache lines, which a wave then
+// writes at once.  What is smaller is read from the caches by the next kernel.  16384 x 2048 bf16, two tiles a CU: the way out 21 -> 11 us.  With the quantizer
+// that reads Y behind it, us through / past the caches: 1024 x 4096 29.6 / 31.4, 2048 x 2048 20.4 / 20.2, 4096 x 2048 43.9 / 41.7, 8192 x 8192 over 8192 429 / 399.
+inline int streamed(int out, const void *y, long count, int N)
+{
+    const long bytes = out == 0 ? 4 : 2;
+    return count * bytes >= 8l << 20 && (N * bytes) % 128 == 0 && (uintptr_t)y % 128 == 0;
 }
 
 inline int threads_of(const Plan8 &plan) { return plan.rows == 256 ? 512 : 256; }
@@ -795,7 +799,8 @@ template <int FORMAT, int WBITS> hipError_t launch_product(int out, const Linear
     }
     const Plan8 plan = plan8(out, a.M, a.N, a.KB);
     const int tiles_m = (a.M + plan.rows - 1) / plan.rows, tiles_n = (a.N + plan.columns - 1) / plan.columns;
-    const TileParams p = {a.qx, a.sx, a.qw, a.sw, plan.parts > 1 ? workspace : a.y, a.M, a.N, a.KB, scale_rows, plan.kb_per_part, tiles_m, tiles_n};
+    const TileParams p = {a.qx, a.sx, a.qw, a.sw, plan.parts > 1 ? workspace : a.y, a.M, a.N, a.KB, scale_rows, plan.kb_per_part, tiles_m, tiles_n,
+                          plan.parts == 1 && plan.rows * plan.columns > 64 * 64 && streamed(out, a.y, (long)a.M * a.N, a.N)};
     const long groups = plan.tiles * plan.parts;
     if (plan.parts == 1)
         return out == 0 ? launch_tiles<FORMAT, 0, true, WBITS>(plan, groups, p, stream)

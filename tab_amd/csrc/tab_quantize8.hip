@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
     const int k = kb * kBlock8 + tx * 8;
     TileRows rows = {(long)tile_m * 128, p.M, ((long)p.M + 127) / 128};
     if constexpr (EXPERTS) {
-        const Run run = find_run<kRunBlock>(p.offsets, p.E, p.M, tile_m, t % 64);
+        const Run run = find_run(p.offsets, p.E, p.M, tile_m, log2_of(kRunBlock), t % 64);
         if (run.expert < 0 || run.expert == p.E) return;
         rows = {run.first, run.end, p.blocks};
     }

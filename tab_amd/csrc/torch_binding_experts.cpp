@@ -168,7 +168,7 @@ Tensor TAB_ExpertsLinear(const Tensor &X, const OptionalTensor &rows, const Tens
     const int *from = int32s(rows, R, X, "rows"), *at = int32s(offsets, E + 1, X, "offsets");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(X.device());
     auto Y = device_empty({R, N}, X.scalar_type(), X);
-    const size_t bytes = tab_experts_linear_workspace_bytes(dtype, M, R, E, N, K);
+    const size_t bytes = tab_experts_linear_workspace_bytes(dtype, w.bits, M, R, E, N, K);
     with_workspace(bytes, X, [&](void *ws, hipStream_t stream) {
         check_status(tab_experts_linear(X.data_ptr(), dtype, (long)ld, M, from, at, QW.data_ptr(), SW.data_ptr(), w.bits, w.block_rows, R, E, N, K, Y.data_ptr(), ws, bytes, stream));
     });
@@ -186,7 +186,7 @@ Tensor experts_packed(const Tensor &QX, const Tensor &SX, const OptionalTensor &
     const int *from = int32s(rows, R, QX, "rows"), *at = int32s(offsets, E + 1, QX, "offsets");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(QX.device());
     auto Y = device_empty({R, N}, out_type, QX);
-    const size_t bytes = tab_experts_linear_packed_workspace_bytes(dtype, R, E, N, K);
+    const size_t bytes = tab_experts_linear_packed_workspace_bytes(dtype, full_sums, w.bits, R, E, N, K);
     with_workspace(bytes, QX, [&](void *ws, hipStream_t stream) {
         check_status(tab_experts_linear_packed(QX.data_ptr(), format, SX.data_ptr(), M, from, at, QW.data_ptr(), SW.data_ptr(), w.bits, w.block_rows, R, E, N, K, Y.data_ptr(),
                                                dtype, full_sums, ws, bytes, stream));
@@ -288,11 +288,13 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
         ctx->saved_data["normalize"] = normalize;
         ctx->saved_data["shape"] = logits.sizes().vec();
         ctx->mark_non_differentiable({out[1], out[2], out[3], out[4]});
+        ctx->set_materialize_grads(false);  // (zeros for the whole numbers would be four launches)
         return out;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads)
     {
         no_second_derivative(grads);
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0];
         const int M = (int)logits.size(0), E = (int)logits.size(1), k = (int)saved[1].size(1);

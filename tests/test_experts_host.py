@@ -13,9 +13,12 @@ from tab_amd import nn as tab_nn
 P = 4096  # an aligned address that is never dereferenced: every call below fails its checks
 
 # (0 fp32 or 1 16-bit output, rows, experts, N, K, half of the tile's rows + columns * 100 + parts of K): every tile, K whole and in parts
-WAYS = [(0, 34, 1, 44, 94, 6401), (0, 34, 3, 47, 1187, 6404), (0, 100, 11, 1774, 68, 9601), (0, 107, 12, 1363, 5321, 9602), (0, 8022, 102, 145, 74, 12801),
-        (1, 38, 1, 40, 67, 6401), (1, 38, 2, 39, 3180, 6404), (1, 44, 2, 37, 3999, 6416), (1, 42, 5, 3469, 67, 9601), (1, 35, 4, 1192, 5954, 9604),
-        (1, 969, 25, 1169, 73, 12801), (1, 10111, 19, 1132, 67, 25601)]
+WAYS = [(0, 42, 1, 44, 66, 6401), (0, 46, 1, 32, 1600, 6404), (0, 54, 1, 50, 1989, 6416), (0, 5765, 59, 66, 66, 9601), (0, 542, 46, 515, 4787, 9602),
+        (0, 846, 20, 1364, 67, 12801), (1, 44, 1, 35, 85, 6401), (1, 1796, 50, 40, 4648, 6402), (1, 49, 1, 45, 1926, 6416), (1, 64, 47, 3550, 74, 9601),
+        (1, 564, 57, 98, 5479, 9604), (1, 1230, 37, 695, 69, 12801), (1, 3961, 51, 978, 87, 25601), (1, 10826, 24, 129, 8020, 25604)]
+# (output, rows, experts, N, K, half of the tile's rows + columns) of the gradients of the weights
+GRAD_WAYS = [(1, 3000, 4, 1100, 1500, 128), (1, 2000, 2, 300, 520, 64), (1, 1059, 46, 67, 131, 96), (1, 1000, 30, 300, 90, 96), (1, 233, 41, 1171, 131, 256), (1, 2000, 41, 1171, 400, 256),
+             (0, 3000, 4, 600, 700, 64), (0, 33, 45, 33, 358, 96), (0, 900, 8, 1000, 1400, 128)]
 
 
 def _refuses(status, message, code=-1):
@@ -26,9 +29,15 @@ def _refuses(status, message, code=-1):
 @pytest.mark.parametrize("out,R,E,N,K,way", WAYS)
 def test_products_take_the_tiles_that_they_are_tested_for(out, R, E, N, K, way):
     way_of = ctypes.CDLL(_capi.LIB_PATH).tab_internal_experts_way
-    assert way_of(out, R, E, N, K) == way
-    if out == 1:
-        assert way_of(2, R, E, N, K) == way
+    for bits in (8, 4):
+        assert way_of(out, bits, R, E, N, K) == way
+        if out == 1:
+            assert way_of(2, bits, R, E, N, K) == way
+
+
+@pytest.mark.parametrize("out,R,E,N,K,way", GRAD_WAYS)
+def test_gradients_take_the_tiles_that_they_are_tested_for(out, R, E, N, K, way):
+    assert ctypes.CDLL(_capi.LIB_PATH).tab_internal_experts_grad_way(out, R, E, N, K) == way
 
 
 def test_sizes():
@@ -38,9 +47,9 @@ def test_sizes():
     for out in (0, 1, 2):
         assert lib.tab_linear4_workspace_bytes(out, 17, 1000, 4096) == 0 < lib.tab_linear4_workspace_bytes(out, 18, 1000, 4096)
         assert lib.tab_linear4_packed_workspace_bytes(out, 17, 1000, 4096) == 0
-        assert lib.tab_experts_linear_workspace_bytes(out, 16, 64, 64, 2048, 4096) == 0
-        assert lib.tab_experts_linear_workspace_bytes(out, 4096, 8192, 8, 512, 300) >= 4096 * (384 + 3)
-        assert lib.tab_experts_linear_workspace_bytes(out, 0, 1, 1, 1, 1) == lib.tab_experts_linear_packed_workspace_bytes(out, 1, -1, 1, 1) == 0
+        assert lib.tab_experts_linear_workspace_bytes(out, 8, 16, 64, 24, 1003, 776) == 0
+        assert lib.tab_experts_linear_workspace_bytes(out, 4, 4096, 8192, 8, 512, 300) >= 4096 * (384 + 3)
+        assert lib.tab_experts_linear_workspace_bytes(out, 8, 0, 1, 1, 1, 1) == lib.tab_experts_linear_packed_workspace_bytes(out, 1, 8, 1, -1, 1, 1) == 0
     assert lib.tab_route_workspace_bytes(128, 64, 4) == 0 < lib.tab_route_workspace_bytes(129, 64, 4)
     assert lib.tab_route_workspace_bytes(129, 1025, 4) == lib.tab_route_workspace_bytes(0, 1, 1) == 0
 

@@ -6,6 +6,7 @@ import experts_reference as ref
 import layers8_reference as ref8
 import tab_amd
 from tab_amd import nn as tab_nn
+from test_experts_host import GRAD_WAYS, WAYS
 
 pytestmark = pytest.mark.gpu
 
@@ -83,7 +84,7 @@ def test_rows_of_tokens(M, k, E, N, K, bits, block_rows, dtype):
 
 # output type, R, E, N, K: every tile, K whole and in parts
 @pytest.mark.parametrize("bits", [8, 4])
-@pytest.mark.parametrize("out,R,E,N,K,way", __import__("test_experts_host").WAYS)
+@pytest.mark.parametrize("out,R,E,N,K,way", WAYS)
 def test_every_tile_and_cut(out, R, E, N, K, way, bits):
     """Rows repeat after 64, experts after two: what they stand for is made on the GPU."""
     dtype = [torch.float32, torch.bfloat16][out]
@@ -229,8 +230,8 @@ def test_gradients_are_products_of_packed_operands(M, k, E, N, K, gather, format
     ref.check(dw, want, mag, R, sixteen, "dw")
 
 
-@pytest.mark.parametrize("out,R,E,N,K", [(1, 3000, 4, 1100, 1500), (1, 2000, 2, 300, 520), (1, 1000, 30, 70, 90), (0, 3000, 4, 600, 700), (1, 9000, 3, 2300, 2600), (1, 600, 20, 256, 130)])
-def test_gradients_of_weights_by_every_tile(out, R, E, N, K):
+@pytest.mark.parametrize("out,R,E,N,K,way", GRAD_WAYS)
+def test_gradients_of_weights_by_every_tile(out, R, E, N, K, way):
     dtype = [torch.float32, torch.bfloat16][out]
     g = torch.Generator("cpu").manual_seed(R)
     offsets = torch.tensor([0] + torch.sort(torch.randint(0, R + 1, (E,), generator=g)).values.tolist(), dtype=torch.int32)
