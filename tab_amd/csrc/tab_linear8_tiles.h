@@ -218,11 +218,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     }
     if constexpr (BY == kKByExpert) {
         const Run run = run_of(p.offsets, p.E, p.x_rows, (int)expert, log2_of(kRunBlock), lane);
-        kb0 = min(run.first, p.KB), kb1 = min(run.end, p.KB);
+        kb0 = (int)min((uint32_t)run.first, (uint32_t)p.KB), kb1 = max(kb0, (int)min((uint32_t)run.end, (uint32_t)p.KB));  // (whatever offsets holds)
     }
 
     // Every expert begins at another block of K: rows of 4096 numbers are as many bytes apart, so that all tiles at the same block would ask the same few
-    // channels of the memory (32 experts of 2048 x 4096, 512 rows each: 149 us, now TURNED)
+    // channels of the memory (32 experts of 2048 x 4096, 512 rows each: 149 us, now 127)
     const int turn = BY == kRowsByExpert && p.kb_per_part == p.KB ? (int)expert % p.KB : 0;
 
     const int wave = __builtin_amdgcn_readfirstlane(t / 64), wm = wave / WN, wn = wave % WN, l16 = lane % 16, quarter = lane / 16;

@@ -454,6 +454,7 @@ Tensor combine(const Tensor &y, const Tensor &any_weights, const Tensor &places,
     check_device(any_weights, y, "weights");
     const auto type = any_weights.scalar_type();
     const Tensor weights = type == torch::kBFloat16 || type == torch::kFloat16 ? any_weights.to(torch::kFloat32) : any_weights;
+    TORCH_CHECK(offsets.numel() > 1, "offsets must have E + 1 elements");
     int32s(offsets, offsets.numel(), y, "offsets");
     if (wants_gradient({&y, &weights})) return CombineFunction::apply(y, weights, places, offsets);
     return TAB_Combine(y.contiguous(), places, weights.contiguous(), as_size(places.size(0), "tokens"), as_size(places.size(1), "choices"), as_size(y.size(0), "rows of y"),

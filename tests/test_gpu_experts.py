@@ -297,3 +297,84 @@ def test_partial_and_expanded_gradients():
     y *= 2  # no view
     with torch.no_grad():
         assert torch.equal(tab_nn.experts_linear8(*both, routing) * 2, y)
+
+
+def _random_weights(E, N, K, bits, seed):
+    """Packed weights by bytes: finite numbers of any size, scales from 2^-7 to 1."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    KB = -(-K // 128)
+    if bits == 8:
+        q = torch.randint(0, 256, (E, N, KB * 128), generator=g, dtype=torch.uint8, device="cuda").bitwise_and_(0xB7).view(torch.float8_e4m3fn)
+        s = torch.randint(120, 128, (E, KB, -(-N // 128)), generator=g, dtype=torch.uint8, device="cuda")
+    else:
+        q = torch.randint(0, 256, (E, N, KB * 64), generator=g, dtype=torch.uint8, device="cuda").view(torch.float4_e2m1fn_x2)
+        s = torch.randint(120, 128, (E, KB, N, 4), generator=g, dtype=torch.uint8, device="cuda")
+    return q, s.view(torch.float8_e8m0fnu)
+
+
+@pytest.mark.parametrize("R", [70, 9000])
+@pytest.mark.parametrize("bits,E", [(8, 70), (4, 140)])
+def test_weights_past_32_bits(bits, E, R):
+    """Experts whose weights begin past 4 GiB: few rows to an expert, and tiles.  (K is a whole number of blocks: what is behind K would not be zeros.)"""
+    N, K = 7683, 8192  # N - 387 is a whole number of blocks
+    QW, SW = _random_weights(E, N, K, bits, 1)
+    assert E * N * K * bits // 8 > 1 << 32
+    x = _rand((50, K), 2).to(torch.bfloat16)
+    g = torch.Generator("cpu").manual_seed(3)
+    rows = torch.randint(0, 50, (R,), generator=g, dtype=torch.int32)
+    offsets = torch.sort(torch.randint(0, R + 1, (E + 1,), generator=g)).values.int()
+    offsets = offsets.clamp(max=R - R // 9)  # the last expert has rows
+    offsets[0], offsets[E] = 0, R
+    y = tab_amd.ExpertsLinear(x.cuda(), rows.cuda(), offsets.cuda(), QW, SW, 50, R, E, N, K)
+    a = ref8.value(*ref8.quantize(x, 1, 0), 1)
+    for e in (0, E // 2, E - 1):
+        first, end = int(offsets[e]), min(int(offsets[e + 1]), int(offsets[e]) + 40)
+        n = slice(N - 300, N)
+        if bits == 8:
+            w = ref8.unpack(QW[e, N - 387:], SW[e][:, (N - 387) // 128:], 128)[-300:]
+        else:
+            w = ref.unpack4(QW[e, n], SW[e][:, n])
+        want, mag = ref.product(a[rows[first:end].long()], w)
+        ref.check(y[first:end, n], want, mag, K, True, f"expert {e}")
+
+
+def test_outputs_past_32_bits():
+    """Rows of Y, and gradients of weights, that begin past 4 GiB (and past 2^31 elements)."""
+    R, E, N, K = 600000, 3, 4000, 64
+    x = _rand((77, K), 4).to(torch.bfloat16)
+    QW, SW, w = _pack(_rand((E, N, K), 5, K ** -0.5), 8)
+    rows = torch.arange(R, dtype=torch.int32) % 77
+    offsets = torch.tensor([0, 1000, 1001, R - 5], dtype=torch.int32)
+    y = tab_amd.ExpertsLinear(x.cuda(), rows.cuda(), offsets.cuda(), QW, SW, 77, R, E, N, K)
+    assert y.numel() > 1 << 31
+    a = ref8.value(*ref8.quantize(x, 1, 0), 1)
+    for e, first, end in ((0, 0, 200), (2, 1001, 1300), (2, R - 300, R - 5)):
+        want, mag = ref.product(a[rows[first:end].long()], w[e])
+        ref.check(y[first:end], want, mag, K, True, f"rows {first}")
+    assert not y[R - 5:].any()
+    # back to the tokens: k = 2
+    places = torch.arange(R, dtype=torch.int32).view(-1, 2)
+    out = tab_amd.Combine(y, places.cuda(), None, R // 2, 2, R, N)
+    last = y[R - 40:].double().cpu()
+    ref.check(out[R // 2 - 20:], last[0::2] + last[1::2], last[0::2].abs() + last[1::2].abs(), 2, False, "combine")
+    del out
+    dout = torch.randn((R // 2, N), device="cuda", dtype=torch.bfloat16)
+    dy, dweights = tab_amd.CombineBackward(dout, y, places.cuda(), torch.ones((R // 2, 2), device="cuda"), None, R // 2, 2, R, N)
+    assert torch.equal(dy[0::2], dout) and torch.equal(dy[1::2], dout)
+    d = dout[R // 2 - 20:].double().cpu()
+    for j in (0, 1):
+        ref.check(dweights[R // 2 - 20:, j], (d * last[j::2]).sum(1), (d * last[j::2]).abs().sum(1), N, False, "dweights")
+
+
+def test_gradients_past_32_bits():
+    R, E, N, K = 3000, 33, 8192, 8200
+    g = torch.Generator("cpu").manual_seed(6)
+    offsets = torch.sort(torch.randint(0, R - 99, (E + 1,), generator=g)).values.int()
+    offsets[0], offsets[E] = 0, R
+    x, dy = _rand((R, K), 7).to(torch.bfloat16), _rand((R, N), 8).to(torch.bfloat16)
+    qx, qd = (tab_amd.Quantize8ByExpert(t.cuda(), None, offsets.cuda(), R, R, E, n) for t, n in ((x, K), (dy, N)))
+    dw = tab_amd.ExpertsGradWeight(*qd, *qx, offsets.cuda(), R, E, N, K, torch.bfloat16)
+    assert dw.numel() > 1 << 31
+    e, a = E - 1, int(offsets[E - 1])
+    want, mag = ref.product(ref.rounded(dy[a:, N - 50:].t(), 1, 0), ref.rounded(x[a:, K - 70:].t(), 1, 0))
+    ref.check(dw[e, N - 50:, K - 70:], want, mag, R - a, True, "the last expert")
