@@ -12,7 +12,7 @@ hipError_t launch_linear4(int out_dtype, const Linear8Args &a, void *workspace, 
 
 hipError_t launch_linear4_rows(int dtype, const Linear8RowsArgs &a, hipStream_t stream)
 {
-    const RowsParams p = {a.x, nullptr, a.qw, a.sw, a.y, a.M, a.N, a.K, blocks8(a.K), a.N, 0, a.ldx, make_div32((uint32_t)blocks8(a.K))};
+    const RowsParams p = {a.x, nullptr, a.qw, a.sw, a.y, a.M, a.N, a.K, blocks8(a.K), a.N, 0, 0, a.ldx, make_div32((uint32_t)blocks8(a.K))};
     return dtype == 0 ? launch_rows<0, 0, 0, 4>(p, stream) : dtype == 1 ? launch_rows<1, 0, 1, 4>(p, stream) : launch_rows<2, 0, 2, 4>(p, stream);
 }
 

@@ -34,7 +34,7 @@ bool linear8_rows_supported(int M, int K) { return rows_fit(M, blocks8(K)); }
 
 hipError_t launch_linear8_rows(int dtype, const Linear8RowsArgs &a, hipStream_t stream)
 {
-    const RowsParams p = {a.x, nullptr, a.qw, a.sw, a.y, a.M, a.N, a.K, blocks8(a.K), w_scale_rows(a.N, a.w_block_rows), 0, a.ldx, make_div32((uint32_t)blocks8(a.K))};
+    const RowsParams p = {a.x, nullptr, a.qw, a.sw, a.y, a.M, a.N, a.K, blocks8(a.K), w_scale_rows(a.N, a.w_block_rows), 0, 0, a.ldx, make_div32((uint32_t)blocks8(a.K))};
     return dtype == 0 ? launch_rows<0, 0, 0>(p, stream) : dtype == 1 ? launch_rows<1, 0, 1>(p, stream) : launch_rows<2, 0, 2>(p, stream);
 }
 

@@ -568,7 +568,7 @@ struct RowsParams {
     const void *x;
     const uint8_t *sx, *qw, *sw;
     void *y;
-    int M, N, K, KB, w_scale_rows, groups_each;
+    int M, N, K, KB, w_scale_rows, groups_each, rows_each;  // rows_each: of X, of a workgroup
     long ldx;
     Div32 div_kb;
 };
@@ -611,8 +611,8 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
     extern __shared__ __attribute__((aligned(16))) uint8_t packed[];
     __shared__ __attribute__((aligned(16))) float sums[WAVES * MT * 256];
     const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64), l16 = lane % 16, quarter = lane / 16;
-    const int stride = rows_stride(p.KB);
-    uint32_t *const scales = reinterpret_cast<uint32_t *>(packed + p.M * stride);
+    const int stride = rows_stride(p.KB), m0 = (int)blockIdx.y * p.rows_each, M = min(p.rows_each, p.M - m0);
+    uint32_t *const scales = reinterpret_cast<uint32_t *>(packed + M * stride);
     const bool w_rows = p.w_scale_rows == p.N;
     // block u of the AHEAD that a wave takes from `first` on: every eighth one, or (of 4 bits) every eighth pair, which is a cache line
     auto block_of = [](int first, int u) { return WBITS == 4 ? first + u / 2 * (2 * WAVES) + u % 2 : first + u * WAVES; };
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
 
     // X into LDS: blocks in the order of memory, 16 lanes a block, AT_ONCE of them on their way
     constexpr int AT_ONCE = 8, STEP = 64 * WAVES / 16;
-    const int blocks = p.M * p.KB;
+    const int blocks = M * p.KB;
     for (int first = t / 16; first < blocks; first += AT_ONCE * STEP) {
         using X = typename Element<INPUT == 3 ? 0 : INPUT>::type;
         Words<X> v[AT_ONCE];
@@ -644,10 +644,10 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
             const int block = first + u * STEP, m = (int)div32(block, p.div_kb), kb = block - m * p.KB;
             if (block >= blocks) break;
             if constexpr (INPUT == 3) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p.x) + (long)block * kBlock8 + l16 * 8);
-                v[u].w[0] = w.x, v[u].w[1] = w.y, v[u].w[2] = p.sx[(long)kb * p.M + m];
+                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p.x) + ((long)m0 * p.KB + block) * kBlock8 + l16 * 8);
+                v[u].w[0] = w.x, v[u].w[1] = w.y, v[u].w[2] = p.sx[(long)kb * p.M + m0 + m];
             } else {
-                v[u] = load_words(static_cast<const X *>(p.x) + m * p.ldx, kb * kBlock8 + l16 * 8, p.K);
+                v[u] = load_words(static_cast<const X *>(p.x) + (m0 + m) * p.ldx, kb * kBlock8 + l16 * 8, p.K);
             }
         }
 #pragma unroll
@@ -659,7 +659,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
             if constexpr (INPUT == 3) w = {v[u].w[0], v[u].w[1]}, byte = v[u].w[2];
             else w = pack_run<X, FORMAT>(v[u], byte);
             *reinterpret_cast<uint2 *>(packed + m * stride + kb * kBlock8 + l16 * 8) = w;
-            if (l16 == 0) scales[kb * p.M + m] = byte;
+            if (l16 == 0) scales[kb * M + m] = byte;
         }
     }
     __syncthreads();
@@ -678,8 +678,8 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
                 const i32x8 wf = w_numbers<WBITS>(w_low[u], w_high[WBITS == 8 ? u : 0]);
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const int m = min(i * 16 + l16, p.M - 1);  // (columns past M repeat the last one and are not stored)
-                    acc[i] = times_rows<FORMAT, OUT, WBITS>(wf, w_scale[u], packed + m * stride + kb * kBlock8, scales[kb * p.M + m], quarter, acc[i]);
+                    const int m = min(i * 16 + l16, M - 1);  // (columns past M repeat the last one and are not stored)
+                    acc[i] = times_rows<FORMAT, OUT, WBITS>(wf, w_scale[u], packed + m * stride + kb * kBlock8, scales[kb * M + m], quarter, acc[i]);
                 }
             }
         }
@@ -692,7 +692,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
             float sum = sums[i];
 #pragma unroll
             for (int k = 1; k < WAVES; k++) sum += sums[k * MT * 256 + i];
-            if (m < p.M && n < p.N) static_cast<T *>(p.y)[(long)m * p.N + n] = (T)sum;
+            if (m < M && n < p.N) static_cast<T *>(p.y)[(long)(m0 + m) * p.N + n] = (T)sum;
         }
         if (group + 1 < group1) __syncthreads();
     }
@@ -700,12 +700,24 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
 
 inline bool rows_fit(int M, int KB) { return M <= kRowsMost && KB <= kRowsLds / kBlock8 && rows_lds(M, KB) <= kRowsLds; }
 
+// The rows of X are cut up among workgroups while a CU gets one at the most: each converts its own rows alone.  Whole / cut, in a replayed graph, 4 bits, bf16, us:
+// by 1003 columns (four cuts) 24 x 2050 7.9 / 4.5, 16 x 4096 8.3 / 4.8; by 2048 (two) 16 x 4096 8.2 / 6.0; by 4096, where two cuts would be two workgroups a CU,
+// 8.4 / 8.5.
+inline int rows_cuts(int M, int groups)
+{
+    const int cuts = groups < 256 ? 256 / groups : 1;
+    return cuts < 8 ? (cuts < M ? cuts : M) : (M < 8 ? M : 8);
+}
+
 template <int INPUT, int FORMAT, int OUT, int WBITS = 8> hipError_t launch_rows(RowsParams p, hipStream_t stream)
 {
     const int groups = (p.N + 15) / 16;
     p.groups_each = (groups + 511) / 512;  // two workgroups a CU, each with X in its LDS once
-    const unsigned workgroups = (unsigned)((groups + p.groups_each - 1) / p.groups_each), lds = (unsigned)rows_lds(p.M, p.KB);
-    if (p.M <= 16) linear8_rows<INPUT, FORMAT, OUT, 1, WBITS><<<workgroups, 64 * kRowsWaves, lds, stream>>>(p);
+    const int cuts = rows_cuts(p.M, groups);
+    p.rows_each = (p.M + cuts - 1) / cuts;
+    const dim3 workgroups((unsigned)((groups + p.groups_each - 1) / p.groups_each), (unsigned)((p.M + p.rows_each - 1) / p.rows_each));
+    const unsigned lds = (unsigned)rows_lds(p.rows_each, p.KB);
+    if (p.rows_each <= 16) linear8_rows<INPUT, FORMAT, OUT, 1, WBITS><<<workgroups, 64 * kRowsWaves, lds, stream>>>(p);
     else linear8_rows<INPUT, FORMAT, OUT, 2, WBITS><<<workgroups, 64 * kRowsWaves, lds, stream>>>(p);
     return hipGetLastError();
 }
@@ -794,7 +806,7 @@ inline hipError_t launch_join(int out, const float *parts, void *y, long count, 
 template <int FORMAT, int WBITS> hipError_t launch_product(int out, const Linear8Args &a, int scale_rows, void *workspace, hipStream_t stream)
 {
     if (rows_fit(a.M, a.KB)) {
-        const RowsParams p = {a.qx, a.sx, a.qw, a.sw, a.y, a.M, a.N, a.KB * kBlock8, a.KB, scale_rows, 0, 0, make_div32((uint32_t)a.KB)};
+        const RowsParams p = {a.qx, a.sx, a.qw, a.sw, a.y, a.M, a.N, a.KB * kBlock8, a.KB, scale_rows, 0, 0, 0, make_div32((uint32_t)a.KB)};
         return out == 0 ? launch_rows<3, FORMAT, 0, WBITS>(p, stream) : out == 1 ? launch_rows<3, FORMAT, 1, WBITS>(p, stream) : launch_rows<3, FORMAT, 2, WBITS>(p, stream);
     }
     const Plan8 plan = plan8(out, a.M, a.N, a.KB);
