@@ -291,6 +291,8 @@ struct Quantize4Args {
 long quantize4_tiles(long rows, int K);  // workgroups of 256 threads
 hipError_t launch_quantize4(int dtype, const Quantize4Args &a, hipStream_t stream);
 hipError_t launch_linear4(int out_dtype, const Linear8Args &a, void *workspace, hipStream_t stream);  // (w_block_rows is not read)
+bool linear4_rows_supported(int M, int N, int K);
+size_t linear4_workspace(int out_dtype, int M, int N, int KB);
 hipError_t launch_linear4_rows(int dtype, const Linear8RowsArgs &a, hipStream_t stream);
 
 struct NormArgs {

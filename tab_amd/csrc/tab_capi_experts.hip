@@ -75,7 +75,10 @@ int tab_quantize4(const void *dev_W, int dtype, int E, int M, int K, long ldw, v
     return e == hipSuccess ? TAB_OK : device_fail(e, "quantize4 launch");
 }
 
-size_t tab_linear4_packed_workspace_bytes(int out_dtype, int M, int N, int K) { return tab_linear8_packed_workspace_bytes(out_dtype, M, N, K); }
+size_t tab_linear4_packed_workspace_bytes(int out_dtype, int M, int N, int K) 
+{
+    return M < 1 || N < 1 || K < 1 ? 0 : tab::linear4_workspace(out_dtype, M, N, tab::blocks8(K));
+}
 
 int tab_linear4_packed(const void *dev_QX, const void *dev_SX, const void *dev_QW, const void *dev_SW, int M, int N, int K, void *dev_Y, int out_dtype,
                        void *workspace, size_t workspace_bytes, void *stream)
@@ -93,7 +96,11 @@ int tab_linear4_packed(const void *dev_QX, const void *dev_SX, const void *dev_Q
     return e == hipSuccess ? TAB_OK : device_fail(e, "linear4 launch");
 }
 
-size_t tab_linear4_workspace_bytes(int dtype, int M, int N, int K) { return tab_linear8_workspace_bytes(dtype, M, N, K); }
+size_t tab_linear4_workspace_bytes(int dtype, int M, int N, int K) 
+{
+    if (M < 1 || N < 1 || K < 1 || tab::linear4_rows_supported(M, N, K)) return 0;
+    return packed_bytes(M, K) + tab_linear4_packed_workspace_bytes(dtype, M, N, K);
+}
 
 int tab_linear4(const void *dev_X, int dtype, long ldx, const void *dev_QW, const void *dev_SW, int M, int N, int K, void *dev_Y, void *workspace,
                 size_t workspace_bytes, void *stream)
@@ -104,7 +111,7 @@ int tab_linear4(const void *dev_X, int dtype, long ldx, const void *dev_QW, cons
     TAB_CHECK(check_packed(dev_QW, dev_SW, "QW or SW"));
     if ((uintptr_t)dev_SW % 4) return fail(TAB_ERR_BAD_ARGUMENT, "SW must be aligned to 4 bytes");
     TAB_CHECK(check_rows(dev_Y, dtype, 1, N, N, "Y"));
-    if (tab::linear8_rows_supported(M, K)) {
+    if (tab::linear4_rows_supported(M, N, K)) {
         const tab::Linear8RowsArgs a = {dev_X, static_cast<const uint8_t *>(dev_QW), static_cast<const uint8_t *>(dev_SW), dev_Y, M, N, K, 1, ldx};
         const hipError_t e = tab::launch_linear4_rows(dtype, a, static_cast<hipStream_t>(stream));
         return e == hipSuccess ? TAB_OK : device_fail(e, "linear4 launch");

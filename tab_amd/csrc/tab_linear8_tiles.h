@@ -557,13 +557,13 @@ template <int OUT> __global__ __launch_bounds__(256) void linear8_join(const flo
     }
 }
 
-// Few rows: bound by reading QW once.  A workgroup takes some groups of 16 rows of QW and all (at most 16 * MT) rows of X.  Its waves take the blocks of
+// Few rows: bound by reading QW once.  A workgroup takes some groups of 16 rows of QW and all rows of X, or a part of them (at most 16 * MT).  Its waves take the blocks of
 // K in turn, each lane loads its 2 x 16 bytes of a block of QW itself, AHEAD blocks at a time, and the waves' sums meet in LDS, added up in a
 // fixed order.  X lies in LDS as packed numbers (rows 16 bytes more than whole blocks apart, so that 8 rows' pieces meet different banks) and scales:
 // INPUT 0 .. 2: fp32 / bf16 / fp16, quantized by the workgroup on the way (a block of a row is 16 lanes of eight); 3: packed.
-// One row of 4096 by 4096 x 4096: 5.2-6.0 us with its launch, 16.9 MB at 2.8-3.2 TB/s (through the tiles and a launch of the quantizer 14).  24 rows of
-// 2050 (fp16) by 1003: 9.3-10.4 us, bound by every workgroup's conversion of all of X, which costs less than a launch for it alone; 16 waves
-// instead of 8 took 5.9-6.4 and 10.9-11.2 us.
+// One row of 4096 by 4096 x 4096: 4.6-6.0 us with its launch, 16.9 MB at 2.8-3.6 TB/s (through the tiles and a launch of the quantizer 14); of 4 bits 4.2, 8.9 MB,
+// most of it the launch.  24 rows of 2050 (fp16) by 1003: 5.4 us, of 4 bits 4.6, bound by every workgroup's conversion of its rows of X (of all of them 9.3-10.4),
+// which costs less than a launch for it alone; 16 waves instead of 8 took 5.9-6.4 and (of all rows) 10.9-11.2 us.
 struct RowsParams {
     const void *x;
     const uint8_t *sx, *qw, *sw;
@@ -575,8 +575,8 @@ struct RowsParams {
 
 // The bound between one launch and quantizer, tiles and join: X in 72 KB of LDS, which up to 16 rows (with 8 KB for the waves' sums) leaves room for two workgroups
 // a CU; with 17 to 32 rows the sums take 16 KB, and a CU holds one.  On both sides of it (bf16, by 4096 columns, a pass among others, us):
-//   one launch   8 x 4096  8.7   12 x 4096 10.4   17 x 4096 13.0   8 x 8000 15.0   32 x 2176 12.3   32 x 1000 7.4   by 1003 columns 24 x 2050 9.0, 32 x 2050 10.4
-//   three        18 x 4096 10.6                                    8 x 9300 12.7   32 x 2304  9.5   33 x 1000 7.0   by 1003 columns 33 x 2050 9.0
+//   one launch   8 x 4096  7.6   12 x 4096  9.2   17 x 4096 11.9   8 x 8000 15.0   32 x 2176  9.7   32 x 1000 7.0   by 1003 columns 24 x 2050 5.4, 32 x 2050 5.7
+//   three        18 x 4096 10.0                                    8 x 9300 12.7   32 x 2304  8.6   33 x 1000 7.4   by 1003 columns 33 x 2050 8.8
 // So the largest X in one launch take up to a fifth longer than three launches would; they meet at about 12 rows of 4096.
 constexpr int kRowsMost = 32;           // rows of X
 constexpr int kRowsLds = 72 << 10;      // bytes of X in LDS
@@ -698,15 +698,24 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear8_rows(const RowsParams
     }
 }
 
-inline bool rows_fit(int M, int KB) { return M <= kRowsMost && KB <= kRowsLds / kBlock8 && rows_lds(M, KB) <= kRowsLds; }
-
 // The rows of X are cut up among workgroups while a CU gets one at the most: each converts its own rows alone.  Whole / cut, in a replayed graph, 4 bits, bf16, us:
 // by 1003 columns (four cuts) 24 x 2050 7.9 / 4.5, 16 x 4096 8.3 / 4.8; by 2048 (two) 16 x 4096 8.2 / 6.0; by 4096, where two cuts would be two workgroups a CU,
-// 8.4 / 8.5.
+// 8.4 / 8.5; more than 16 cuts gain nothing (128 x 4096 by 64: eight 8.3, sixteen 5.9).
 inline int rows_cuts(int M, int groups)
 {
-    const int cuts = groups < 256 ? 256 / groups : 1;
-    return cuts < 8 ? (cuts < M ? cuts : M) : (M < 8 ? M : 8);
+    const int free = groups < 256 ? 256 / groups : 1, cuts = free < 16 ? free : 16;
+    return cuts < M ? cuts : M;
+}
+
+// One launch, where a workgroup's rows of X fit.  With weights of 4 bits that goes by the rows after the cut: one launch / three, bf16, us: by 64 columns 128 x 4096
+// 5.9 / 11.5, 256 x 1024 5.0 / 7.7; by 1003 64 x 4096 8.6 / 10.4, 32 x 8192 11.9 / 12.3; by 2048 64 x 2050 9.5 / 9.3.  With weights of 8 bits by all rows,
+// as before the cut: the ways differ in the order of their sums, and a product keeps its bits.
+inline bool rows_fit(int M, int KB) { return M <= kRowsMost && KB <= kRowsLds / kBlock8 && rows_lds(M, KB) <= kRowsLds; }
+template <int WBITS> bool rows_way(int M, int N, int KB)
+{
+    if (WBITS == 8) return rows_fit(M, KB);
+    const int cuts = rows_cuts(M, (N + 15) / 16);
+    return rows_fit((M + cuts - 1) / cuts, KB);
 }
 
 template <int INPUT, int FORMAT, int OUT, int WBITS = 8> hipError_t launch_rows(RowsParams p, hipStream_t stream)
@@ -805,7 +814,7 @@ inline hipError_t launch_join(int out, const float *parts, void *y, long count, 
 // One product of a packed activation: few rows, or tiles, with a launch that joins the parts of K
 template <int FORMAT, int WBITS> hipError_t launch_product(int out, const Linear8Args &a, int scale_rows, void *workspace, hipStream_t stream)
 {
-    if (rows_fit(a.M, a.KB)) {
+    if (rows_way<WBITS>(a.M, a.N, a.KB)) {
         const RowsParams p = {a.qx, a.sx, a.qw, a.sw, a.y, a.M, a.N, a.KB * kBlock8, a.KB, scale_rows, 0, 0, 0, make_div32((uint32_t)a.KB)};
         return out == 0 ? launch_rows<3, FORMAT, 0, WBITS>(p, stream) : out == 1 ? launch_rows<3, FORMAT, 1, WBITS>(p, stream) : launch_rows<3, FORMAT, 2, WBITS>(p, stream);
     }

@@ -46,8 +46,10 @@ def test_sizes():
     assert [lib.tab_run_blocks(r, e) for r, e in ((0, 1), (1, 0), (1, 1), (1, 9), (128, 1), (129, 1), (129, 2), (256, 300), (1000, 4))] == [0, 0, 1, 1, 1, 2, 2, 256, 11]
     assert tab_amd.run_blocks(1000, 4) == 11
     for out in (0, 1, 2):
-        assert lib.tab_linear4_workspace_bytes(out, 17, 1000, 4096) == 0 < lib.tab_linear4_workspace_bytes(out, 18, 1000, 4096)
-        assert lib.tab_linear4_packed_workspace_bytes(out, 17, 1000, 4096) == 0
+        # one launch, its rows cut up among four workgroups (1000 columns) or whole (4096)
+        assert lib.tab_linear4_workspace_bytes(out, 68, 1000, 4096) == 0 < lib.tab_linear4_workspace_bytes(out, 69, 1000, 4096)
+        assert lib.tab_linear4_workspace_bytes(out, 17, 4096, 4096) == 0 < lib.tab_linear4_workspace_bytes(out, 18, 4096, 4096)
+        assert lib.tab_linear4_packed_workspace_bytes(out, 68, 1000, 4096) == lib.tab_linear4_packed_workspace_bytes(out, 17, 4096, 4096) == 0
         assert lib.tab_experts_linear_workspace_bytes(out, 8, 16, 64, 24, 1003, 776) == 0
         assert lib.tab_experts_linear_workspace_bytes(out, 4, 4096, 8192, 8, 512, 300) >= 4096 * (384 + 3)
         assert lib.tab_experts_linear_workspace_bytes(out, 8, 0, 1, 1, 1, 1) == lib.tab_experts_linear_packed_workspace_bytes(out, 1, 8, 1, -1, 1, 1) == 0
@@ -93,15 +95,15 @@ def test_linear4_refusals():
     _refuses(p(SW=P + 2), "4 bytes")
     _refuses(p(Y=None), "null device pointer: Y")
     _refuses(p(M=0x7fffffff), "32-bit offsets", -2)
-    _refuses(p(M=40, K=8192, ws=None), "workspace", -3)
+    _refuses(p(M=400, K=8192, ws=None), "workspace", -3)
     x = lambda X=P, dtype=0, ld=256, QW=P, SW=P, M=64, N=64, K=256, Y=P, ws=P, bytes=1 << 30: lib.tab_linear4(X, dtype, ld, QW, SW, M, N, K, Y, ws, bytes, None)  # noqa: E731
     _refuses(x(dtype=3), "dtype")
     _refuses(x(K=0), "positive")
     _refuses(x(X=None), "null device pointer: X")
     _refuses(x(ld=255), "row stride")
     _refuses(x(SW=P + 1), "4 bytes")
-    _refuses(x(bytes=16), "workspace", -3)
-    _refuses(x(ws=P + 8), "workspace", -3)
+    _refuses(x(M=1000, bytes=16), "workspace", -3)
+    _refuses(x(M=1000, ws=P + 8), "workspace", -3)
 
 
 def test_route_refusals():

@@ -67,9 +67,10 @@ def test_quantize4_takes_no_scale_below_the_smallest():
     _same_packed(Q, S, x)
 
 
-# every way the product is computed: rows (1 .. 32), tiles of 64 with K in parts and whole, of 128, of 256
+# every way the product is computed: rows (whole, cut up among workgroups), tiles of 64 with K in parts and whole, of 128, of 256
 SIZES = [(1, 1, 1), (1, 16, 128), (1, 1000, 2050), (2, 17, 129), (15, 40, 1024), (15, 33, 4096), (16, 33, 4096), (17, 20, 4096), (16, 100, 640), (16, 8300, 130), (17, 33, 300),
-         (31, 64, 128), (32, 130, 2000), (33, 5, 77), (40, 1003, 640), (64, 64, 128), (65, 65, 1153), (100, 72, 8192), (3, 50, 30000), (129, 300, 257), (300, 129, 4000), (500, 777, 520)]
+         (31, 64, 128), (32, 130, 2000), (33, 5, 77), (40, 1003, 640), (64, 64, 128), (65, 65, 1153), (100, 72, 8192), (3, 50, 30000), (129, 300, 257), (300, 129, 4000), (500, 777, 520),
+         (33, 4096, 300), (96, 1003, 2050), (68, 1000, 4096), (69, 1000, 4096), (256, 64, 1024), (512, 16, 640), (513, 16, 640), (130, 2048, 1100), (70, 4100, 520)]
 
 
 @types
