@@ -16,10 +16,11 @@ P = 4096  # an aligned address that is never dereferenced: every call below fail
 WAYS = [(0, 42, 1, 44, 66, 6401), (0, 46, 1, 32, 1600, 6404), (0, 54, 1, 50, 1989, 6416), (0, 5765, 59, 66, 66, 9601), (0, 542, 46, 515, 4787, 9602),
         (0, 846, 20, 1364, 67, 12801), (1, 44, 1, 35, 85, 6401), (1, 1796, 50, 40, 4648, 6402), (1, 49, 1, 45, 1926, 6416), (1, 64, 47, 3550, 74, 9601),
         (1, 564, 57, 98, 5479, 9604), (1, 1230, 37, 695, 69, 12801), (1, 3961, 51, 978, 87, 25601), (1, 10826, 24, 129, 8020, 25604),
-        (1, 30000, 20, 1088, 100, 25601), (1, 30000, 20, 1003, 300, 25601)]
+        (1, 30000, 20, 1088, 100, 25601), (1, 30000, 20, 1003, 300, 25601), (1, 45000, 1000, 33, 140, 6401), (1, 30000, 129, 300, 300, 12801), (0, 9000, 200, 40, 70, 6401)]
 # (output, rows, experts, N, K, half of the tile's rows + columns) of the gradients of the weights
 GRAD_WAYS = [(1, 3000, 4, 1100, 1500, 128), (1, 2000, 2, 300, 520, 64), (1, 1059, 46, 67, 131, 96), (1, 1000, 30, 300, 90, 96), (1, 233, 41, 1171, 131, 256), (1, 2000, 41, 1171, 400, 256),
-             (0, 3000, 4, 600, 700, 64), (0, 33, 45, 33, 358, 96), (0, 900, 8, 1000, 1400, 128)]
+             (0, 3000, 4, 600, 700, 64), (0, 33, 45, 33, 358, 96), (0, 900, 8, 1000, 1400, 128),
+             (1, 3000, 130, 67, 131, 64), (0, 900, 1000, 40, 50, 64), (1, 9000, 1024, 33, 20, 64)]
 
 
 def _refuses(status, message, code=-1):

@@ -203,3 +203,23 @@ def test_packed_experts_keep_their_weights():
     assert layer.QW.dtype == torch.float4_e2m1fn_x2 and torch.equal(layer.QW.view(torch.uint8), qw) and torch.equal(layer(x, routing), want)
     with pytest.raises(RuntimeError, match="inference"):
         layer(x.requires_grad_(), routing)
+
+
+def test_calls_on_two_streams_at_once():
+    """Nothing is shared between calls: two streams run the same layers on inputs of their own, neither waiting for the other."""
+    D = 256
+    block, layer = _mixture(D, 200, 6, 2).packed(8), tab_nn.Linear4.from_float(_rand((D, D), 1))
+    xs = [_rand((rows, D), 90 + rows).cuda() for rows in (5, 300, 300, 70)]
+    with torch.no_grad():
+        want = [layer(block(x)) for x in xs]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        got = [[], []]
+        for turn in range(6):
+            for i, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    got[i].append(layer(block(xs[(turn + i) % 4])))
+        torch.cuda.synchronize()
+    for i in range(2):
+        for turn, y in enumerate(got[i]):
+            assert torch.equal(y, want[(turn + i) % 4])
