@@ -286,7 +286,7 @@ def Quantize4(X, M, K):
 
 def Linear4(X, QW, SW, M, N, K):
     """Linear8 with a weight that Quantize4 packed: X (M x K) is quantized on the way to 8 bits, Y (M, N) has X's type, sums as there.  One launch where the rows
-    that a workgroup takes fit, all of them or, with fewer than 2048 columns, a part."""
+    that a workgroup takes fit, all of them or, with up to 2048 columns, a part."""
     try:
         return _C.Linear4(X, QW, SW, M, N, K)
     except TypeError:

@@ -1,5 +1,6 @@
 // Gradients of the experts' weights: dW[e] = sum over the rows r of expert e of dY[r]^T X[r], from both operands packed along the rows by blocks of 128 that
-// belong to one expert.  Every expert has the same tiles, and a tile goes through its expert's own blocks.
+// belong to one expert.  Every expert has the same tiles, and a tile goes through its expert's own blocks.  16384 rows, 16 experts of 2048 x 2048, E5M2: 97-100 us, 1.4
+// PFLOP/s: 1024 tiles of 256 x 256, four rounds of the chip with some eight steps each, so the way in and out of a tile takes more than half of its time.
 #include "tab_linear8_tiles.h"
 
 namespace tab {

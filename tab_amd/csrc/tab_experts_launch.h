@@ -30,7 +30,8 @@ hipError_t launch_expert_product(int out, bool full_sums, const ExpertsPlan &pla
 // Few rows to an expert: bound by reading the weights of the experts that are chosen.  A workgroup takes at most 2^log_most rows of an expert and some groups of
 // 16 rows of its weight, `split` waves to a group, which take its blocks of K in turn, 2 * AHEAD of them on their way in every wave.  The rows of X lie in
 // LDS, as in linear8_rows.  What a small call takes is the way to the weights: the expert, its rows' numbers, the rows, each a round trip to memory, so
-// the first blocks of the weight are asked for as soon as the expert is known.
+// the first blocks of the weight are asked for as soon as the expert is known.  60 rows, 24 experts of 1003 x 776, fp16: 8.0 us (a quantizer and tiles 18.7); 64 rows, 64
+// experts of 2048 x 4096, 4 bits: 29 us, 184 MB at 6.2 TB/s.
 struct ExpertRowsParams {
     const void *x;
     const uint8_t *sx, *qw, *sw;

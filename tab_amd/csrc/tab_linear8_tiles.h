@@ -159,9 +159,9 @@ template <typename T> __device__ __forceinline__ void store4(T *y, f32x4 v)
 // by the way of its operands into LDS (54 bytes a clock and CU measured; reads of LDS reach 200).  What cost most was a wave that waits to get a load
 // out, or whose scalar instructions make the load's address, and does not multiply meanwhile.  So a step's operands are read from LDS while the
 // step before is multiplied, loads, reads and products alternate, and a load takes two scalar instructions and one addition.
-//   256 x 256  8192^3 404-406 us, 2.7 PFLOP/s, in a replayed graph (432-442 with X's quantizer; 430-460 under a profiler's trace; a library's fp8 product with one
-//              scale a tensor 361)
-//   128 x 128  4096 x 2048 x 4096 37-41 us, 1.7-1.9 PFLOP/s
+//   256 x 256  8192^3 363 us, 3.03 PFLOP/s, in a replayed graph, its output past the caches (404-406 through them; 389 with X's quantizer; a library's fp8 product
+//              with one scale a tensor 361); weights of 4 bits 332
+//   128 x 128  4096 x 2048 x 4096 33 us, 2.1 PFLOP/s
 //   64 x 128   512 x 4096 x 4096 13.8 us, 1.25 PFLOP/s (64 x 64 16.4; both 19 with read and multiplied in turn)
 //   64 x 64    128 x 4096 x 4096 9.0 us (14.0 in turn); fp32 1000 x 776 x 520 6.6 us
 // A step is one block of K: 128 bytes of each of the tile's rows and their scales,

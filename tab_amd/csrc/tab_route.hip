@@ -6,6 +6,9 @@
 //
 // An expert at -inf is closed and never chosen; a token with fewer than k open experts has -1 and the weight 0 in the remaining places.  NaN counts as the largest
 // logit, so that it stays visible: the weights of its token become NaN.  Ties go to the lower index; -0 and 0 are equal.
+//
+// Bound by latency: a choice is one maximum over the wave after the other, and a row's place one exchange through LDS after the other.  16 tokens, 64 experts, 4
+// choices: one launch of 4.0 us; 16384 tokens (bf16) 8.0 + 8.2, their gradient 5.4 (2 MB read, 0.9 MB of whole numbers written).
 #include "tab_blocks8.h"
 #include "tab_common.h"
 #include "tab_experts.h"
@@ -53,7 +56,7 @@ struct RouteParams {
     float *weights;
     int *experts, *rows, *places, *offsets, *counts;  // counts: [workgroups][E], of more than one workgroup
     long ld;
-    int M, E, k, each, normalize;                     // each: tokens of a workgroup
+    int M, E, k, each, normalize, workgroups;         // each: tokens of a workgroup
 };
 
 // Places of the rows of a workgroup's tokens: the rows of its experts begin at `base`.  Every wave has a run of tokens and counters of its own,
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(kThreads) void route_place(const RouteParams p)
     const int t = threadIdx.x, parts = kThreads / p.E, part = t / p.E, e = t - part * p.E;
     int sum = 0, mine = 0;
     if (part < parts)
-        for (int g = part; g < (int)gridDim.x; g += parts) {
+        for (int g = part; g < p.workgroups; g += parts) {
             const int n = p.counts[(long)g * p.E + e];
             sum += n;
             if (g < (int)blockIdx.x) mine += n;
@@ -334,7 +337,7 @@ size_t route_workspace(int M, int E, int) { return workgroups(M) == 1 ? 0 : ((si
 
 hipError_t launch_route(int dtype, const RouteArgs &a, hipStream_t stream)
 {
-    const RouteParams p = {a.logits, a.weights, a.experts, a.rows, a.places, a.offsets, a.workspace, a.ld, a.M, a.E, a.k, tokens_each(a.M), a.normalize};
+    const RouteParams p = {a.logits, a.weights, a.experts, a.rows, a.places, a.offsets, a.workspace, a.ld, a.M, a.E, a.k, tokens_each(a.M), a.normalize, workgroups(a.M)};
     return dtype == 0 ? launch_choose<0>(p, stream) : dtype == 1 ? launch_choose<1>(p, stream) : launch_choose<2>(p, stream);
 }
 
