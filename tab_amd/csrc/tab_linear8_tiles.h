@@ -213,6 +213,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     int kb0 = (int)part * p.kb_per_part, kb1 = min(p.KB, kb0 + p.kb_per_part);
     if constexpr (BY == kRowsByExpert) {
         const Run run = find_run(p.offsets, p.E, p.M, tile_m, log2_of(BM), lane);
+        if (run.expert < 0) return;  // (offsets out of order, the count of their tiles past 32 bits)
         expert = (uint32_t)run.expert, m0 = run.first, end_m = run.end;
         if (run.expert == p.E) expert = 0, kb1 = kb0;  // rows of no expert: zeros
     }
