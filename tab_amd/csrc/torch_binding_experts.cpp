@@ -336,6 +336,7 @@ struct ExpertsFunction : torch::autograd::Function<ExpertsFunction> {
     static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const Tensor &rows, const Tensor &places, const Tensor &offsets,
                           bool gather, int64_t grad_format)
     {
+        const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
         const bool need_dx = x.requires_grad(), need_dw = w.requires_grad();
         const Tensor x2 = matrix(x), w2 = w.contiguous();
         const int K = as_size(x2.size(1), "columns of x"), N = as_size(w.size(1), "rows of an expert's weight");

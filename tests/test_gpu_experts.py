@@ -299,6 +299,26 @@ def test_partial_and_expanded_gradients():
         assert torch.equal(tab_nn.experts_linear8(*both, routing) * 2, y)
 
 
+def test_activations_of_16_bits_and_weights_of_32():
+    """Weights that are bf16 numbers, held in fp32: the same y and dx, and dw in the weights' type."""
+    M, k, E, N, K = 90, 2, 4, 70, 260
+    routing = tab_nn.Routing(*_cuda(ref.plan(M, E, k, 6)))
+    x, w = _rand((M, K), 20).to(torch.bfloat16).cuda().requires_grad_(), _rand((E, N, K), 21).to(torch.bfloat16).cuda().requires_grad_()
+    wide = w.detach().float().requires_grad_()
+    dy = _rand((M * k, N), 22).to(torch.bfloat16).cuda()
+    y, z = tab_nn.experts_linear8(x, w, routing), tab_nn.experts_linear8(x, wide, routing)
+    assert z.dtype == torch.bfloat16 and torch.equal(y, z)
+    (dx, dw), (dx2, dw2) = torch.autograd.grad(y, (x, w), dy), torch.autograd.grad(z, (x, wide), dy)
+    assert torch.equal(dx, dx2) and dw2.dtype == torch.float32
+    # both are sums of the same products: one bound for each
+    d, v = dy.double().cpu(), x.detach().double().cpu()
+    rows, offsets = routing.rows.cpu(), routing.offsets.cpu()
+    for e, first, end in ref.runs(offsets):
+        want, mag = ref.product(ref.rounded(d[first:end].t(), 1, 0), ref.rounded(v[rows[first:end].long()].t(), 1, 0))
+        ref.check(dw[e], want, mag, end - first, True, "16 bits")
+        ref.check(dw2[e], want, mag, end - first, False, "32 bits")
+
+
 def _random_weights(E, N, K, bits, seed):
     """Packed weights by bytes: finite numbers of any size, scales from 2^-7 to 1."""
     g = torch.Generator("cuda").manual_seed(seed)

@@ -178,3 +178,18 @@ def test_layer_keeps_its_weight(convert):
     assert torch.equal(layer(x), want)
     with pytest.raises(RuntimeError, match="inference"):
         layer(x.requires_grad_())
+
+
+@pytest.mark.parametrize("M", [2, 300])
+def test_weight_past_32_bits(M):
+    """A weight of more than 4 GiB, its scales and its outputs far behind its beginning: few rows, and tiles."""
+    N, K = 1100003, 8192
+    g = torch.Generator("cuda").manual_seed(1)
+    QW = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8, device="cuda").view(torch.float4_e2m1fn_x2)
+    SW = torch.randint(120, 128, (K // 128, N, 4), generator=g, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    x = _rand((M, K), 2).to(torch.bfloat16)
+    y = tab_amd.Linear4(x.cuda(), QW, SW, M, N, K)
+    a = ref8.value(*ref8.quantize(x, 1, 0), 1)
+    for n in (slice(0, 200), slice(N - 300, N)):
+        want, mag = ref.product(a, ref.unpack4(QW[n], SW[:, n]))
+        ref.check(y[:, n], want, mag, K, True, f"columns from {n.start}")
