@@ -75,7 +75,7 @@ int tab_quantize4(const void *dev_W, int dtype, int E, int M, int K, long ldw, v
     return e == hipSuccess ? TAB_OK : device_fail(e, "quantize4 launch");
 }
 
-size_t tab_linear4_packed_workspace_bytes(int out_dtype, int M, int N, int K) 
+size_t tab_linear4_packed_workspace_bytes(int out_dtype, int M, int N, int K)
 {
     return M < 1 || N < 1 || K < 1 ? 0 : tab::linear4_workspace(out_dtype, M, N, tab::blocks8(K));
 }
@@ -96,7 +96,7 @@ int tab_linear4_packed(const void *dev_QX, const void *dev_SX, const void *dev_Q
     return e == hipSuccess ? TAB_OK : device_fail(e, "linear4 launch");
 }
 
-size_t tab_linear4_workspace_bytes(int dtype, int M, int N, int K) 
+size_t tab_linear4_workspace_bytes(int dtype, int M, int N, int K)
 {
     if (M < 1 || N < 1 || K < 1 || tab::linear4_rows_supported(M, N, K)) return 0;
     return packed_bytes(M, K) + tab_linear4_packed_workspace_bytes(dtype, M, N, K);

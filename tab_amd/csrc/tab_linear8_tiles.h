@@ -776,13 +776,13 @@ inline Plan8 plan8(int out, int M, int N, int KB)
     return best;
 }
 
-// Whether Y (`count` elements of type `out` in rows of N) is written past the caches: from 8 MB on, where its rows are whole cache lines, which a wave then
+// Whether Y (`count` elements of type `out` in rows of N) is written past the caches: from 16 MB on, where its rows are whole cache lines, which a wave then
 // writes at once.  What is smaller is read from the caches by the next kernel.  16384 x 2048 bf16, two tiles a CU: the way out 21 -> 11 us.  With the quantizer
 // that reads Y behind it, us through / past the caches: 1024 x 4096 29.6 / 31.4, 2048 x 2048 20.4 / 20.2, 4096 x 2048 43.9 / 41.7, 8192 x 8192 over 8192 429 / 399.
 inline int streamed(int out, const void *y, long count, int N)
 {
     const long bytes = out == 0 ? 4 : 2;
-    return count * bytes >= 8l << 20 && (N * bytes) % 128 == 0 && (uintptr_t)y % 128 == 0;
+    return count * bytes >= 16l << 20 && (N * bytes) % 128 == 0 && (uintptr_t)y % 128 == 0;
 }
 
 inline int threads_of(const Plan8 &plan) { return plan.rows == 256 ? 512 : 256; }
