@@ -91,3 +91,23 @@ def test_sums_are_rounded_once(dtype):
     y = torch.tensor([[256.0], [-255.0], [0.0078125]]).to(dtype)
     out = tab_amd.Combine(y.cuda(), torch.tensor([[0, 1, 2]], dtype=torch.int32).cuda(), torch.ones((1, 3), device="cuda"), 1, 3, 3, 1)
     assert torch.equal(out.cpu(), torch.tensor([[1.0078125]]).to(dtype))
+
+
+def test_gradients_are_differences():
+    """Linear in the rows and in the weights: with small whole numbers the differences are exact."""
+    M, k, D = 7, 2, 9
+    plan = ref.plan(M, 4, k, 2, closed=1)
+    g = torch.Generator("cpu").manual_seed(3)
+    y, w, dout = (torch.randint(-4, 5, s, generator=g).float() for s in ((M * k, D), (M, k), (M, D)))
+    f = lambda a, b: float((tab_nn.combine(a.cuda(), tab_nn.Routing(b.cuda(), *(t.cuda() for t in plan[1:]))).cpu() * dout).sum())  # noqa: E731
+    yd, wd = y.cuda().requires_grad_(), w.cuda().requires_grad_()
+    dy, dw = torch.autograd.grad(tab_nn.combine(yd, tab_nn.Routing(wd, *(t.cuda() for t in plan[1:]))), (yd, wd), dout.cuda())
+    for r in range(0, M * k, 3):
+        d = torch.zeros_like(y)
+        d[r, r % D] = 1
+        assert f(y + d, w) - f(y - d, w) == 2 * float(dy[r, r % D])
+    for t in range(M):
+        for j in range(k):
+            d = torch.zeros_like(w)
+            d[t, j] = 1
+            assert f(y, w + d) - f(y, w - d) == 2 * float(dw[t, j])
