@@ -51,6 +51,9 @@ int check_experts(int M, const int *rows, const int *offsets, int R, int E, int 
     return TAB_OK;
 }
 
+// Weights of 4 bits have full sums towards fp32 in any case
+bool full_sums_of(int full_sums, int w_bits) { return full_sums != 0 || w_bits == 4; }
+
 size_t parts_bytes(const tab::ExpertsPlan &plan, int R, int N) { return plan.few || plan.parts == 1 ? 0 : (size_t)plan.parts * (size_t)R * (size_t)N * sizeof(float); }
 
 tab::ExpertsArgs experts_args(const void *x, const void *sx, long ldx, int M, const int *rows, const int *offsets, const void *qw, const void *sw, int w_block_rows,
@@ -198,7 +201,7 @@ int tab_quantize8_by_expert(const void *dev_X, int dtype, long ldx, int M, const
 
 size_t tab_experts_linear_packed_workspace_bytes(int out_dtype, int full_sums, int w_bits, int R, int E, int N, int K)
 {
-    return R < 1 || E < 1 || N < 1 || K < 1 ? 0 : parts_bytes(tab::experts_plan(out_dtype, full_sums != 0, w_bits, R, E, N, tab::blocks8(K)), R, N);
+    return R < 1 || E < 1 || N < 1 || K < 1 ? 0 : parts_bytes(tab::experts_plan(out_dtype, full_sums_of(full_sums, w_bits), w_bits, R, E, N, tab::blocks8(K)), R, N);
 }
 
 int tab_experts_linear_packed(const void *dev_QX, int x_format, const void *dev_SX, int M, const int *dev_rows, const int *dev_offsets, const void *dev_QW,
@@ -206,14 +209,14 @@ int tab_experts_linear_packed(const void *dev_QX, int x_format, const void *dev_
                               void *workspace, size_t workspace_bytes, void *stream)
 {
     TAB_CHECK(check_format(x_format));
-    TAB_CHECK(check_experts(M, dev_rows, dev_offsets, R, E, N, K, out_dtype, full_sums != 0, w_bits, w_block_rows));
+    TAB_CHECK(check_experts(M, dev_rows, dev_offsets, R, E, N, K, out_dtype, full_sums_of(full_sums, w_bits), w_bits, w_block_rows));
     if (w_bits == 4 && x_format != TAB_E4M3) return fail(TAB_ERR_BAD_ARGUMENT, "weights of 4 bits take activations in E4M3");
     TAB_CHECK(check_packed(dev_QX, dev_SX, "QX or SX"));
     TAB_CHECK(check_packed(dev_QW, dev_SW, "QW or SW"));
     if (w_bits == 4 && (uintptr_t)dev_SW % 4) return fail(TAB_ERR_BAD_ARGUMENT, "SW must be aligned to 4 bytes");
     TAB_CHECK(check_rows(dev_Y, out_dtype, 1, N, N, "Y"));
     TAB_CHECK(check_workspace(workspace, workspace_bytes, tab_experts_linear_packed_workspace_bytes(out_dtype, full_sums, w_bits, R, E, N, K)));
-    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, full_sums != 0, w_bits, R, E, N, tab::blocks8(K));
+    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, full_sums_of(full_sums, w_bits), w_bits, R, E, N, tab::blocks8(K));
     const tab::ExpertsArgs a = experts_args(dev_QX, dev_SX, 0, M, dev_rows, dev_offsets, dev_QW, dev_SW, w_block_rows, R, E, N, K, dev_Y);
     const hipError_t e = w_bits == 4 ? tab::launch_experts4(out_dtype, plan, a, workspace, static_cast<hipStream_t>(stream))
                                      : tab::launch_experts8(out_dtype, full_sums != 0, x_format, plan, a, workspace, static_cast<hipStream_t>(stream));

@@ -5,6 +5,7 @@ import torch
 import experts_reference as ref
 import layers8_reference as ref8
 import tab_amd
+from tab_amd import _capi
 from tab_amd import nn as tab_nn
 from test_experts_host import GRAD_WAYS, WAYS
 
@@ -317,6 +318,35 @@ def test_activations_of_16_bits_and_weights_of_32():
         want, mag = ref.product(ref.rounded(d[first:end].t(), 1, 0), ref.rounded(v[rows[first:end].long()].t(), 1, 0))
         ref.check(dw[e], want, mag, end - first, True, "16 bits")
         ref.check(dw2[e], want, mag, end - first, False, "32 bits")
+
+
+@pytest.mark.parametrize("R", [30, 9000])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_fp32_outputs_with_the_sums_of_16_bits(bits, R):
+    """full_sums 0 through the C ABI: within its bound; with weights of 4 bits there is no such form, the sums are the full ones."""
+    E, N, K = 8, 1024, 300
+    x, w = _rand((R, K), 30).to(torch.bfloat16), _rand((E, N, K), 31, 0.1)
+    QW, SW, values = _pack(w, bits)
+    QX, SX = tab_amd.Quantize8(x.cuda(), R, K)
+    g = torch.Generator("cpu").manual_seed(32)
+    offsets = torch.sort(torch.randint(0, R + 1, (E + 1,), generator=g)).values.int()
+    offsets[0] = 0
+    lib, on = _capi.load(), offsets.cuda()
+    y = [torch.full((R, N), float("nan"), device="cuda") for _ in range(2)]
+    for full in (0, 1):
+        size = lib.tab_experts_linear_packed_workspace_bytes(0, full, bits, R, E, N, K)
+        ws = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+        status = lib.tab_experts_linear_packed(QX.data_ptr(), 0, SX.data_ptr(), R, None, on.data_ptr(), QW.data_ptr(), SW.data_ptr(), bits, 128, R, E, N, K, y[full].data_ptr(),
+                                               0, full, ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+        assert status == 0, lib.tab_last_error().decode()
+    a = ref8.unpack(QX, SX, 1)
+    want, mag = torch.zeros((R, N), dtype=torch.float64), torch.zeros((R, N), dtype=torch.float64)
+    for e, first, end in ref.runs(offsets):
+        want[first:end], mag[first:end] = ref.product(a[first:end], values[e])
+    ref.check(y[1], want, mag, K, False, "full sums")
+    ref.check(y[0], want, mag, K, bits == 8, "sums of 16 bits")
+    if bits == 4:
+        assert torch.equal(y[0], y[1])
 
 
 def _random_weights(E, N, K, bits, seed):
