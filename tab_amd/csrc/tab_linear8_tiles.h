@@ -381,7 +381,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
         asm volatile("" ::: "memory");
     };
     auto all_read = [] { __builtin_amdgcn_s_waitcnt(0xc07f); };  // this wave's reads of LDS are done
-        auto load_first = [&] {
+    auto load_first = [&] {
 #pragma unroll
         for (int k = 0; k < STAGES; k++)
 #pragma unroll
