@@ -1,5 +1,6 @@
 // Products of rows sorted by expert with 8-bit weights, and the rule that picks their kernel.  16384 rows, bf16: 32 experts of 2048 x 4096 150-159 us, 1.75-1.8 PFLOP/s
-// (640 tiles of 256 x 256 with a quarter of their rows empty, 2.5 rounds of the chip); 16 of 2048 x 2048 85-90, rows in fp32 100-104.
+// (640 tiles of 256 x 256 with a quarter of their rows empty, 2.5 rounds of the chip; 512 rows each 124, one weight for all 107, as linear8's kernel); 16 of 2048 x 2048
+// 82-90 (1024 rows each 64), rows in fp32 100-104.
 #include "tab_experts_launch.h"
 
 namespace tab {
