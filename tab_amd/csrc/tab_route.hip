@@ -231,7 +231,8 @@ __global__ __launch_bounds__(kThreads) void route_place(const RouteParams p)
     if (t < p.E) begin[t] += mine;
     __syncthreads();
     const int token0 = (int)blockIdx.x * p.each, token1 = min(token0 + p.each, p.M);
-    for (int r = max(all_rows, token0 * p.k) + t; r < token1 * p.k; r += kThreads) p.rows[r] = -1;
+    // (unsigned: the step behind the last row may pass 2^31)
+    for (uint32_t r = (uint32_t)max(all_rows, token0 * p.k) + t; r < (uint32_t)(token1 * p.k); r += kThreads) p.rows[r] = -1;
     place_rows(p, token0, token1, begin, counters);
 }
 

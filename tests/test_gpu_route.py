@@ -171,3 +171,26 @@ def test_same_call_same_bits_and_more_dimensions():
     assert dx.shape == x.shape
     with pytest.raises(RuntimeError, match="second derivatives"):
         torch.autograd.grad(tab_nn.route(x, 4).weights.sum(), x, create_graph=True)
+
+
+def test_as_many_rows_as_a_call_may_have():
+    """2^31 - 544 rows: the steps of a workgroup's threads past the last row must not come round to numbers below zero.  (43 GB of the GPU's memory.)"""
+    k, closed = 32, 3
+    M = (0x7fffffff - 512) // k
+    logits = (-torch.arange(k, device="cuda", dtype=torch.bfloat16)).repeat(M, 1)
+    logits[M - closed:] = float("-inf")
+    weights, experts, rows, places, offsets = tab_amd.Route(logits, M, k, k)
+    del logits
+    n = M - closed  # rows of each expert
+    assert torch.equal(offsets.cpu(), torch.arange(k + 1, dtype=torch.int32) * n)
+    tokens = torch.arange(n, device="cuda", dtype=torch.int32)
+    for e in range(k):
+        assert torch.equal(rows[e * n:(e + 1) * n], tokens)
+        assert torch.equal(places[:n, e], tokens + e * n)
+        assert (experts[:n, e] == e).all() and (weights[:n, e] == weights[0, e]).all()
+    assert (rows[k * n:] == -1).all() and (places[n:] == -1).all() and (experts[n:] == -1).all() and not weights[n:].any()
+    want = torch.softmax(-torch.arange(k, dtype=torch.float64), 0)
+    # a difference exact in fp32, an exponential, a sum of 32 and a division: as in the test of the weights
+    assert ((weights[0].cpu().double() - want).abs() <= (32 + 80) * 2.0 ** -23 * want).all()
+    del weights, experts, rows, places
+    torch.cuda.empty_cache()
