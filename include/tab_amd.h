@@ -345,7 +345,7 @@ int tab_norm_residual_backward(const void *dev_dR, const void *dev_dH, const voi
  *      16-byte aligned
  *   S  E8M0 bytes [E][ceil(K/128)][M][4], one for each group of 32 of a row, 4-byte aligned
  * A group's scale is the smallest power of two from 2^-126 on with which its largest magnitude fits, a packed number the nearest one to W, half to
- * even.  The format knows neither infinities nor NaN: a group that holds one has the scale 255, NaN.
+ * even.  The format knows neither infinities nor NaN: a group that holds one has the scale 255, NaN.  All products take weights of up to 2^29 - 1 rows.
  */
 int tab_quantize4(const void *dev_W, int dtype, int E, int M, int K, long ldw, void *dev_Q, void *dev_S, void *stream);
 

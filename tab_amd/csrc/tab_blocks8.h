@@ -260,6 +260,7 @@ struct Linear8Args {
     int w_block_rows;  // rows of QW under one scale: 1 or 128
 };
 constexpr int kBlocks8Most = 65535;   // blocks of K: 256 packed rows stay below 2^31 bytes
+constexpr int kRows4Most = 0x1fffffff;  // rows of a weight of 4 bits: their four scale bytes each stay below 2^31 (and what Quantize4 packs in one launch)
 size_t linear8_workspace(int out_dtype, int M, int N, int KB);
 long linear8_threads(int out_dtype, int M, int N, int KB);  // of the launch
 int linear8_way(int out_dtype, int M, int N, int KB);  // 0: few rows; else (the tile's rows + columns) / 2 * 100 + the parts of K

@@ -24,6 +24,12 @@ int check_weight_bits(int bits, int w_block_rows)
     return TAB_OK;
 }
 
+// Columns of a product with weights of 4 bits
+int check_columns4(int N)
+{
+    return N > tab::kRows4Most ? fail(TAB_ERR_BAD_SHAPE, "weights of 4 bits may have %d rows, got %d: their scales are found by 32-bit offsets", tab::kRows4Most, N) : TAB_OK;
+}
+
 // Rows sorted by expert
 int check_runs(int M, const int *rows, const int *offsets, int R, int E)
 {
@@ -44,6 +50,7 @@ int check_experts(int M, const int *rows, const int *offsets, int R, int E, int 
     if (N < 1 || K < 1) return fail(TAB_ERR_BAD_ARGUMENT, "N and K must be positive");
     const int KB = tab::blocks8(K);
     if (N > kMostRows || KB > tab::kBlocks8Most) return fail(TAB_ERR_BAD_SHAPE, "product too large for 32-bit offsets into a tile");
+    if (w_bits == 4) TAB_CHECK(check_columns4(N));
     const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, full_sums, w_bits, R, E, N, KB);
     if (plan.workgroups * 512 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "product too large for one launch");
     if (!plan.few && (unsigned long)M * (unsigned long)KB * tab::kBlock8 > 0xe0000000ul)
@@ -88,6 +95,7 @@ int tab_linear4_packed(const void *dev_QX, const void *dev_SX, const void *dev_Q
 {
     TAB_CHECK(check_type(out_dtype, "out_dtype"));
     TAB_CHECK(check_linear(out_dtype, M, N, K));
+    TAB_CHECK(check_columns4(N));
     TAB_CHECK(check_packed(dev_QX, dev_SX, "QX or SX"));
     TAB_CHECK(check_packed(dev_QW, dev_SW, "QW or SW"));
     if ((uintptr_t)dev_SW % 4) return fail(TAB_ERR_BAD_ARGUMENT, "SW must be aligned to 4 bytes");
@@ -110,6 +118,7 @@ int tab_linear4(const void *dev_X, int dtype, long ldx, const void *dev_QW, cons
 {
     TAB_CHECK(check_type(dtype, "dtype"));
     TAB_CHECK(check_linear(dtype, M, N, K));
+    TAB_CHECK(check_columns4(N));
     TAB_CHECK(check_rows(dev_X, dtype, M, K, ldx, "X"));
     TAB_CHECK(check_packed(dev_QW, dev_SW, "QW or SW"));
     if ((uintptr_t)dev_SW % 4) return fail(TAB_ERR_BAD_ARGUMENT, "SW must be aligned to 4 bytes");

@@ -266,3 +266,17 @@ def test_tangents_are_refused_and_not_dropped():
                      lambda: tab_nn.PackedExperts(q, s, 3, 128, 8)(dual(4, 128), routing)):
             with pytest.raises(RuntimeError, match="forward mode"):
                 call()
+
+
+@pytest.mark.parametrize("N", [1 << 29, (1 << 29) + 16, 0x7fffffff - 512])
+@pytest.mark.parametrize("M,K", [(1, 128), (1, 300), (700, 128)])
+def test_weights_of_4_bits_whose_scales_32_bits_do_not_reach(M, K, N):
+    """Four scale bytes a row: from 2^29 rows on the offset of a row's, and of the next block of K's, would come round to below zero."""
+    lib, E, R, W = _capi.load(), 1, 1, 1 << 40
+    for dtype in (0, 1, 2):
+        _refuses(lib.tab_linear4(P, dtype, 1 << 10, P, P, M, N, K, P, P, W, None), "", -2)
+        _refuses(lib.tab_linear4_packed(P, P, P, P, M, N, K, P, dtype, P, W, None), "", -2)
+        _refuses(lib.tab_experts_linear(P, dtype, 1 << 10, M, P, P, P, P, 4, 1, R, E, N, K, P, P, W, None), "", -2)
+        _refuses(lib.tab_experts_linear_packed(P, 0, P, M, P, P, P, P, 4, 1, R, E, N, K, P, dtype, 1, P, W, None), "", -2)
+    if M == 1 and K == 128:
+        _refuses(lib.tab_linear4(P, 1, 1 << 10, P, P, M, N, K, P, P, W, None), "weights of 4 bits", -2)
