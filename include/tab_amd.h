@@ -387,7 +387,7 @@ int tab_route_backward(const float *dev_dweights, const float *dev_weights, cons
  *                 4: those of tab_quantize4
  * tab_experts_linear quantizes X on the way (E4M3, 1 x 128); Y has X's type.  Few rows to an expert take one launch.  tab_experts_linear_packed takes X packed;
  * full_sums 0 lets an fp32 Y have the sums of a 16-bit one (8-bit weights; see tab_linear8_packed).  X may take at most 3.5 GiB packed, or any size
- * where few rows take one launch.
+ * where few rows take one launch or dev_rows is NULL.
  */
 size_t tab_experts_linear_workspace_bytes(int dtype, int w_bits, int M, int R, int E, int N, int K);
 int tab_experts_linear(const void *dev_X, int dtype, long ldx, int M, const int *dev_rows, const int *dev_offsets, const void *dev_QW, const void *dev_SW, int w_bits,

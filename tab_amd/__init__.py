@@ -349,7 +349,7 @@ def _call_rows(fn, before, rows, after, ints, *rest):
 def ExpertsLinear(X, rows, offsets, QW, SW, M, R, E, N, K):
     """Rows sorted by expert times their expert's weight: Y (R, N) of X's type, Y[r] = X[rows[r]] QW[e]^T for offsets[e] <= r < offsets[e + 1], zeros
     behind offsets[E].  X (M x K) is quantized on the way as Linear8 does; rows and offsets are Route's, rows None where X is sorted already (M = R).  QW, SW:
-    the experts' weights from QuantizeExperts, 8 or 4 bits.  Few rows to an expert take one launch; otherwise X may take at most 3.5 GiB packed."""
+    the experts' weights from QuantizeExperts, 8 or 4 bits.  Few rows to an expert take one launch; otherwise, with rows, X may take at most 3.5 GiB packed."""
     try:
         return _C.ExpertsLinear(X, rows, offsets, QW, SW, M, R, E, N, K)
     except TypeError:

@@ -53,8 +53,9 @@ int check_experts(int M, const int *rows, const int *offsets, int R, int E, int 
     if (w_bits == 4) TAB_CHECK(check_columns4(N));
     const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, full_sums, w_bits, R, E, N, KB);
     if (plan.workgroups * 512 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "product too large for one launch");
-    if (!plan.few && (unsigned long)M * (unsigned long)KB * tab::kBlock8 > 0xe0000000ul)
-        return fail(TAB_ERR_BAD_SHAPE, "X takes more than 3.5 GiB packed: too large for 32-bit offsets");
+    // listed rows are read by 32-bit offsets into all of X, rows as they are sorted by those into a tile
+    if (!plan.few && rows && (unsigned long)M * (unsigned long)KB * tab::kBlock8 > 0xe0000000ul)
+        return fail(TAB_ERR_BAD_SHAPE, "X takes more than 3.5 GiB packed: too large for the 32-bit offsets of listed rows");
     return TAB_OK;
 }
 

@@ -228,7 +228,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
 
     const int wave = __builtin_amdgcn_readfirstlane(t / 64), wm = wave / WN, wn = wave % WN, l16 = lane % 16, quarter = lane / 16;
     const int row_bytes = p.KB * kBlock8, w_row_bytes = p.KB * kWBlock, rows_x = min(BM, end_m - m0), rows_w = min(BN, p.N - n0);
-    const uint8_t *const qx = p.qx + (GATHER ? 0 : (long)m0 * row_bytes);
+    // one buffer holds X: listed rows from the first one on, as a list may name any, others from the tile's
+    int x_first = m0;
+    if constexpr (GATHER) x_first = p.rows ? 0 : m0;
+    const uint8_t *const qx = p.qx + (long)x_first * row_bytes;
     const uint8_t *const qw = p.qw + ((BY == kRowsByExpert ? (long)expert * p.N : 0) + n0) * (long)w_row_bytes;
     const uint8_t *const sw = p.sw + (BY == kRowsByExpert ? (long)expert * p.KB * p.w_scale_rows * (WBITS == 4 ? 4 : 1) : 0);
     // load i of a wave is eight rows of an operand's tile, eight lanes a row: of W the waves take turns, of X those that multiply the rows
@@ -236,12 +239,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     const uint32_t x_at = (uint32_t)(first_x + lane / 8) * (uint32_t)row_bytes + (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
     uint32_t w_at = (uint32_t)(first_w + lane / W_LANES) * (uint32_t)w_row_bytes + (uint32_t)(turn * kWBlock) +
                     (uint32_t)(WBITS == 4 ? (lane % 4) ^ (lane / 16) : (lane % 8) ^ (lane / 8)) * 16;
-    // row `row` of the tile in the buffer of all of X, in units of `unit` bytes
+    // row `row` of the tile in the buffer of X, in units of `unit` bytes
     auto gathered = [&](int row, int unit) {
         if constexpr (GATHER) {
             if (row >= rows_x) return kGatherMost;
-            const int from = p.rows ? p.rows[m0 + row] : m0 + row;
-            return from >= 0 && from < p.x_rows ? (uint32_t)from * (uint32_t)unit : kGatherMost;
+            const int from = p.rows ? p.rows[m0 + row] : row;
+            return from >= 0 && from < p.x_rows - x_first ? (uint32_t)from * (uint32_t)unit : kGatherMost;
         }
         return 0u;
     };
@@ -258,7 +261,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     auto scales_of = [&](bool x, int place, bool any) {
         const int groups = x ? TM : TN, row = place / (16 * groups) * (16 * groups) + place % groups * 16 + place / groups % 16;
         if constexpr (GATHER)
-            if (x) return Scales{p.sx + (long)first * p.x_rows, p.x_rows, !any ? 0 : p.x_rows, gathered(row, 1)};
+            if (x) return Scales{p.sx + x_first + (long)first * p.x_rows, p.x_rows, !any ? 0 : p.x_rows - x_first, gathered(row, 1)};
         if (WBITS == 4 && !x) return Scales{sw + ((long)first * p.N + n0) * 4, p.N * 4, any ? rows_w * 4 : 0, (uint32_t)row * 4};
         const int step = x ? p.M : p.w_scale_rows;
         return Scales{(x ? p.sx + m0 : sw + (row_scales ? n0 : n0 / kBlock8)) + (long)first * step, step,
@@ -270,7 +273,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tiles(const typename 
     const uint32_t lds_at = lds_address(lds);
     // the rows of an operand's tile are one buffer: rows past its end, and with a size of zero all of it, load as zeros
     i32x4 x_rows = buffer(qx, rows_x * row_bytes), w_rows = buffer(qw, rows_w * w_row_bytes);
-    if constexpr (GATHER) x_rows[2] = (int)((uint32_t)p.x_rows * (uint32_t)row_bytes);  // of up to kGatherMost bytes
+    if constexpr (GATHER) x_rows[2] = __builtin_amdgcn_readfirstlane((int)(uint32_t)min((unsigned long)(p.x_rows - x_first) * (unsigned long)row_bytes, (unsigned long)kGatherMost));
     auto sized = [](i32x4 b, bool live) { return i32x4{b[0], b[1], live ? b[2] : 0, b[3]}; };
     // load i of step kb into the part of LDS at `stage`, the scales last (those of one step after another).  Past the end of K zeros, so
     // that the count of a wave's loads stays the same.

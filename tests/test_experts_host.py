@@ -280,3 +280,13 @@ def test_weights_of_4_bits_whose_scales_32_bits_do_not_reach(M, K, N):
         _refuses(lib.tab_experts_linear_packed(P, 0, P, M, P, P, P, P, 4, 1, R, E, N, K, P, dtype, 1, P, W, None), "", -2)
     if M == 1 and K == 128:
         _refuses(lib.tab_linear4(P, 1, 1 << 10, P, P, M, N, K, P, P, W, None), "weights of 4 bits", -2)
+
+
+def test_sorted_rows_have_no_bound_that_listed_ones_have():
+    """(Refused for their workspace, which is checked behind the sizes.)"""
+    lib, R, N, K = _capi.load(), 1 << 24, 64, 256
+    for bits in (8, 4):
+        for rows, message, code in ((P, "3.5 GiB", -2), (None, "workspace", -3)):
+            _refuses(lib.tab_experts_linear(P, 1, K, R, rows, P, P, P, bits, 128, R, 8, N, K, P, None, 0, None), message, code)
+    _refuses(lib.tab_experts_linear_packed(P, 0, P, R, P, P, P, P, 8, 128, R, 8, N, K, None, 1, 0, None, 0, None), "3.5 GiB", -2)
+    _refuses(lib.tab_experts_linear_packed(P, 0, P, R, None, P, P, P, 8, 128, R, 8, N, K, None, 1, 0, None, 0, None), "null device pointer: Y")

@@ -428,3 +428,47 @@ def test_gradients_past_32_bits():
     e, a = E - 1, int(offsets[E - 1])
     want, mag = ref.product(ref.rounded(dy[a:, N - 50:].t(), 1, 0), ref.rounded(x[a:, K - 70:].t(), 1, 0))
     ref.check(dw[e, N - 50:, K - 70:], want, mag, R - a, True, "the last expert")
+
+
+@pytest.mark.parametrize("bits,dtype", [(8, torch.bfloat16), (4, torch.float32)])
+def test_sorted_rows_past_32_bits(bits, dtype):
+    """Rows that come sorted, past 4 GiB of packed numbers: each tile reads its own, so there is no bound on all of them as there is on listed ones."""
+    R, E, N, K = 560000, 3, 40, 8192
+    g = torch.Generator("cuda").manual_seed(11)
+    x = torch.randint(-3, 4, (R, K), generator=g, dtype=torch.int8, device="cuda").to(dtype)
+    w = torch.randint(-3, 4, (E, N, K), generator=torch.Generator("cpu").manual_seed(12)).float()  # (no number of 4 bits is 5)
+    QW, SW = tab_amd.QuantizeExperts(w.cuda(), E, N, K, bits)
+    offsets = torch.tensor([0, 1000, 300003, R - 77], dtype=torch.int32)
+    y = tab_amd.ExpertsLinear(x, None, offsets.cuda(), QW, SW, R, R, E, N, K)
+    assert not y[R - 77:].any()
+    for e, first, end in ((0, 0, 1000), (1, 1000, 1300), (1, 299000, 300003), (2, 300003, 300300), (2, R - 700, R - 77)):
+        want = x[first:end].double().cpu() @ w[e].double().t()  # whole numbers below 2^17: exact but for the output's rounding
+        assert torch.equal(y[first:end].cpu(), want.to(dtype)), f"rows {first}"
+
+
+def test_training_past_32_bits():
+    """Gradients of more sorted rows than listed ones could be: what the forward pass takes, the backward pass takes."""
+    M, k, E, N, K = 280000, 2, 3, 8192, 16
+    R = M * k
+    assert R * N > 1 << 32
+    g = torch.Generator("cpu").manual_seed(13)
+    x = torch.randint(-4, 5, (M, K), generator=g).to(torch.bfloat16)
+    w = torch.randint(-3, 4, (E, N, K), generator=g).float()
+    routing = tab_nn.route(torch.randn((M, E), generator=g).cuda(), k)
+    rows, places, offsets = (t.cpu() for t in routing[2:])
+    xd, wd = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y = tab_nn.experts_linear8(xd, wd, routing)
+    dy = torch.randint(-1, 2, (R, N), generator=torch.Generator("cuda").manual_seed(14), dtype=torch.int8, device="cuda").to(torch.bfloat16)
+    dx, dw = torch.autograd.grad(y, (xd, wd), dy)
+    x64, w64, at = x.double(), w.double(), offsets.tolist()
+    for e in range(E):
+        first, end = at[e], at[e + 1]
+        assert torch.equal(y[end - 50:end].cpu().double(), x64[rows[end - 50:end].long()] @ w64[e].t()), f"expert {e}"  # whole numbers up to 192
+        n = slice(N - 40, N)
+        assert torch.equal(dw[e, n].cpu().double(), dy[first:end, n].double().cpu().t() @ x64[rows[first:end].long()]), f"gradient of weight {e}"  # below 2^24
+    for t in (0, 1, M // 2, *range(M - 60, M)):
+        want = 0
+        for p in places[t].tolist():
+            e = next(e for e in range(E) if at[e] <= p < at[e + 1])
+            want = want + dy[p].double().cpu() @ w64[e]
+        assert torch.equal(dx[t].cpu(), want.to(torch.bfloat16)), f"gradient of token {t}"
