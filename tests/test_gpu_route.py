@@ -194,3 +194,23 @@ def test_as_many_rows_as_a_call_may_have():
     assert ((weights[0].cpu().double() - want).abs() <= (32 + 80) * 2.0 ** -23 * want).all()
     del weights, experts, rows, places
     torch.cuda.empty_cache()
+
+
+def test_gradients_of_more_tokens_than_a_launch_has_waves():
+    """Past 2^26 tokens a wave takes several."""
+    M, E = (1 << 26) + 70001, 2
+    logits = torch.randn((M, E), generator=torch.Generator("cuda").manual_seed(1), device="cuda", dtype=torch.bfloat16)
+    x = logits.requires_grad_()
+    routing = tab_nn.route(x, 1, normalize=False)
+    g = torch.randn((M, 1), generator=torch.Generator("cuda").manual_seed(2), device="cuda")
+    dx, = torch.autograd.grad(routing.weights, x, g)
+    for at in (slice(0, 1000), slice(0, None, 6007), slice(M - 100000, M)):
+        v, e, gt = logits.detach()[at].double(), routing.experts[at].long(), g[at].double()
+        p = torch.softmax(v, 1)
+        w = p.gather(1, e)
+        chosen = torch.zeros_like(p).scatter_(1, e, gt)
+        want, mag = p * (chosen - gt * w), p * (chosen.abs() + (gt * w).abs())
+        assert torch.equal(e, torch.where(v[:, :1] >= v[:, 1:], 0, 1))
+        # as in the test of the gradients
+        off, spread = (dx[at].double() - want).abs(), (v[:, :1] - v[:, 1:]).abs()
+        assert (off <= (spread + 80) * 2.0 ** -23 * mag + ref.UNIT[torch.bfloat16] * (1 + 2.0 ** -10) * want.abs() + ref.TINY[torch.bfloat16]).all()
