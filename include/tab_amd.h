@@ -412,6 +412,9 @@ int tab_quantize8_by_expert(const void *dev_X, int dtype, long ldx, int M, const
 /* dW[e] (N x K) = sum over the rows r of expert e of dY[r]^T X[r], from dY (R x N) and X (E4M3) packed by tab_quantize8_by_expert; zeros for an expert without rows. */
 int tab_experts_grad_weight(const void *dev_QD, int d_format, const void *dev_SD, const void *dev_QX, const void *dev_SX, const int *dev_offsets, int R, int E, int N,
                             int K, void *dev_dW, int out_dtype, void *stream);
+/* Whether the gradients of Y (R x N) = X W^T by expert are within the bounds of the calls that they take, so that a training step can be refused before its
+ * first product: that of X (of_x; M tokens of k choices each, or with k 0 the R sorted rows) and those of W (of_w: up to 65535 of tab_run_blocks).  Host only. */
+int tab_experts_check_gradients(int x_dtype, int w_dtype, int M, int k, int R, int E, int N, int K, int of_x, int of_w);
 
 /*
  * The experts' rows back to their tokens: out[t] (M x D) = sum over j of weights[t][j] Y[places[t][j]], Y R x D; a place outside Y is left out.  weights NULL: ones.

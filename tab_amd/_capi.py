@@ -66,6 +66,7 @@ SIGNATURES = {
     "tab_run_blocks": (_int, [_int] * 2),
     "tab_quantize8_by_expert": (_int, [_vp, _int, ctypes.c_long, _int, _vp, _vp] + [_int] * 4 + [_vp] * 5),
     "tab_experts_grad_weight": (_int, [_vp, _int] + [_vp] * 4 + [_int] * 4 + [_vp, _int, _vp]),
+    "tab_experts_check_gradients": (_int, [_int] * 10),
     "tab_combine": (_int, [_vp, _int, _vp, _vp] + [_int] * 4 + [_vp, _int, _vp]),
     "tab_combine_backward": (_int, [_vp, _vp, _int] + [_vp] * 3 + [_int] * 4 + [_vp] * 3),
 }

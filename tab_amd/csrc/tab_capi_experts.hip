@@ -30,15 +30,36 @@ int check_columns4(int N)
     return N > tab::kRows4Most ? fail(TAB_ERR_BAD_SHAPE, "weights of 4 bits may have %d rows, got %d: their scales are found by 32-bit offsets", tab::kRows4Most, N) : TAB_OK;
 }
 
-// Rows sorted by expert
-int check_runs(int M, const int *rows, const int *offsets, int R, int E)
+// Rows sorted by expert: the sizes of what is done with them, then the operands
+int check_run_sizes(int M, int R, int E)
 {
     if (M < 1 || R < 1) return fail(TAB_ERR_BAD_ARGUMENT, "M and R must be positive");
     if (E < 1 || E > tab::kExpertsMost) return fail(TAB_ERR_BAD_ARGUMENT, "there must be 1 to %d experts, got %d", tab::kExpertsMost, E);
     if (M > kMostRows || R > kMostRows) return fail(TAB_ERR_BAD_SHAPE, "too many rows: %d and %d", M, R);
+    return TAB_OK;
+}
+
+int check_runs(int M, const int *rows, const int *offsets, int R, int E)
+{
+    TAB_CHECK(check_run_sizes(M, R, E));
     TAB_CHECK(check_int32(rows, "rows", true));
     TAB_CHECK(check_int32(offsets, "offsets"));
     if (!rows && M != R) return fail(TAB_ERR_BAD_ARGUMENT, "without rows X has the R = %d rows of Y, got %d", R, M);
+    return TAB_OK;
+}
+
+int check_experts_sizes(int M, bool listed, int R, int E, int N, int K, int out_dtype, bool full_sums, int w_bits)
+{
+    TAB_CHECK(check_run_sizes(M, R, E));
+    if (N < 1 || K < 1) return fail(TAB_ERR_BAD_ARGUMENT, "N and K must be positive");
+    const int KB = tab::blocks8(K);
+    if (N > kMostRows || KB > tab::kBlocks8Most) return fail(TAB_ERR_BAD_SHAPE, "product too large for 32-bit offsets into a tile");
+    if (w_bits == 4) TAB_CHECK(check_columns4(N));
+    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, full_sums, w_bits, R, E, N, KB);
+    if (plan.workgroups * 512 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "product too large for one launch");
+    // listed rows are read by 32-bit offsets into all of X, rows as they are sorted by those into a tile
+    if (!plan.few && listed && (unsigned long)M * (unsigned long)KB * tab::kBlock8 > 0xe0000000ul)
+        return fail(TAB_ERR_BAD_SHAPE, "X takes more than 3.5 GiB packed: too large for the 32-bit offsets of listed rows");
     return TAB_OK;
 }
 
@@ -47,15 +68,32 @@ int check_experts(int M, const int *rows, const int *offsets, int R, int E, int 
     TAB_CHECK(check_type(out_dtype, "out_dtype"));
     TAB_CHECK(check_weight_bits(w_bits, w_block_rows));
     TAB_CHECK(check_runs(M, rows, offsets, R, E));
+    return check_experts_sizes(M, rows != nullptr, R, E, N, K, out_dtype, full_sums, w_bits);
+}
+
+int check_by_expert_sizes(int M, int R, int E, int K)
+{
+    TAB_CHECK(check_run_sizes(M, R, E));
+    if (K < 1) return fail(TAB_ERR_BAD_ARGUMENT, "K must be positive");
+    if ((long)tab::run_blocks_most(R, E) * tab::blocks8(K) * 256 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "matrix too large for one launch");
+    return TAB_OK;
+}
+
+int check_grad_sizes(int R, int E, int N, int K, int out_dtype)
+{
+    TAB_CHECK(check_run_sizes(R, R, E));
     if (N < 1 || K < 1) return fail(TAB_ERR_BAD_ARGUMENT, "N and K must be positive");
-    const int KB = tab::blocks8(K);
-    if (N > kMostRows || KB > tab::kBlocks8Most) return fail(TAB_ERR_BAD_SHAPE, "product too large for 32-bit offsets into a tile");
-    if (w_bits == 4) TAB_CHECK(check_columns4(N));
-    const tab::ExpertsPlan plan = tab::experts_plan(out_dtype, full_sums, w_bits, R, E, N, KB);
-    if (plan.workgroups * 512 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "product too large for one launch");
-    // listed rows are read by 32-bit offsets into all of X, rows as they are sorted by those into a tile
-    if (!plan.few && rows && (unsigned long)M * (unsigned long)KB * tab::kBlock8 > 0xe0000000ul)
-        return fail(TAB_ERR_BAD_SHAPE, "X takes more than 3.5 GiB packed: too large for the 32-bit offsets of listed rows");
+    if (N > kMostRows || K > kMostRows || tab::run_blocks_most(R, E) > tab::kBlocks8Most)
+        return fail(TAB_ERR_BAD_SHAPE, "gradients of weights from more blocks of rows than %d: too large for 32-bit offsets into a tile", tab::kBlocks8Most);
+    if (tab::experts_grad_workgroups(out_dtype, R, E, N, K) * 512 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "product too large for one launch");
+    return TAB_OK;
+}
+
+int check_combine_sizes(int M, int k, int R, int D)
+{
+    if (M < 1 || k < 1 || R < 1 || D < 1) return fail(TAB_ERR_BAD_ARGUMENT, "M, k, R and D must be positive");
+    if ((long)M * k > kMostRows || R > kMostRows || D > kMostRows || (long)M * ((D + 7) / 8) > kMostRows || (long)M * 256 > kMostThreads)
+        return fail(TAB_ERR_BAD_SHAPE, "too large for one launch");
     return TAB_OK;
 }
 
@@ -199,8 +237,7 @@ int tab_quantize8_by_expert(const void *dev_X, int dtype, long ldx, int M, const
     TAB_CHECK(check_type(dtype, "dtype"));
     TAB_CHECK(check_format(format));
     TAB_CHECK(check_runs(M, dev_rows, dev_offsets, R, E));
-    if (K < 1) return fail(TAB_ERR_BAD_ARGUMENT, "K must be positive");
-    if ((long)tab::run_blocks_most(R, E) * tab::blocks8(K) * 256 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "matrix too large for one launch");
+    TAB_CHECK(check_by_expert_sizes(M, R, E, K));
     TAB_CHECK(check_rows(dev_X, dtype, M, K, ldx, "X"));
     if (dev_Q || dev_S) TAB_CHECK(check_packed(dev_Q, dev_S, "Q or S"));
     TAB_CHECK(check_packed(dev_QT, dev_ST, "QT or ST"));
@@ -269,24 +306,36 @@ int tab_experts_grad_weight(const void *dev_QD, int d_format, const void *dev_SD
     TAB_CHECK(check_format(d_format));
     TAB_CHECK(check_type(out_dtype, "out_dtype"));
     TAB_CHECK(check_runs(R, nullptr, dev_offsets, R, E));
-    if (N < 1 || K < 1) return fail(TAB_ERR_BAD_ARGUMENT, "N and K must be positive");
-    const int KB = tab::run_blocks_most(R, E);
-    if (N > kMostRows || K > kMostRows || KB > tab::kBlocks8Most) return fail(TAB_ERR_BAD_SHAPE, "product too large for 32-bit offsets into a tile");
-    if (tab::experts_grad_workgroups(out_dtype, R, E, N, K) * 512 > kMostThreads) return fail(TAB_ERR_BAD_SHAPE, "product too large for one launch");
+    TAB_CHECK(check_grad_sizes(R, E, N, K, out_dtype));
     TAB_CHECK(check_packed(dev_QD, dev_SD, "QD or SD"));
     TAB_CHECK(check_packed(dev_QX, dev_SX, "QX or SX"));
     TAB_CHECK(check_rows(dev_dW, out_dtype, 1, K, K, "dW"));
     const tab::ExpertsGradArgs a = {static_cast<const uint8_t *>(dev_QD), static_cast<const uint8_t *>(dev_SD), static_cast<const uint8_t *>(dev_QX),
-                                    static_cast<const uint8_t *>(dev_SX), dev_dW, dev_offsets, R, E, N, K, KB};
+                                    static_cast<const uint8_t *>(dev_SX), dev_dW, dev_offsets, R, E, N, K, tab::run_blocks_most(R, E)};
     const hipError_t e = tab::launch_experts_grad(out_dtype, d_format, a, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? TAB_OK : device_fail(e, "experts gradient launch");
 }
 
+int tab_experts_check_gradients(int x_dtype, int w_dtype, int M, int k, int R, int E, int N, int K, int of_x, int of_w)
+{
+    TAB_CHECK(check_type(x_dtype, "x_dtype"));
+    TAB_CHECK(check_type(w_dtype, "w_dtype"));
+    if (of_w) {
+        TAB_CHECK(check_by_expert_sizes(R, R, E, N));
+        TAB_CHECK(check_grad_sizes(R, E, N, K, w_dtype));
+    }
+    if (of_x) {
+        // dY, its rows sorted, times the transposed weights; the rows of a token added up from fp32
+        if (!of_w) TAB_CHECK(check_quantize(R, N, 1, false));
+        TAB_CHECK(check_experts_sizes(R, false, R, E, K, N, k ? TAB_F32 : x_dtype, x_dtype == TAB_F32, 8));
+        if (k) TAB_CHECK(check_combine_sizes(M, k, R, K));
+    }
+    return TAB_OK;
+}
+
 static int check_combine(int M, int k, int R, int D, const int *places, const float *weights)
 {
-    if (M < 1 || k < 1 || R < 1 || D < 1) return fail(TAB_ERR_BAD_ARGUMENT, "M, k, R and D must be positive");
-    if ((long)M * k > kMostRows || R > kMostRows || D > kMostRows || (long)M * ((D + 7) / 8) > kMostRows || (long)M * 256 > kMostThreads)
-        return fail(TAB_ERR_BAD_SHAPE, "too large for one launch");
+    TAB_CHECK(check_combine_sizes(M, k, R, D));
     TAB_CHECK(check_int32(places, "places"));
     return check_int32(weights, "weights", true);
 }

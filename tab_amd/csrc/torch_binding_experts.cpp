@@ -341,6 +341,8 @@ struct ExpertsFunction : torch::autograd::Function<ExpertsFunction> {
         const Tensor x2 = matrix(x), w2 = w.contiguous();
         const int K = as_size(x2.size(1), "columns of x"), N = as_size(w.size(1), "rows of an expert's weight");
         const Sizes s(x, rows, places, offsets, w.size(0), gather);
+        // what the backward pass would refuse is refused here
+        check_status(tab_experts_check_gradients(dtype_code(x.scalar_type(), "x"), dtype_code(w.scalar_type(), "w"), s.M, gather ? s.k : 0, s.R, s.E, N, K, need_dx, need_dw));
         const auto from = gather ? OptionalTensor(rows) : c10::nullopt;
         Tensor q, sx, qt, st;
         if (need_dw) {

@@ -223,7 +223,8 @@ def route(logits, k, normalize=True):
 def experts_linear8(x, w, routing, gather=True, grad_format=E4M3):
     """Rows sorted by expert times their expert's weight w (E, N, K) in 8-bit numbers: y (rows, N) of x's type, zeros in the rows of no expert.
     x (..., K) holds the routing's tokens, or with gather=False its sorted rows, as a product before left them.  Differentiable in x and w as linear8 is: the
-    rows of a token are added up in fp32, blocks of 128 rows under one scale belong to one expert.  w is packed anew in every call: for weights that stay,
+    rows of a token are added up in fp32, blocks of 128 rows under one scale belong to one expert.  Sizes whose gradients would be
+    refused are refused here already.  w is packed anew in every call: for weights that stay,
     see PackedExperts."""
     return _C.experts_linear8(x, w, routing.rows, routing.places, routing.offsets, bool(gather), int(grad_format))
 

@@ -290,3 +290,27 @@ def test_sorted_rows_have_no_bound_that_listed_ones_have():
             _refuses(lib.tab_experts_linear(P, 1, K, R, rows, P, P, P, bits, 128, R, 8, N, K, P, None, 0, None), message, code)
     _refuses(lib.tab_experts_linear_packed(P, 0, P, R, P, P, P, P, 8, 128, R, 8, N, K, None, 1, 0, None, 0, None), "3.5 GiB", -2)
     _refuses(lib.tab_experts_linear_packed(P, 0, P, R, None, P, P, P, 8, 128, R, 8, N, K, None, 1, 0, None, 0, None), "null device pointer: Y")
+
+
+@pytest.mark.parametrize("dtype,w_dtype", [(0, 0), (1, 1), (2, 0), (1, 0)])
+@pytest.mark.parametrize("M,k,E,N,K", [(100, 2, 4, 64, 64), (128 * 65536, 1, 1, 8, 8), (128 * 65535, 1, 1, 8, 8), (128 * 65535, 1, 2, 8, 8), (1 << 24, 1, 1, 8, 8), ((1 << 24) - 1, 1, 1, 8, 8),
+                                       (1 << 23, 2, 3, 8, 8), (1 << 23, 0, 3, 8, 8), (1 << 20, 1, 3, 65536, 8), (1 << 20, 0, 3, 8, 65536), (1 << 14, 2, 1024, 1 << 15, 1 << 16),
+                                       (1 << 22, 4, 7, 20000, 16), (500, 2, 3, 128 * 65536, 8), (1000, 8, 1024, 8192, 8192)])
+def test_training_is_refused_where_its_gradients_would_be(M, k, E, N, K, dtype, w_dtype):
+    """The check agrees with the calls that the backward pass makes (which refuse a null pointer once the sizes are accepted)."""
+    lib, R = _capi.load(), M * max(k, 1)
+
+    def taken(status):
+        if status == -2:
+            return False
+        assert status == -1 and "null device pointer" in lib.tab_last_error().decode()
+        return True
+
+    by_expert = taken(lib.tab_quantize8_by_expert(None, dtype, N, R, None, P, R, E, N, 0, None, None, P, P, None))
+    of_w = by_expert and taken(lib.tab_experts_grad_weight(None, 0, P, P, P, P, R, E, N, K, P, w_dtype, None))
+    product = taken(lib.tab_experts_linear_packed(None, 0, P, R, None, P, P, P, 8, 128, R, E, K, N, P, 0 if k else dtype, dtype == 0, P, 1 << 60, None))
+    product = product and (k == 0 or taken(lib.tab_combine(P, 0, None, None, M, k, R, K, P, dtype, None)))
+    rows = taken(lib.tab_quantize8(None, dtype, R, N, N, 1, 0, P, P, None, None, None))
+    for want_x, want_w, want in ((0, 0, True), (0, 1, of_w), (1, 0, rows and product), (1, 1, of_w and product)):
+        status = lib.tab_experts_check_gradients(dtype, w_dtype, M, k, R, E, N, K, want_x, want_w)
+        assert status == (0 if want else -2), (want_x, want_w)

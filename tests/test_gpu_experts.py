@@ -472,3 +472,16 @@ def test_training_past_32_bits():
             e = next(e for e in range(E) if at[e] <= p < at[e + 1])
             want = want + dy[p].double().cpu() @ w64[e]
         assert torch.equal(dx[t].cpu(), want.to(torch.bfloat16)), f"gradient of token {t}"
+
+
+def test_training_is_refused_before_its_first_product():
+    """More rows than the gradients of the weights may have: the forward pass says so where a gradient of them is wanted, and runs where none is."""
+    M, E, N, K = 128 * 65535 + 1, 1, 8, 8
+    x, w = torch.ones((M, K), device="cuda", dtype=torch.bfloat16), torch.ones((E, N, K), device="cuda", dtype=torch.bfloat16)
+    routing = tab_nn.route(torch.zeros((M, E), device="cuda"), 1)
+    with pytest.raises(tab_amd.TabError, match="blocks of rows"):
+        tab_nn.experts_linear8(x, w.requires_grad_(), routing)
+    y = tab_nn.experts_linear8(x.requires_grad_(), w.detach(), routing)
+    assert (y == K).all()
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert (dx == N).all()
