@@ -116,13 +116,13 @@ inline void no_tangent(std::initializer_list<const Tensor *> tensors)
 {
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
     for (const Tensor *t : tensors)
-        TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), "the 8-bit layers and the norms have no derivatives in forward mode (an input has a tangent)");
+        TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), "this layer has no derivatives in forward mode (an input has a tangent)");
 }
 
 // The kernels' gradients are no graph: asking for their derivatives is an error, not a zero.
 inline void no_second_derivative(const torch::autograd::variable_list &grads)
 {
-    TORCH_CHECK(!at::GradMode::is_enabled(), "the 8-bit layers and the norms have no second derivatives (create_graph)");
+    TORCH_CHECK(!at::GradMode::is_enabled(), "this layer has no second derivatives (create_graph)");
     for (const Tensor &g : grads) no_tangent({&g});
 }
 

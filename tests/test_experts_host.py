@@ -314,3 +314,15 @@ def test_training_is_refused_where_its_gradients_would_be(M, k, E, N, K, dtype, 
     for want_x, want_w, want in ((0, 0, True), (0, 1, of_w), (1, 0, rows and product), (1, 1, of_w and product)):
         status = lib.tab_experts_check_gradients(dtype, w_dtype, M, k, R, E, N, K, want_x, want_w)
         assert status == (0 if want else -2), (want_x, want_w)
+
+
+def test_refusals_of_derivatives_name_no_other_layer():
+    """A router or a 4-bit layer that refuses a tangent does not speak of 8-bit layers or norms."""
+    i = torch.zeros(8, dtype=torch.int32)
+    routing = tab_nn.Routing(torch.zeros(4, 2), i.view(4, 2), i, i.view(4, 2), torch.zeros(4, dtype=torch.int32))
+    with forward_ad.dual_level():
+        dual = lambda *shape: forward_ad.make_dual(torch.ones(shape), torch.ones(shape))  # noqa: E731
+        for call in (lambda: tab_nn.route(dual(4, 3), 2), lambda: tab_nn.combine(dual(8, 5), routing)):
+            with pytest.raises(RuntimeError) as error:
+                call()
+            assert "forward mode" in str(error.value) and "8-bit" not in str(error.value) and "norms" not in str(error.value)
