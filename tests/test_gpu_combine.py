@@ -111,3 +111,30 @@ def test_gradients_are_differences():
             d = torch.zeros_like(w)
             d[t, j] = 1
             assert f(y, w + d) - f(y, w - d) == 2 * float(dw[t, j])
+
+
+@types
+@pytest.mark.parametrize("D", [90, 700])
+def test_gradients_leave_out_places_that_are_no_rows(D, dtype):
+    """Rows that are some choice's place, once each, have their gradient, weights whose place is no row have none; other rows are nobody's."""
+    M, k, R = 50, 3, 130
+    g = torch.Generator("cpu").manual_seed(5)
+    places = torch.randperm(R, generator=g)[:120].int()
+    places = torch.cat((places, torch.tensor([-1, R, R + 4, 1 << 30, -7, -(1 << 31), 0x7fffffff, -1, -1, R] * 3, dtype=torch.int32)))[torch.randperm(M * k, generator=g)].view(M, k)
+    there = (places >= 0) & (places < R)
+    assert int(there.sum()) == 120
+    y, w, dout = _rand((R, D), 3).to(dtype), _rand((M, k), 4), _rand((M, D), 6).to(dtype)
+    dy, dw = tab_amd.CombineBackward(dout.cuda(), y.cuda(), places.cuda(), w.cuda(), None, M, k, R, D)
+    at = places[there].long()
+    want = (w.double()[..., None] * dout.double()[:, None])[there]
+    ref.check(dy.cpu()[at], want, want.abs(), 1, False, "dy")
+    products = torch.where(there[..., None], dout.double()[:, None] * y.double()[torch.where(there, places, 0).long()], 0.0)
+    ref.check(dw, products.sum(dim=2), products.abs().sum(dim=2), D, False, "dweights")
+    assert not dw.cpu()[~there].any()
+    # with a number of rows that are used, those behind it are zeros, whoever's place they are not
+    inside = torch.where(places < 100, places, -1)
+    dy, _ = tab_amd.CombineBackward(dout.cuda(), y.cuda(), inside.cuda(), w.cuda(), torch.tensor([0, 100], dtype=torch.int32, device="cuda"), M, k, R, D)
+    assert not dy[100:].any()
+    on = (inside >= 0)
+    want = (w.double()[..., None] * dout.double()[:, None])[on]
+    ref.check(dy.cpu()[inside[on].long()], want, want.abs(), 1, False, "dy of the rows that are used")
