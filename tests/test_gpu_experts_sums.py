@@ -145,3 +145,101 @@ def test_a_token_does_not_depend_on_its_batch(rows, bits, dtype):
             assert torch.equal(block(x[t:t + 1])[0], got[t]), t
         some = torch.arange(0, rows, 3, device="cuda")
         assert torch.equal(block(x[some]), got[some])
+
+
+# ---- operands that were packed elsewhere: scale bytes that the quantizers do not give -----------------------------------------------------
+
+
+def _packed8(R, K, seed, byte, block_rows=1):
+    """Numbers of 4 to 448 (of 2^-7 to 7/8 under bytes from 253 on) under one scale byte."""
+    x = _rand((R, K), seed)
+    x = torch.sign(x) * (x.abs() * 40).clamp(4, 448)
+    q = torch.zeros(R, ref8.blocks(K) * 128)
+    q[:, :K] = ref8.nearest8(x.double(), 0).float() / (512 if byte >= 253 else 1)
+    s = torch.full((ref8.blocks(K), -(-R // block_rows)), byte, dtype=torch.uint8)
+    return q.to(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu)
+
+
+def _packed4(R, K, seed, byte):
+    """Numbers 4 and 6 (1/2 under bytes from 253 on) of either sign under one scale byte."""
+    g = torch.Generator("cpu").manual_seed(seed)
+    code = torch.randint(6, 8, (R, K), generator=g) if byte < 253 else torch.ones((R, K), dtype=torch.int64)
+    code = code + 8 * torch.randint(0, 2, (R, K), generator=g)
+    c = torch.zeros((R, ref8.blocks(K) * 128), dtype=torch.int64)
+    c[:, :K] = code
+    q = (c[:, 0::2] | c[:, 1::2] << 4).to(torch.uint8).view(torch.float4_e2m1fn_x2)
+    return q, torch.full((ref8.blocks(K), R, 4), byte, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+
+
+SCALES = [(0, 254), (254, 0), (0, 127), (127, 0), (1, 253), (240, 10)]
+outputs = pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+
+
+def _check_scales(y, a, b, out):
+    """As for other products; a sum below 2^-126 may count as zero."""
+    want, magnitudes = a @ b.t().contiguous(), a.abs() @ b.abs().t().contiguous()
+    bound = (a.shape[1] * 2.0 ** -24 + (0 if out == torch.float32 else 2.0 ** -10)) * magnitudes + ref.UNIT[out] * (1 + 2.0 ** -10) * want.abs() + 2.0 ** -126
+    off = (y.cpu().double() - want).abs()
+    assert off.shape == bound.shape and bool((off <= bound).all()), float((off / bound).max())
+
+
+@outputs
+@pytest.mark.parametrize("M,N,K", [(1, 40, 300), (20, 40, 300), (600, 72, 300), (700, 8299, 130), (2970, 643, 130)])
+@pytest.mark.parametrize("x_byte,w_byte", SCALES)
+def test_extreme_scales_of_4_bit_weights(x_byte, w_byte, M, N, K, out):
+    """2^(byte - 127) for every byte below 255, also 2^-127.  No number is below 2^-126 after its scale, and none above fp32's largest."""
+    QX, SX = _packed8(M, K, 1, x_byte)
+    QW, SW = _packed4(N, K, 2, w_byte)
+    y = tab_amd.Linear4Packed(QX.cuda(), SX.cuda(), QW.cuda(), SW.cuda(), M, N, K, out)
+    _check_scales(y, ref8.unpack(QX, SX, 1), ref.unpack4(QW, SW), out)
+
+
+@outputs
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("R,E,N,K", [(12, 3, 40, 300), (600, 2, 300, 300), (3000, 2, 643, 130)])
+@pytest.mark.parametrize("x_byte,w_byte", SCALES + [(127, 255), (255, 127)])
+def test_extreme_scales_by_expert(x_byte, w_byte, R, E, N, K, bits, out):
+    """The same, and byte 255, which is NaN: one expert's weight has it, or one row of x."""
+    x_nan, w_nan = x_byte == 255, w_byte == 255
+    QX, SX = _packed8(R, K, 3, 127 if x_nan else x_byte)
+    packed = [_packed4(N, K, 4 + e, 127 if w_nan else w_byte) if bits == 4 else _packed8(N, K, 4 + e, 127 if w_nan else w_byte, 128) for e in range(E)]
+    b = [ref.unpack4(*p) if bits == 4 else ref8.unpack(*p, 128) for p in packed]
+    QW, SW = (torch.stack([p[i].view(torch.uint8) for p in packed]).view(packed[0][i].dtype) for i in (0, 1))
+    a = ref8.unpack(QX, SX, 1)
+    if x_nan:
+        SX.view(torch.uint8)[0, R // 2] = 255
+    if w_nan:
+        SW.view(torch.uint8)[E - 1] = 255
+    offsets = torch.tensor([0] + [R * (e + 1) // E for e in range(E)], dtype=torch.int32)
+    y = tab_amd.ExpertsLinearPacked(QX.cuda(), SX.cuda(), None, offsets.cuda(), QW.cuda(), SW.cuda(), R, R, E, N, K, out).cpu()
+    nan = torch.zeros((R, N), dtype=torch.bool)
+    if x_nan:
+        nan[R // 2] = True
+    if w_nan:
+        nan[int(offsets[E - 1]):] = True
+    assert torch.equal(torch.isnan(y), nan)
+    for e, first, end in ref.runs(offsets):
+        rows = [r for r in range(first, end) if not nan[r].any()]
+        if rows:
+            _check_scales(y[rows], a[rows], b[e], out)
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,E", [(1, 1), (5, 4), (700, 3), (200, 128)])
+def test_a_batch_of_padding_alone(rows, E, dtype, normalize):
+    """Every expert closed to every token: no rows, zeros out, and zeros for all gradients."""
+    N, K, k = 140, 300, min(E, 2)
+    x, w = _rand((rows, K), 1).to(dtype).cuda().requires_grad_(), _rand((E, N, K), 2).to(dtype).cuda().requires_grad_()
+    logits = torch.full((rows, E), -float("inf"), device="cuda", dtype=dtype, requires_grad=True)
+    routing = tab_nn.route(logits, k, normalize)
+    assert not routing.offsets.any() and (routing.rows == -1).all() and not routing.weights.any()
+    y = tab_nn.experts_linear8(x, w, routing)
+    out = tab_nn.combine(y, routing)
+    assert y.shape == (rows * k, N) and not y.any() and not out.any()
+    for g in torch.autograd.grad(out, (x, w, logits), torch.ones_like(out)):
+        assert not g.any()
+    with torch.no_grad():
+        for bits in (8, 4):
+            layer = tab_nn.PackedExperts.from_float(w, bits)
+            assert not layer(x.detach(), routing).any() and not layer(_rand((rows * k, K), 3).to(dtype).cuda(), routing, gather=False).any()
