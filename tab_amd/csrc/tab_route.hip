@@ -245,57 +245,56 @@ struct RouteGradParams {
     int M, E, k, normalize;
 };
 
-// A wave takes a token (or, past 2^26 of them, a few); its choices' weights and gradients go from lane to lane
+// A wave takes a token; its choices' weights and gradients go from lane to lane
 template <int DTYPE, int V> __global__ __launch_bounds__(256) void route_grad(const RouteGradParams p)
 {
     using T = typename Element<DTYPE>::type;
-    const int lane = threadIdx.x % 64;
-    for (long token = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)threadIdx.x / 64); token < p.M; token += 4l * gridDim.x) {
-        const long at = token * p.k + lane;
-        const int expert = lane < p.k ? p.experts[at] : -1;
-        const bool open = expert >= 0;
-        const float w = open ? p.weights[at] : 0.f, g = open ? p.dweights[at] : 0.f, mean = wave_sum(w * g);
-        float chosen[V], part[V];  // the gradient of the expert's weight; what the expert's softmax is
-        if (p.normalize) {
+    const int lane = threadIdx.x % 64, token = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)threadIdx.x / 64);
+    if (token >= p.M) return;
+    const long at = (long)token * p.k + lane;
+    const int expert = lane < p.k ? p.experts[at] : -1;
+    const bool open = expert >= 0;
+    const float w = open ? p.weights[at] : 0.f, g = open ? p.dweights[at] : 0.f, mean = wave_sum(w * g);
+    float chosen[V], part[V];  // the gradient of the expert's weight; what the expert's softmax is
+    if (p.normalize) {
 #pragma unroll
-            for (int i = 0; i < V; i++) chosen[i] = part[i] = 0.f;
-        } else {
-            const T *const row = static_cast<const T *>(p.logits) + token * p.ld;
-            uint32_t most = 0;
-            float sum = 0.f;
+        for (int i = 0; i < V; i++) chosen[i] = part[i] = 0.f;
+    } else {
+        const T *const row = static_cast<const T *>(p.logits) + (long)token * p.ld;
+        uint32_t most = 0;
+        float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                part[i] = i * 64 + lane < p.E ? (float)row[i * 64 + lane] : -__builtin_inff();
-                most = max(most, order_code(part[i]));
-                chosen[i] = 0.f;
-            }
-            most = wave_max(most);
-            const float top = value_of(most);
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                part[i] = most ? expf(part[i] - top) : 0.f;
-                sum += part[i];
-            }
-            sum = wave_sum(sum);
-#pragma unroll
-            for (int i = 0; i < V; i++) part[i] = most ? part[i] / sum : 0.f;
+        for (int i = 0; i < V; i++) {
+            part[i] = i * 64 + lane < p.E ? (float)row[i * 64 + lane] : -__builtin_inff();
+            most = max(most, order_code(part[i]));
+            chosen[i] = 0.f;
         }
-        for (int j = 0; j < p.k; j++) {
-            const int e = __builtin_amdgcn_readlane(expert, j);
-            if (e < 0) break;
-            const float gj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), j)), wj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
+        most = wave_max(most);
+        const float top = value_of(most);
 #pragma unroll
-            for (int i = 0; i < V; i++)
-                if (e == i * 64 + lane) {
-                    chosen[i] = gj;
-                    if (p.normalize) part[i] = wj;
-                }
+        for (int i = 0; i < V; i++) {
+            part[i] = most ? expf(part[i] - top) : 0.f;
+            sum += part[i];
         }
-        T *const out = static_cast<T *>(p.dlogits) + token * p.E;
+        sum = wave_sum(sum);
+#pragma unroll
+        for (int i = 0; i < V; i++) part[i] = most ? part[i] / sum : 0.f;
+    }
+    for (int j = 0; j < p.k; j++) {
+        const int e = __builtin_amdgcn_readlane(expert, j);
+        if (e < 0) break;
+        const float gj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), j)), wj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
 #pragma unroll
         for (int i = 0; i < V; i++)
-            if (i * 64 + lane < p.E) out[i * 64 + lane] = (T)(part[i] * (chosen[i] - mean));
+            if (e == i * 64 + lane) {
+                chosen[i] = gj;
+                if (p.normalize) part[i] = wj;
+            }
     }
+    T *const out = static_cast<T *>(p.dlogits) + (long)token * p.E;
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        if (i * 64 + lane < p.E) out[i * 64 + lane] = (T)(part[i] * (chosen[i] - mean));
 }
 
 // One workgroup for few tokens; else at most 256, so that each can add the others' numbers up
@@ -322,12 +321,9 @@ template <int DTYPE> hipError_t launch_choose(const RouteParams &p, hipStream_t 
            : p.E <= 512 ? launch_v<DTYPE, 8>(p, stream) : launch_v<DTYPE, 16>(p, stream);
 }
 
-constexpr long kGradWorkgroups = 0xffffff;  // a launch may hold 2^32 threads
-
 template <int DTYPE> hipError_t launch_grad(const RouteGradParams &p, hipStream_t stream)
 {
-    const long fours = ((long)p.M + 3) / 4;
-    const unsigned n = fours < kGradWorkgroups ? (unsigned)fours : (unsigned)kGradWorkgroups;
+    const unsigned n = (unsigned)(((long)p.M + 3) / 4);
     if (p.E <= 64) route_grad<DTYPE, 1><<<n, 256, 0, stream>>>(p);
     else if (p.E <= 128) route_grad<DTYPE, 2><<<n, 256, 0, stream>>>(p);
     else if (p.E <= 256) route_grad<DTYPE, 4><<<n, 256, 0, stream>>>(p);
@@ -348,8 +344,17 @@ hipError_t launch_route(int dtype, const RouteArgs &a, hipStream_t stream)
 
 hipError_t launch_route_grad(int dtype, const RouteGradArgs &a, hipStream_t stream)
 {
-    const RouteGradParams p = {a.dweights, a.weights, a.experts, a.logits, a.dlogits, a.ld, a.M, a.E, a.k, a.normalize};
-    return dtype == 0 ? launch_grad<0>(p, stream) : dtype == 1 ? launch_grad<1>(p, stream) : launch_grad<2>(p, stream);
+    // a launch may hold 2^32 threads, 64 a token (a loop over tokens inside the kernel took 4-9 % longer)
+    constexpr long kMost = 1l << 25;
+    const long element = dtype == 0 ? 4 : 2;
+    for (long first = 0; first < a.M; first += kMost) {
+        const long M = a.M - first < kMost ? a.M - first : kMost, choice = first * a.k;
+        const RouteGradParams p = {a.dweights + choice, a.weights + choice, a.experts + choice, static_cast<const char *>(a.logits) + first * a.ld * element,
+                                   static_cast<char *>(a.dlogits) + first * a.E * element, a.ld, (int)M, a.E, a.k, a.normalize};
+        const hipError_t e = dtype == 0 ? launch_grad<0>(p, stream) : dtype == 1 ? launch_grad<1>(p, stream) : launch_grad<2>(p, stream);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace tab
