@@ -4,8 +4,9 @@
 // 16-bit outputs: v_mfma_scale_f32_16x16x128_f8f6f4.  One instruction is a 16 x 16 tile over one block of K, and it takes the E8M0 bytes of its
 // 16 rows and 16 columns as operands, so the scales cost no vector instruction and the sums stay in one set of fp32 accumulators.  Inside
 // the instruction, products of eight neighbours in K are aligned to the largest of them and keep 13 bits below it (measured): 1.5e-5 of the
-// output's size for normal operands, far below the 2^-8 or 2^-11 of the output's own rounding, but not what an fp32 output is for.  (512 x 4096 x 4096: 1.2 % of
-// the bf16 outputs are the other neighbour of what the fp32 output rounds to; off the fp32 output by 0.0016633 of its size instead of 0.0016632.)
+// output's size for normal operands, far below the 2^-8 or 2^-11 of the output's own rounding, but not what an fp32 output is for.  (Outputs that are the other
+// neighbour of what full sums round to: 0.5-1.7 % in bf16, 3-7 % in fp16.  Off the exact product, of its size: 512 x 4096 x 4096 bf16 0.0016633 instead of 0.0016632,
+// K = 776 fp16 0.0002077 instead of 0.0002070.  The same call gives the same bits.)
 // fp32 outputs (EXACT): the numbers times their scales are bf16 numbers exactly (4 of 8 significant bits, the exponent range of fp32), made by one
 // conversion of two numbers, and v_mfma_f32_16x16x32_bf16 multiplies them at half the rate with full fp32 sums.  A number below 2^-126 may
 // count as zero there.
@@ -745,8 +746,10 @@ struct Plan8 {
 
 // The tile and the parts that K is cut into: the least of what a launch takes by the busiest CU's work.  A step of one of the tiles that a CU holds at
 // once takes `alone` us (latency) or, of all its tiles, `among` (throughput), a tile's way out `out`; parts are written in fp32, read and added
-// up by a launch of their own.  Constants fitted to every (tile, parts) of 60 products of 33 .. 16384 rows, 64 .. 8192 columns and K on an MI355X;
-// what the rule picks takes 0.6 % (16-bit output) and 0.3 % (fp32) longer than the best of them in the mean, at most 14 % (40 x 64 x 8192).
+// up by a launch of their own.  Constants fitted to every (tile, parts) of 60 products of 33 .. 16384 rows, 64 .. 8192 columns and K on an MI355X, with weights of 8
+// bits and before outputs left past the caches; what they pick now, over the best, on 132 other products, mean and worst:
+//   8 bits   500 and more rows 1.2 %, 13 % (5423 x 394 over 538)   34 .. 550 rows 4.3 %, 53 % (99 x 78 over 7912)   fp32 1.4 %, 12 % (2749 x 468 over 133)
+//   4 bits                     2.9 %, 24 % (the same)                             2.4 %, 16 %                            1.8 %, 11 %
 struct TileTimes { int rows, columns, held; double alone, among, out; };
 // The same of tiles over experts (16-bit sums, and full ones); their ways out are shorter, past the caches
 constexpr TileTimes kExpertTiles[] = {{64, 64, 3, 0.092, 0.165, 0.46}, {64, 128, 2, 0.237, 0.235, 0.725}, {128, 128, 2, 0.509, 0.41, 0.923}, {256, 256, 1, 0.96, 0.945, 2.854}};
@@ -781,7 +784,8 @@ inline Plan8 plan8(int out, int M, int N, int KB)
 
 // Whether Y (`count` elements of type `out` in rows of N) is written past the caches: from 16 MB on, where its rows are whole cache lines, which a wave then
 // writes at once.  What is smaller is read from the caches by the next kernel.  16384 x 2048 bf16, two tiles a CU: the way out 21 -> 11 us.  With the quantizer
-// that reads Y behind it, us through / past the caches: 1024 x 4096 29.6 / 31.4, 2048 x 2048 20.4 / 20.2, 4096 x 2048 43.9 / 41.7, 8192 x 8192 over 8192 429 / 399.
+// that reads Y behind it, in a replayed graph, us through / past the caches: 1024 x 4096 over 4096 27.5 / 27.3, 2048 x 2048 over 2048 19.4 / 19.2, 4096 x 2048 over 4096
+// 40.2 / 39.1, 4096 x 4096 over 2048 40.9 / 41.5, 8192 x 8192 over 8192 423 / 415.
 inline int streamed(int out, const void *y, long count, int N)
 {
     const long bytes = out == 0 ? 4 : 2;
